@@ -349,7 +349,7 @@ def work(case):
     heads, kv_heads, dim = case["heads"], case["kv_heads"], case["dim"]
     held = case["bits"] // 8
     if case["kind"] == "append":
-        return dict(bytes=rows * dim * (4 * heads + 2 * kv_heads * (2 + held)), flops=rows * 3 * 2 * case["pairs"] * (heads + kv_heads))
+        return dict(bytes=rows * dim * ((4 * heads if case["pairs"] else 0) + 2 * kv_heads * (2 + held)), flops=rows * 3 * 2 * case["pairs"] * (heads + kv_heads))
     keys = pairs = 0
     for n, m in zip(new, length):
         lo = max(0, m - n - case["window"] + 1) if case["window"] else 0
