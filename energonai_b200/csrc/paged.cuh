@@ -1,0 +1,65 @@
+// What the kernels over paged caches share: the layout of a packed batch, conversions between e4m3 codes and
+// fp16 / fp32, and the limits that every page number passes before it becomes an address.
+#pragma once
+
+#include "common.cuh"
+
+namespace eb {
+namespace {
+
+// Rows starts[b] .. starts[b + 1] of a packed batch are the last tokens of sequence b, which has lengths[b] positions
+// with them; position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].  Nothing that the
+// device arrays hold leads outside the tensors: rows are bounded by `rows`, pages by `pages`, table columns by
+// `table_cols`; what lies outside is left out.
+struct PagedBatch {
+  const int *tables, *starts, *lengths;
+  long long table_ld;
+  int batch, rows, table_cols, pages, page_shift;
+};
+
+struct PagedRows {
+  int row0, count, past, length;       // first row, rows, positions in front of them, positions in all
+};
+__device__ __forceinline__ PagedRows paged_rows(const PagedBatch &p, int b) {
+  PagedRows r;
+  r.row0 = max(p.starts[b], 0);
+  r.count = min(p.starts[b + 1], p.rows) - r.row0;
+  r.length = p.lengths[b];
+  r.past = r.length - (p.starts[b + 1] - p.starts[b]);
+  if (r.past < 0 || r.count < 0) r.count = 0;          // (no such sequence)
+  return r;
+}
+__device__ __forceinline__ int paged_page(const PagedBatch &p, int b, int at) {   // page of table entry `at`, or -1
+  if (at < 0 || at >= p.table_cols) return -1;
+  const int id = p.tables[(long long)b * p.table_ld + at];
+  return id >= 0 && id < p.pages ? id : -1;
+}
+
+// e4m3 has a subset of fp16's values; both conversions are exact or round to nearest even.
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {             // (the lower 16 bits)
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)codes));
+  return r;
+}
+__device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Host side of the checks that all entry points make of a packed batch.
+inline int paged_check(const char *what, PagedBatch &p, const int32_t *tables, long long table_ld, const int32_t *starts, const int32_t *lengths, int batch,
+                       int rows, int table_cols, int pages, int page_size) {
+  EB_REQUIRE(tables && starts && lengths, "%s: null pointer", what);
+  EB_REQUIRE(batch > 0 && batch <= 65535 && rows > 0 && table_cols > 0 && table_ld >= table_cols && pages > 0, "%s: bad sizes", what);
+  EB_REQUIRE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "%s: pages of %d positions not supported (16, 32, 64 or 128)", what,
+             page_size);
+  EB_REQUIRE((long long)table_cols * page_size < (1ll << 30), "%s: a table addresses at most 2^30 positions", what);
+  p.tables = tables; p.table_ld = table_ld; p.starts = starts; p.lengths = lengths; p.batch = batch; p.rows = rows; p.table_cols = table_cols;
+  p.pages = pages;
+  p.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
+  return EB_OK;
+}
+
+}  // namespace
+}  // namespace eb

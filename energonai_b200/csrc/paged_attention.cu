@@ -1,0 +1,531 @@
+// Attention of few new tokens per sequence over a paged cache (generation steps, draft tokens): one pass over the keys and
+// values, 16-bit or e4m3 codes with a scale for each page and head.  Bound by memory: a cached byte is read
+// once per key / value head and serves all query heads that share it.
+//
+// Both products are mma.sync tiles with the cached rows on the long side: S^T = K Q^T (16 keys x 8 query rows) and
+// O^T += V^T P^T (16 dimensions x 8 query rows), so that 8 query rows (token, head of the group) fill a tile.  A
+// warp takes 16 keys at a time, straight from global memory into the fragments of its lanes: the contraction of S
+// runs over dimensions in any order and that of O over keys in any order, so each lane loads 16 bytes where they lie
+// and the queries are laid out to match; 8 lanes cover a row, every sector is used, and neither
+// shared memory nor a barrier stands between memory and the tensor core.  P^T comes from S^T by an 8 x 8 transpose
+// within the warp.  The next keys are requested as soon as the scores are done, the next values behind the second
+// product; 12 to 16 warps per multiprocessor keep 50 KB and more in flight.
+//
+// e4m3 codes become fp16 (exact), whatever the model's type: queries of bf16 models go to fp16 with a power of two per
+// row, which keeps all their bits.  A page's key scale multiplies its scores; the value scale z is added to the exponent,
+// 2^(s + log2 z - m), so that fp16 weights keep their precision where pages differ in magnitude, and taken out of the sum again.
+//
+// The reference m of a row is raised only when a score exceeds it by 2^8 (one vote per tile instead of a reduction).
+// Weights of bf16 caches are split into two bf16 pieces, which costs tensor time that is there and keeps
+// the result within its own rounding; fp16 weights are rounded once and the sum adds up the rounded ones.
+//
+// Keys are split over CTAs by a fixed number of keys per CTA (short sequences then take fewer CTAs), the warps of a
+// CTA take every fourth tile; partial rows are merged in order, across CTAs by a second launch.
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace eb {
+namespace {
+
+constexpr int kStepWarps = 4;
+constexpr float kLog2eStep = 1.4426950408889634f;
+constexpr float kGrow = 8.f;
+
+struct StepParams {
+  PagedBatch batch;
+  const void *q;
+  void *o;
+  long long ldq, ldo;
+  const void *k_pages, *v_pages;
+  const float *k_scale, *v_scale;
+  int kv_heads, group, window, few;      // few: sequences with more rows (tokens x group) than this are left to the prompt kernel
+  int row_tiles, chunk;                  // tiles of query rows, keys per CTA
+  float scale_log2;
+  float *part;                           // [batch][kv_heads][row tiles][splits][rows][D + 2], or null: one split
+  int splits;
+};
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <typename T> __device__ __forceinline__ void mma_tile(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Keys that the query rows of a tile see: [lo, hi), and the rows' own limits.
+struct StepTile {
+  int rows, past, lo, hi;
+};
+__device__ __forceinline__ StepTile step_tile(const StepParams &p, const PagedRows &r, int rt, int tile_rows) {
+  StepTile t;
+  const int all = r.count * p.group;
+  t.rows = min(tile_rows, all - rt * tile_rows);
+  t.past = r.past;
+  const int first = r.past + rt * tile_rows / p.group, last = r.past + (rt * tile_rows + t.rows - 1) / p.group;
+  t.hi = min(last + 1, p.batch.table_cols << p.batch.page_shift);
+  t.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+  return t;
+}
+
+// T: type of queries and output; EIGHT: e4m3 pages; NT: tiles of 8 query rows
+template <typename T, bool EIGHT, int D, int NT>
+__global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : NT == 1 ? (EIGHT ? 4 : 3) : 2) paged_step_kernel(const StepParams p) {
+  using M = typename std::conditional<EIGHT, __half, T>::type;           // operand type of the products
+  constexpr bool kSplitP = std::is_same<M, __nv_bfloat16>::value;
+  constexpr int kRowsT = 8 * NT, kTiles = D / 16;
+  constexpr int kKeyRegs = EIGHT ? D / 16 : D / 8;                       // registers per lane and key row
+  constexpr int kValRegs = EIGHT ? D / 32 : D / 16;                      // ... and value row
+  __shared__ float red[kStepWarps][kRowsT][D + 2];
+  griddep_wait();
+  griddep_launch();
+  const int split = blockIdx.x, hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const PagedRows r = paged_rows(p.batch, b);
+  if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
+  const StepTile t = step_tile(p, r, rt, kRowsT);
+  const int lo = (t.lo & ~15) + split * p.chunk, hi = split == p.splits - 1 ? t.hi : min(t.hi, lo + p.chunk);
+  if (split > 0 && lo >= hi) return;
+
+  // ---- queries: fragments of the second operand, k index permuted like the keys ----
+  uint32_t qf[NT][kTiles][2];
+  float factor[NT][2];                                                   // exponent of a score, for the two query rows of this lane
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int row = rt * kRowsT + n * 8 + g, tok = row / p.group, head = hk * p.group + row % p.group;
+    const bool there = n * 8 + g < t.rows;
+    const T *q = reinterpret_cast<const T *>(p.q) + (long long)(r.row0 + tok) * p.ldq + (long long)head * D;
+    float row_factor = p.scale_log2;
+    // chunk j of 16 bytes of codes (16 dimensions) or of 16-bit values (8), taken by lane c as chunk c + 4 j
+    constexpr int kPer = EIGHT ? 16 : 8, kChunks = D / kPer / 4;
+    uint4 raw[kTiles / 2];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+      for (int i = 0; i < kPer / 8; ++i)
+        raw[j * (kPer / 8) + i] = there ? *reinterpret_cast<const uint4 *>(q + (c + 4 * j) * kPer + i * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kTiles / 2; ++i) {
+      qf[n][2 * i][0] = raw[i].x;
+      qf[n][2 * i][1] = raw[i].y;
+      qf[n][2 * i + 1][0] = raw[i].z;
+      qf[n][2 * i + 1][1] = raw[i].w;
+    }
+    if constexpr (EIGHT && std::is_same<T, __nv_bfloat16>::value) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 f = unpack2<__nv_bfloat16>(qf[n][i][e]);
+          m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      // the largest magnitude to [2^14, 2^15): what falls out of fp16's range below is 2^-38 of it
+      const int e = min(max(14 - ((__float_as_int(m) >> 23) - 127), -100), 100);
+      const float up = __int_as_float((127 + e) << 23);
+      row_factor *= __int_as_float((127 - e) << 23);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 f = unpack2<__nv_bfloat16>(qf[n][i][k]);
+          qf[n][i][k] = pack2<__half>(f.x * up, f.y * up);
+        }
+    }
+    factor[n][0] = __shfl_sync(0xffffffffu, row_factor, 8 * c);          // (row 2c is held by lanes 8c .. 8c + 3)
+    factor[n][1] = __shfl_sync(0xffffffffu, row_factor, 8 * c + 4);
+  }
+  int row_pos[NT][2];                                                    // position of the two query rows
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) row_pos[n][e] = t.past + (rt * kRowsT + n * 8 + 2 * c + e) / p.group;
+  const int first_pos = t.past + rt * kRowsT / p.group, last_pos = t.past + (rt * kRowsT + t.rows - 1) / p.group;
+
+  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
+    l_run[n][0] = l_run[n][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
+  }
+
+  constexpr long long kRowBytes = EIGHT ? D : 2 * D;
+  const long long block_bytes = kRowBytes << p.batch.page_shift;
+  const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.k_pages), *vp = reinterpret_cast<const uint8_t *>(p.v_pages);
+  const int blocks = hi > lo ? (hi - lo + 15) / 16 : 0, mine = blocks > warp ? (blocks - warp + kStepWarps - 1) / kStepWarps : 0;
+  // lane l holds the page of this warp's tile 32 n + l (and its scales)
+  int ids = -1;
+  float ks = 1.f, vs = 1.f;
+  auto fetch_ids = [&](int i0) {
+    ids = -1;
+    if (i0 + lane < mine) ids = paged_page(p.batch, b, (lo + (warp + (i0 + lane) * kStepWarps) * 16) >> p.batch.page_shift);
+    if (EIGHT && ids >= 0) {
+      ks = p.k_scale[(long long)ids * p.kv_heads + hk];
+      vs = p.v_scale[(long long)ids * p.kv_heads + hk];
+    }
+  };
+  uint32_t kr[2][kKeyRegs], vr[4][kValRegs];
+  // address of the 16 rows of tile i (null: no such page)
+  auto tile_at = [&](const uint8_t *pool, int i, int id) {
+    const int key = lo + (warp + i * kStepWarps) * 16;
+    return pool + ((long long)id * p.kv_heads + hk) * block_bytes + (key & ((1 << p.batch.page_shift) - 1)) * kRowBytes;
+  };
+  auto load_keys = [&](int i, int id) {
+    const uint8_t *x = tile_at(kp, i, id) + g * kRowBytes + c * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < kKeyRegs / 4; ++j) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(x + h * 8 * kRowBytes + j * 64));
+        kr[h][4 * j] = w.x;
+        kr[h][4 * j + 1] = w.y;
+        kr[h][4 * j + 2] = w.z;
+        kr[h][4 * j + 3] = w.w;
+      }
+  };
+  // value rows 2c, 2c + 1, 2c + 8, 2c + 9; dimensions by g
+  auto load_values = [&](int i, int id) {
+    const uint8_t *x = tile_at(vp, i, id) + 2 * c * kRowBytes;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint8_t *y = x + ((h & 1) + (h >> 1) * 8) * kRowBytes;
+      if constexpr (kValRegs == 2) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(y + g * 8));
+        vr[h][0] = w.x;
+        vr[h][1] = w.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kValRegs / 4; ++j) {
+          const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(y + j * 128 + g * 16));
+          vr[h][4 * j] = w.x;
+          vr[h][4 * j + 1] = w.y;
+          vr[h][4 * j + 2] = w.z;
+          vr[h][4 * j + 3] = w.w;
+        }
+      }
+    }
+  };
+  fetch_ids(0);
+  int id = __shfl_sync(0xffffffffu, ids, 0);
+  float k_now = __shfl_sync(0xffffffffu, ks, 0), v_now = __shfl_sync(0xffffffffu, vs, 0);
+  if (mine > 0 && id >= 0) {
+    load_keys(0, id);
+    load_values(0, id);
+  }
+  for (int i = 0; i < mine; ++i) {
+    const int key0 = lo + (warp + i * kStepWarps) * 16, id_now = id;
+    const float ks_now = k_now, vs_now = v_now;
+    if (i + 1 < mine) {
+      if (((i + 1) & 31) == 0) fetch_ids(i + 1);
+      id = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
+      if (EIGHT) {
+        k_now = __shfl_sync(0xffffffffu, ks, (i + 1) & 31);
+        v_now = __shfl_sync(0xffffffffu, vs, (i + 1) & 31);
+      }
+    }
+    const bool more = i + 1 < mine && id >= 0;
+    if (id_now < 0) {                                                    // (a page that is none: nothing to see)
+      if (more) {
+        load_keys(i + 1, id);
+        load_values(i + 1, id);
+      }
+      continue;
+    }
+    // ---- scores ----
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) {
+      uint32_t a0, a1, a2, a3;
+      if constexpr (EIGHT) {
+        a0 = e4m3x2_to_half2(kr[0][k]);
+        a1 = e4m3x2_to_half2(kr[1][k]);
+        a2 = e4m3x2_to_half2(kr[0][k] >> 16);
+        a3 = e4m3x2_to_half2(kr[1][k] >> 16);
+      } else {
+        a0 = kr[0][2 * k];
+        a1 = kr[1][2 * k];
+        a2 = kr[0][2 * k + 1];
+        a3 = kr[1][2 * k + 1];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_tile<M>(s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+    }
+    if (more) load_keys(i + 1, id);
+    const float v_log = EIGHT ? __log2f(vs_now) : 0.f, v_inv = EIGHT ? 1.f / vs_now : 1.f;
+    const bool whole = key0 + 16 <= min(hi, first_pos + 1) && key0 >= t.lo && (p.window == 0 || key0 > last_pos - p.window);
+    bool grows = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float v = EIGHT ? fmaf(s[n][e], factor[n][e & 1] * ks_now, v_log) : s[n][e] * factor[n][e & 1];
+        if (!whole) {
+          const int key = key0 + g + (e >> 1) * 8, pos = row_pos[n][e & 1];
+          if (key >= hi || key > pos || (p.window > 0 && key <= pos - p.window)) v = -INFINITY;
+        }
+        s[n][e] = v;
+        grows |= v > m_ref[n][e & 1] + kGrow;
+      }
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float m = fmaxf(m_ref[n][e], fmaxf(s[n][e], s[n][e + 2]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          const float alpha = pow2(m_ref[n][e] - m);
+          m_ref[n][e] = m;
+          l_run[n][e] *= alpha;
+#pragma unroll
+          for (int k = 0; k < kTiles; ++k) {
+            acc[n][k][e] *= alpha;
+            acc[n][k][e + 2] *= alpha;
+          }
+        }
+    }
+    uint32_t pf[NT][2], pl[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float w0 = pow2(s[n][2 * h] - m_ref[n][0]), w1 = pow2(s[n][2 * h + 1] - m_ref[n][1]);
+        const uint32_t w = pack2<M>(w0, w1);
+        const float2 rounded = unpack2<M>(w);
+        pf[n][h] = transposed(w);
+        if constexpr (kSplitP) {
+          pl[n][h] = transposed(pack2<M>(w0 - rounded.x, w1 - rounded.y));
+          l_run[n][0] += w0;
+          l_run[n][1] += w1;
+        } else {
+          l_run[n][0] = fmaf(rounded.x, v_inv, l_run[n][0]);
+          l_run[n][1] = fmaf(rounded.y, v_inv, l_run[n][1]);
+        }
+      }
+    // value rows that no query row of the tile sees may hold anything
+    if (key0 + 16 > hi || key0 < t.lo) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int key = key0 + 2 * c + (h & 1) + (h >> 1) * 8;
+        if (key >= hi || key < t.lo) {
+#pragma unroll
+          for (int j = 0; j < kValRegs; ++j) vr[h][j] = 0;
+        }
+      }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int k = 0; k < kTiles; ++k) {
+      uint32_t a0, a1, a2, a3;
+      if constexpr (EIGHT) {
+        // bytes 2 (k % 2) and the next of word k / 2: two dimensions of four keys
+        const uint32_t sel = (k & 1) ? 0x7362 : 0x5140;
+        const uint32_t x = __byte_perm(vr[0][k / 2], vr[1][k / 2], sel), y = __byte_perm(vr[2][k / 2], vr[3][k / 2], sel);
+        a0 = e4m3x2_to_half2(x);
+        a1 = e4m3x2_to_half2(x >> 16);
+        a2 = e4m3x2_to_half2(y);
+        a3 = e4m3x2_to_half2(y >> 16);
+      } else {
+        a0 = __byte_perm(vr[0][k], vr[1][k], 0x5410);
+        a1 = __byte_perm(vr[0][k], vr[1][k], 0x7632);
+        a2 = __byte_perm(vr[2][k], vr[3][k], 0x5410);
+        a3 = __byte_perm(vr[2][k], vr[3][k], 0x7632);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_tile<M>(acc[n][k], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+        if constexpr (kSplitP) mma_tile<M>(acc[n][k], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+      }
+    }
+    if (more) load_values(i + 1, id);
+  }
+
+  // ---- the warps' partial rows ----
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[n][e];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      float *row = red[warp][n * 8 + 2 * c + e];
+#pragma unroll
+      for (int k = 0; k < kTiles; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // tile k of e4m3 rows: dimensions (D / 8) g + 2 k + h; of 16-bit rows: 8 g + 2 (k % 4) + h of half k / 4
+          const int d = EIGHT ? D / 8 * g + 2 * k + h : k / 4 * 64 + 8 * g + 2 * (k % 4) + h;
+          row[d] = acc[n][k][e + 2 * h];
+        }
+      if (g == 0) {
+        row[D] = m_ref[n][e];
+        row[D + 1] = l;
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.rows * (D / 2); i += kStepWarps * 32) {
+    const int row = i / (D / 2), d = 2 * (i % (D / 2));
+    float m = red[0][row][D], l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 1; w < kStepWarps; ++w) m = fmaxf(m, red[w][row][D]);
+#pragma unroll
+    for (int w = 0; w < kStepWarps; ++w) {
+      const float a = pow2(red[w][row][D] - m);
+      l = fmaf(red[w][row][D + 1], a, l);
+      x = fmaf(red[w][row][d], a, x);
+      y = fmaf(red[w][row][d + 1], a, y);
+    }
+    if (p.part) {
+      float *out = p.part + ((((long long)b * p.kv_heads + hk) * p.row_tiles + rt) * p.splits + split) * kRowsT * (D + 2) + row * (D + 2);
+      *reinterpret_cast<float2 *>(out + d) = make_float2(x, y);
+      if (d == 0) *reinterpret_cast<float2 *>(out + D) = make_float2(m, l);
+    } else {
+      const int all = rt * kRowsT + row;
+      T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D + d;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint32_t *>(out) = pack2<T>(x * inv, y * inv);
+    }
+  }
+}
+
+// Merges the splits of a row, in order: a warp per row.
+template <typename T, int D, int NT> __global__ void __launch_bounds__(128) paged_merge_kernel(const StepParams p) {
+  constexpr int kRowsT = 8 * NT, kPer = D / 32;
+  griddep_wait();
+  griddep_launch();
+  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z, row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PagedRows r = paged_rows(p.batch, b);
+  if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
+  const StepTile t = step_tile(p, r, rt, kRowsT);
+  if (row >= t.rows) return;
+  const int splits = min(p.splits, max(1, (t.hi - (t.lo & ~15) + p.chunk - 1) / p.chunk));
+  const float *in = p.part + (((long long)b * p.kv_heads + hk) * p.row_tiles + rt) * p.splits * kRowsT * (D + 2) + row * (D + 2);
+  float m = -3.402823466e38f, l = 0.f, x[kPer];
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, in[(long long)s * kRowsT * (D + 2) + D]);
+  m = warp_max(m);
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) x[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float *one = in + (long long)s * kRowsT * (D + 2);
+    const float2 ml = *reinterpret_cast<const float2 *>(one + D);
+    const float a = pow2(ml.x - m);
+    l = fmaf(ml.y, a, l);
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 v = *reinterpret_cast<const float2 *>(one + lane * kPer + e);
+      x[e] = fmaf(v.x, a, x[e]);
+      x[e + 1] = fmaf(v.y, a, x[e + 1]);
+    }
+  }
+  const int all = rt * kRowsT + row;
+  T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D + lane * kPer;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t *>(out + e) = pack2<T>(x[e] * inv, x[e + 1] * inv);
+}
+
+template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParams &p, cudaStream_t st) {
+  launch_pdl(paged_step_kernel<T, EIGHT, D, NT>, dim3(p.splits, p.kv_heads * p.row_tiles, p.batch.batch), dim3(kStepWarps * 32), 0, st, p);
+  if (p.part) launch_pdl(paged_merge_kernel<T, D, NT>, dim3(2 * NT, p.kv_heads * p.row_tiles, p.batch.batch), dim3(128), 0, st, p);
+  return check_launch("paged_attention");
+}
+
+// How the step form cuts a call: query rows per tile, tiles, keys per CTA, splits.
+struct StepPlan {
+  int tiles8, row_tiles, chunk, splits;
+};
+StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys) {
+  StepPlan s;
+  s.tiles8 = rows_per_head > 8 ? 2 : 1;
+  s.row_tiles = (rows_per_head + 8 * s.tiles8 - 1) / (8 * s.tiles8);
+  const long long units = (long long)batch * kv_heads * s.row_tiles, want = (8ll * sm_count() + units - 1) / units;
+  keys += 15;                                               // (the first tile may begin in front of the first key)
+  long long chunk = (keys + want - 1) / want, least = (keys + 511) / 512;
+  if (chunk < 256) chunk = 256;
+  if (chunk < least) chunk = least;
+  chunk = (chunk + 63) / 64 * 64;
+  s.splits = (int)((keys + chunk - 1) / chunk);
+  s.chunk = (int)chunk;
+  return s;
+}
+long long step_keys(long long most_length, int window, int most_new) {
+  const long long seen = (long long)window + most_new;
+  return window > 0 && seen < most_length ? seen : most_length;
+}
+size_t step_scratch(const StepPlan &s, int batch, int kv_heads, int head_dim) {
+  return s.splits > 1 ? (size_t)batch * kv_heads * s.row_tiles * s.splits * 8 * s.tiles8 * (head_dim + 2) * sizeof(float) : 0;
+}
+
+}  // namespace
+}  // namespace eb
+
+using namespace eb;
+
+extern "C" size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || most_new <= 0 || most_length <= 0 || window < 0 || heads % kv_heads) return 0;
+  const int rows = most_new * (heads / kv_heads);
+  return step_scratch(step_plan(batch, kv_heads, rows, step_keys(most_length, window, most_new)), batch, kv_heads, head_dim);
+}
+
+extern "C" int eb_paged_attention(const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int kv_heads, int head_dim,
+                                  const void *k_pages, const void *v_pages, const float *k_scale, const float *v_scale, int pages, int page_size,
+                                  const int32_t *tables, long long table_ld, int table_cols, const int32_t *starts, const int32_t *lengths, int batch,
+                                  int most_new, int most_length, int window, float scale, int dtype, void *scratch, size_t scratch_bytes, void *stream) {
+  if (rows == 0 || batch == 0 || most_new == 0) return EB_OK;
+  StepParams p{};
+  if (int rc = paged_check("paged_attention", p.batch, tables, table_ld, starts, lengths, batch, rows, table_cols, pages, page_size)) return rc;
+  EB_REQUIRE(dtype == EB_F16 || dtype == EB_BF16, "paged_attention: fp16 or bf16 only (dtype %d)", dtype);
+  EB_REQUIRE(head_dim == 64 || head_dim == 128, "paged_attention: head_dim %d not supported (64 or 128)", head_dim);
+  EB_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && (long long)heads * head_dim < (1 << 28), "paged_attention: %d heads do not share %d key / value heads", heads, kv_heads);
+  EB_REQUIRE(q && out && k_pages && v_pages, "paged_attention: null pointer");
+  EB_REQUIRE(!k_scale == !v_scale, "paged_attention: 8-bit pages have scales for keys and for values");
+  EB_REQUIRE(most_new > 0 && most_length > 0 && window >= 0, "paged_attention: bad limits (most_new %d, most_length %d, window %d)", most_new, most_length, window);
+  EB_REQUIRE(scale > 0.f, "paged_attention: the scale must be positive");
+  EB_REQUIRE(ldq >= (long long)heads * head_dim && ldo >= (long long)heads * head_dim && ldq % 8 == 0 && ldo % 8 == 0,
+             "paged_attention: row strides must be multiples of 8 elements that hold a row");
+  EB_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_pages) && aligned16(v_pages), "paged_attention: pointers must be 16-byte aligned");
+  if (most_new > rows) most_new = rows;
+  const long long reach = (long long)table_cols * page_size;
+  if (most_length > reach) most_length = (int)reach;
+  const int group = heads / kv_heads;
+  EB_REQUIRE((long long)most_new * group < (1 << 30), "paged_attention: too many rows");
+  const StepPlan s = step_plan(batch, kv_heads, most_new * group, step_keys(most_length, window, most_new));
+  EB_REQUIRE((long long)kv_heads * s.row_tiles <= 65535, "paged_attention: %d row tiles of %d heads exceed the grid", s.row_tiles, kv_heads);
+  const size_t need = step_scratch(s, batch, kv_heads, head_dim);
+  EB_REQUIRE(need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= need), "paged_attention: %zu bytes of scratch needed, %zu given", need, scratch_bytes);
+  p.q = q; p.o = out; p.ldq = ldq; p.ldo = ldo; p.k_pages = k_pages; p.v_pages = v_pages; p.k_scale = k_scale; p.v_scale = v_scale;
+  p.kv_heads = kv_heads; p.group = group; p.window = window; p.few = 1 << 30; p.row_tiles = s.row_tiles; p.chunk = s.chunk; p.splits = s.splits;
+  p.scale_log2 = scale * kLog2eStep; p.part = need ? reinterpret_cast<float *>(scratch) : nullptr;
+  cudaStream_t st = as_stream(stream);
+#define EB_STEP(T, E, D) (s.tiles8 == 1 ? launch_step<T, E, D, 1>(p, st) : launch_step<T, E, D, 2>(p, st))
+#define EB_STEP_D(T, E) (head_dim == 64 ? EB_STEP(T, E, 64) : EB_STEP(T, E, 128))
+  if (dtype == EB_F16) return k_scale ? EB_STEP_D(__half, true) : EB_STEP_D(__half, false);
+  return k_scale ? EB_STEP_D(__nv_bfloat16, true) : EB_STEP_D(__nv_bfloat16, false);
+#undef EB_STEP_D
+#undef EB_STEP
+}

@@ -1,0 +1,280 @@
+"""Kernels over paged caches against the restatement in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from paged_plain import E4M3, Case
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def close(got, want, tol, what=""):
+    got = got.double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all(), what
+    over = (got - want).abs() - tol
+    assert float(over.max()) <= 0, f"{what}: {float(over.max()):.3g} above the tolerance, at {int(over.flatten().argmax())}"
+
+
+def frequencies(pairs):
+    return 10000.0 ** (-torch.arange(pairs, dtype=torch.float64) / max(1, pairs))
+
+
+def check_append(c, pairs, got, pools, scales):
+    freq = frequencies(pairs).float() if pairs else None
+    want = c.append(freq)
+    n = c.starts[-1]
+    close(got[:n], want[0][0][:n], want[0][1][:n], "queries")
+    for i, name in ((0, "keys"), (1, "values")):
+        value, tol, scale = want[1 + i]
+        have = pools[i].double().cpu()
+        if c.bits == 8:
+            assert torch.equal(scales[i].cpu(), scale), name
+            have = have * scale.double()[..., None, None]
+        assert torch.equal(torch.isnan(have), torch.isnan(value)), name
+        there = ~torch.isnan(value)
+        assert bool(((have - value).abs()[there] <= tol[there]).all()), (name, float(((have - value).abs() - tol)[there].max()))
+
+
+BATCHES = [([1], [0]), ([1, 1, 1, 1, 1], [0, 15, 16, 31, 300]), ([5, 0, 1, 37], [7, 9, 64, 0]), ([150, 3], [0, 130]), ([16], [16])]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("new,past", BATCHES)
+@pytest.mark.parametrize("heads,kv_heads,dim,page,pairs", [(4, 4, 64, 16, 32), (6, 2, 128, 32, 64), (5, 1, 64, 128, 0), (3, 3, 128, 64, 11)])
+def test_append(new, past, heads, kv_heads, dim, page, pairs, bits, dtype):
+    from energonai_b200.paged import paged_append
+    c = Case(new, past, heads, kv_heads, dim, page, dtype, bits, seed=sum(new) + dim)
+    (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    freq = frequencies(pairs).float().cuda() if pairs else None
+    got = paged_append(q, k, v, *pools, tables, starts, lengths, most_new, freq=freq, k_scale=scales[0], v_scale=scales[1])
+    assert (got is q) == (pairs == 0)
+    check_append(c, pairs, got, pools, scales)
+
+
+def test_append_takes_columns_of_a_projection_and_leaves_other_rows():
+    from energonai_b200.paged import paged_append
+    c = Case([4, 1], [3, 40], 4, 2, 64, 16, BF16, 8, seed=5, pad_rows=3)
+    (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device(bad=1 << 30)
+    proj = torch.cat([q, k, v, torch.zeros_like(q)], 1)
+    q, k, v = proj[:, :256], proj[:, 256:384], proj[:, 384:512]
+    before = proj.clone()
+    got = paged_append(q, k, v, *pools, tables, starts, lengths, most_new, freq=frequencies(32).float().cuda(), k_scale=scales[0], v_scale=scales[1], q_out=q)
+    assert got.data_ptr() == proj.data_ptr()
+    check_append(c, 32, got, pools, scales)
+    assert torch.equal(proj[:, 256:], before[:, 256:]) and torch.equal(proj[5:], before[5:])
+
+
+def test_append_far_positions():
+    """The angle is taken in 64 bits: at position 2 million a 32-bit one would be off by 0.1."""
+    from energonai_b200.paged import paged_append
+    c = Case([2], [0], 2, 2, 128, 128, F16, 16, seed=3)
+    far = 2_000_000 // 128 * 128
+    (q, k, v), pools, scales, (_, starts, _, most_new) = c.device()
+    tables = torch.full((1, far // 128 + 1), -1, dtype=torch.int32, device="cuda")
+    tables[0, -1] = c.tables[0][0]
+    lengths = torch.tensor([far + 2], dtype=torch.int32, device="cuda")
+    got = paged_append(q, k, v, *pools, tables, starts, lengths, most_new, freq=frequencies(64).float().cuda())
+    c.past, c.length = [far], [far + 2]
+    x, slack = c.turned(c.q, frequencies(64).float())
+    close(got, x.flatten(1), (2.0 ** -11 * (x.abs() + slack) + slack).flatten(1))
+    x, slack = c.turned(c.k, frequencies(64).float())
+    have = pools[0][c.tables[0][0], :, :2].transpose(0, 1)
+    close(have, x, 2.0 ** -11 * (x.abs() + slack) + slack)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_eight_bit_pages_token_by_token(dtype):
+    """A page's scale grows with its largest value, earlier codes follow; zeros, the smallest and the largest numbers, infinities
+    and NaN."""
+    from energonai_b200.paged import paged_append
+    c = Case([1], [0], 1, 1, 64, 16, dtype, 8, seed=9)
+    (q, k, v), pools, scales, (tables, starts, _, _) = c.device()
+    big = float(torch.finfo(dtype).max)
+    rows = [torch.zeros(64), torch.full((64,), 1e-6), torch.linspace(-3, 3, 64), torch.linspace(-40, 40, 64), torch.full((64,), big), torch.linspace(-1, 1, 64)]
+    rows[3][5], rows[3][6], rows[3][7] = float("inf"), float("-inf"), float("nan")
+    held = torch.zeros(0, 64, dtype=torch.float64)
+    scale = 0.0
+    for n, row in enumerate(rows):
+        x = row.to(dtype)[None].cuda()
+        lengths = torch.tensor([n + 1], dtype=torch.int32, device="cuda")
+        paged_append(x, x, x, *pools, tables, starts, lengths, 1, k_scale=scales[0], v_scale=scales[1])
+        x = x.double().cpu()
+        x[~torch.isfinite(x)] = float("nan")
+        m = float(x.nan_to_num(0).abs().max())
+        need = 2.0 ** max(-100, math.ceil(math.log2(m / 448))) if m else 2.0 ** -100
+        scale = need if n == 0 else max(scale, need)
+        held = torch.cat([(held / scale).float().to(E4M3).double() * scale, (x / scale).float().to(E4M3).double() * scale])
+        for i in (0, 1):
+            assert float(scales[i][c.tables[0][0], 0]) == scale, n
+            have = pools[i][c.tables[0][0], 0, :n + 1].double().cpu() * scale
+            assert torch.equal(have.nan_to_num(7.0), held.nan_to_num(7.0)) and torch.equal(have.isnan(), held.isnan()), n
+
+
+STEPS = [([1], [0]), ([1], [16]), ([1, 1, 1], [3, 4000, 1023]), ([1] * 17, list(range(0, 34, 2))), ([1, 0, 1], [700, 5, 31])]
+FEW = [([2, 5, 1], [0, 100, 513]), ([16], [1]), ([7, 3], [0, 2047]), ([33], [0])]
+HEADS = [(4, 4, 64), (2, 2, 128), (8, 2, 128), (7, 1, 64), (12, 1, 128), (10, 2, 128), (16, 1, 64), (17, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype,bits", [(F16, 16), (BF16, 16), (F16, 8), (BF16, 8)])
+@pytest.mark.parametrize("new,past", STEPS + FEW)
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+def test_attention_of_few_tokens(new, past, heads, kv_heads, dim, bits, dtype):
+    from energonai_b200.paged import paged_attention
+    page = (16, 32, 64, 128)[(heads + len(new)) % 4]
+    c = Case(new, past, heads, kv_heads, dim, page, dtype, bits, seed=heads + sum(past))
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    for window in (0, 20) if max(past) < 2000 else (0, 700):
+        got = paged_attention(q, *pools, tables, starts, lengths, most_new, max(c.length), window=window, k_scale=scales[0], v_scale=scales[1])
+        close(got, *c.attention(window=window), f"window {window}")
+
+
+@pytest.mark.parametrize("dtype,bits", [(BF16, 16), (BF16, 8), (F16, 8)])
+@pytest.mark.parametrize("magnitude", [1e-3, 30.0, 1e4])
+def test_attention_magnitudes(magnitude, bits, dtype):
+    """Scores from almost equal to one-sided, queries far above and below fp16's normal range in bf16."""
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 3], [100, 50], 4, 2, 128, 16, dtype, bits, seed=4, magnitude=magnitude if dtype == BF16 or magnitude < 1e4 else 3e3)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    scale = 1 / magnitude if magnitude > 100 else 0.3
+    got = paged_attention(q, *pools, tables, starts, lengths, most_new, scale=scale, k_scale=scales[0], v_scale=scales[1])
+    close(got, *c.attention(scale=scale))
+
+
+def test_pages_of_very_different_scales():
+    """Values of one page are 2^30 times those of another: rows that look at the small page only keep their precision."""
+    from energonai_b200.paged import paged_attention
+    c = Case([1], [31], 1, 1, 64, 16, F16, 8, seed=8)
+    c.scale[1][c.tables[0][0]] *= 2.0 ** 30
+    c.scale[0][:] = 2.0 ** -6
+    c.pool[0] = torch.zeros_like(c.pool[0], dtype=torch.float32).to(E4M3)
+    first, second = c.tables[0]
+    c.pool[0][first] = torch.full((1, 16, 64), -448.0).to(E4M3)              # far below the keys of the second page
+    c.q = torch.full_like(c.q, 4.0)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    got = paged_attention(q, *pools, tables, starts, lengths, most_new, scale=1.0, k_scale=scales[0], v_scale=scales[1])
+    close(got, *c.attention(scale=1.0))
+
+
+def test_rows_without_keys_and_rows_behind_the_last_sequence():
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 2], [40, 5], 4, 4, 64, 16, F16, 16, seed=2, pad_rows=4)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device(bad=1 << 29)
+    tables[0] = -1                                                           # the first sequence has no pages at all
+    out = torch.full_like(q, 3.0)
+    paged_attention(q, *pools, tables, starts, lengths, most_new, out=out)
+    want, tol = c.attention()
+    assert not out[0].any()
+    close(out[1:3], want[1:3], tol[1:3])
+    assert bool((out[3:] == 3.0).all())
+
+
+def test_strided_queries_and_output():
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 4], [70, 9], 4, 2, 128, 32, BF16, 16, seed=6)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    wide, out = torch.zeros(5, 1024 + 8, dtype=BF16, device="cuda"), torch.zeros(5, 2048, dtype=BF16, device="cuda")
+    wide[:, 8:520] = q
+    got = paged_attention(wide[:, 8:520], *pools, tables, starts, lengths, most_new, out=out[:, 512:1024])
+    close(got, *c.attention())
+    assert not out[:, :512].any() and not out[:, 1024:].any()
+
+
+def test_results_do_not_depend_on_the_other_sequences():
+    """A sequence gets the same bits alone and in a batch that is cut alike, and the same bits every time."""
+    from energonai_b200.paged import paged_attention
+    c = Case([1] * 8, [900, 3, 77, 1500, 64, 640, 1, 2000], 8, 2, 128, 16, BF16, 8, seed=1)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    kw = dict(k_scale=scales[0], v_scale=scales[1])
+    a = paged_attention(q, *pools, tables, starts, lengths, 1, **kw)
+    for _ in range(3):
+        assert torch.equal(a, paged_attention(q, *pools, tables, starts, lengths, 1, **kw))
+
+
+def test_replay_with_other_lengths():
+    """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
+    from energonai_b200.paged import page_pools, paged_append, paged_attention
+    B, H, G, D, page, steps = 3, 4, 2, 64, 16, 20
+    past = [0, 14, 250]
+    cols = 20
+    c = Case([steps] * B, past, H, G, D, page, F16, 8, seed=11)
+    rows = [slice(c.starts[b], c.starts[b] + steps) for b in range(B)]
+    freq = frequencies(32).float().cuda()
+    pools, scales = [p.cuda() for p in c.pool], [s.cuda() for s in c.scale]
+    tables = torch.full((B, cols), -1, dtype=torch.int32, device="cuda")
+    for b, t in enumerate(c.tables):
+        tables[b, :len(t)] = torch.tensor(t, dtype=torch.int32)
+    starts = torch.arange(B + 1, dtype=torch.int32, device="cuda")
+    lengths = torch.tensor(past, dtype=torch.int32, device="cuda")
+    q, k, v = (torch.zeros(B, n, dtype=F16, device="cuda") for n in (H * D, G * D, G * D))
+    out = torch.zeros(B, H * D, dtype=F16, device="cuda")
+
+    def step():
+        lengths.add_(1)
+        turned = paged_append(q, k, v, *pools, tables, starts, lengths, 1, freq=freq, k_scale=scales[0], v_scale=scales[1])
+        paged_attention(turned, *pools, tables, starts, lengths, 1, 2000, k_scale=scales[0], v_scale=scales[1], out=out)
+
+    keep = [t.clone() for t in (*pools, *scales, lengths)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    with torch.cuda.graph(other):
+        step()
+    for t, old in zip((*pools, *scales, lengths), keep):
+        t.copy_(old)
+    got, eager = [], []
+    for i in range(steps):
+        for t, src in ((q, c.q), (k, c.k), (v, c.v)):
+            t.copy_(torch.stack([src[r][i] for r in rows]))
+        (graph if i % 3 else other).replay()
+        got.append(out.clone())
+    after = [t.clone() for t in (*pools, *scales)]
+    for t, old in zip((*pools, *scales, lengths), keep):
+        t.copy_(old)
+    for i in range(steps):
+        for t, src in ((q, c.q), (k, c.k), (v, c.v)):
+            t.copy_(torch.stack([src[r][i] for r in rows]))
+        step()
+        eager.append(out.clone())
+    assert all(torch.equal(a, b) for a, b in zip(got, eager))
+    assert all(torch.equal(a.view(torch.uint8), t.view(torch.uint8)) for a, t in zip(after, (*pools, *scales)))
+    # the last step against the restatement over what the pages hold now
+    c.pool, c.scale = [p.cpu() for p in pools], [s.cpu() for s in scales]
+    turned, _ = c.turned(c.q, frequencies(32).float())
+    c.q = turned.flatten(1).to(F16)
+    want, tol = c.attention()
+    last = [r.stop - 1 for r in rows]
+    close(got[-1], want[last], tol[last] + 2.0 ** -9)                        # (the queries' last bits may differ: 2^-11 of scores up to 4)
+
+
+def test_refusals():
+    from energonai_b200.paged import paged_append, paged_attention
+    c = Case([1], [4], 4, 2, 64, 16, F16, 8, seed=1)
+    (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    kw = dict(k_scale=scales[0], v_scale=scales[1])
+    for fn, args in ((paged_append, (q, k, v)), (paged_attention, (q,))):
+        for bad, words in ((dict(k_scale=None), "scales"), (dict(k_scale=None, v_scale=None), "pools of"), (dict(k_scale=scales[0].half()), "scales")):
+            with pytest.raises(RuntimeError, match=words):
+                fn(*args, *pools, tables, starts, lengths, most_new, **{**kw, **bad})
+        for bad in ((tables.long(), starts, lengths), (tables, starts[:1], lengths), (tables, starts, lengths[:0]), (tables[0], starts, lengths)):
+            with pytest.raises(RuntimeError, match="int32"):
+                fn(*args, *pools, *bad, most_new, **kw)
+        with pytest.raises(RuntimeError, match="pools"):
+            fn(*args, pools[0], pools[1][:1], tables, starts, lengths, most_new, **kw)
+        with pytest.raises(RuntimeError, match="CUDA"):
+            fn(*args, pools[0], pools[1], tables.cpu(), starts, lengths, most_new, **kw)
+    with pytest.raises(RuntimeError, match="contiguous columns"):
+        paged_append(q, k.bfloat16(), v, *pools, tables, starts, lengths, most_new, **kw)
+    with pytest.raises(RuntimeError, match="frequencies"):
+        paged_append(q, k, v, *pools, tables, starts, lengths, most_new, freq=torch.ones(33, device="cuda"), **kw)
+    with pytest.raises(RuntimeError, match="unsupported dtype|fp16"):
+        paged_attention(q.float(), pools[0].float(), pools[1].float(), tables, starts, lengths, most_new)
+    with pytest.raises(RuntimeError, match="window"):
+        paged_attention(q, *pools, tables, starts, lengths, most_new, window=-1, **kw)
