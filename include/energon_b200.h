@@ -921,6 +921,16 @@ EB_API int eb_paged_attention(const void *q, long long ldq, void *out, long long
                        void *stream);
 EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window);
 
+/* Low-rank adapters of many requests: for the rows starts[b] to starts[b + 1] - 1 (at most most_new) of each sequence, with
+ * i = index[b],  delta = scales[i] (x a[i]^T) b[i]^T,  a [adapters][rank][width], b [adapters][columns][rank], rank a multiple
+ * of 8 up to 128.  An index outside of 0 .. adapters - 1, and rows behind the last sequence: zeros.  delta is what the
+ * projection beside it adds as its residual.  scratch: eb_adapter_scratch_bytes(...) bytes, 16-byte aligned, of any content.
+ * No counterpart in the reference. */
+EB_API int eb_adapter_delta(const void *x, long long ldx, const void *a, const void *b, const float *scales, const int32_t *index,
+                     const int32_t *starts, void *delta, long long ldd, int rows, int width, int columns, int rank, int adapters, int batch,
+                     int most_new, int dtype, void *scratch, size_t scratch_bytes, void *stream);
+EB_API size_t eb_adapter_scratch_bytes(int rows, int width, int rank, int batch, int most_new);
+
 /* Device-side waits are bounded; when one expires the kernel records it and returns.  This
  * reads (synchronously) the status word of the current device: out4[0] = 0 or EB_ETIMEDOUT,
  * out4[1] = which wait, out4[2] = block, out4[3] = detail.  clear != 0 resets it.  No

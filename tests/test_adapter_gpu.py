@@ -1,0 +1,121 @@
+"""Low-rank adapters of many requests against products in 64 bits."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+UNIT = {F16: 2.0 ** -11, BF16: 2.0 ** -8}
+
+
+class Case:
+    def __init__(self, new, width, columns, rank, adapters, dtype, seed=0, pad_rows=0):
+        g = torch.Generator().manual_seed(seed)
+        rnd = lambda *shape: torch.randn(*shape, generator=g)
+        self.new, self.starts = new, [0]
+        for n in new:
+            self.starts.append(self.starts[-1] + n)
+        self.rows, self.dtype, self.most_new = self.starts[-1] + pad_rows, dtype, max(1, max(new))
+        self.x, self.w = rnd(self.rows, width).to(dtype), (rnd(columns, width) / width ** 0.5).to(dtype)
+        self.a, self.b = (rnd(adapters, rank, width) / width ** 0.5).to(dtype), (rnd(adapters, columns, rank) / rank ** 0.5).to(dtype)
+        self.bias, self.scales = rnd(columns).to(dtype), 0.25 + torch.rand(adapters, generator=g)
+        self.index = torch.randint(-1, adapters, (len(new),), generator=g, dtype=torch.int32)
+        self.index[-1] = 0
+
+    def device(self):
+        return [t.cuda() for t in (self.a, self.b, self.scales, self.index)] + [torch.tensor(self.starts, dtype=torch.int32, device="cuda"), self.most_new]
+
+    def delta(self):
+        """(delta, tolerance): its rounding, and fp32 sums of `width` products: a tile adds up 16 products and rounds (truncates) into the
+        accumulator once, 2^-23 of the running sum per tile of a slice of 1 / 4 or less of the width, bounded by
+        2^-23 width / 64 + 2^-20 of the sum of magnitudes; the second product adds 2^-20, and the pieces of the low-rank row 2^-16 (bf16)."""
+        out, size = torch.zeros(self.rows, self.b.shape[1], dtype=torch.float64), torch.zeros(self.rows, self.b.shape[1], dtype=torch.float64)
+        for s, i in enumerate(self.index.tolist()):
+            if 0 <= i < self.a.shape[0] and self.new[s]:
+                r = slice(self.starts[s], self.starts[s + 1])
+                x, a, b, scale = self.x[r].double(), self.a[i].double(), self.b[i].double(), float(self.scales[i])
+                out[r] = scale * (x @ a.T) @ b.T
+                size[r] = scale * (x.abs() @ a.abs().T) @ b.abs().T
+                if self.dtype == BF16:
+                    size[r] += scale * 2.0 ** 4 * (x @ a.T).abs() @ b.abs().T                # (2^-16, in units of 2^-20)
+        return out, UNIT[self.dtype] * out.abs() + (2.0 ** -23 * self.x.shape[1] / 64 + 2.0 ** -19) * size
+
+
+def close(got, want, tol):
+    got = got.double().cpu()
+    assert got.shape == want.shape and torch.isfinite(got).all()
+    assert float(((got - want).abs() - tol).max()) <= 0
+
+
+SHAPES = [([1], 64, 64, 8, 1), ([1] * 9, 768, 2304, 16, 4), ([1] * 70, 5120, 1024, 24, 90), ([5, 1, 40, 0, 2], 200, 136, 32, 3), ([130, 17, 64], 1024, 520, 64, 2),
+          ([33], 136, 1032, 128, 2), ([16, 16], 4096, 264, 8, 2), ([15, 1, 1], 2048, 40, 120, 5)]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,width,columns,rank,adapters", SHAPES)
+def test_delta_and_product(new, width, columns, rank, adapters, dtype):
+    from energonai_b200.adapter import adapter_delta, adapter_product
+    c = Case(new, width, columns, rank, adapters, dtype, seed=width + rank, pad_rows=3)
+    want, tol = c.delta()
+    close(adapter_delta(c.x.cuda(), *c.device()), want, tol)
+    y = c.x.double() @ c.w.double().T + c.bias.double()
+    size = c.x.double().abs() @ c.w.double().abs().T + c.bias.double().abs()
+    got = adapter_product(c.x.cuda(), c.w.cuda(), *c.device(), bias=c.bias.cuda())
+    # the sum is rounded once, delta before it
+    close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * width / 16 + 2.0 ** -20) * size)
+
+
+def test_many_rows_behind_the_last_sequence():
+    from energonai_b200.adapter import adapter_delta
+    c = Case([1, 2], 64, 96, 8, 2, F16, seed=3, pad_rows=500)
+    delta = adapter_delta(c.x.cuda(), *c.device())
+    close(delta, *c.delta())
+    assert not delta[3:].any()
+
+
+def test_other_indices_are_none():
+    from energonai_b200.adapter import adapter_delta
+    c = Case([2, 3, 1], 64, 96, 8, 2, BF16, seed=4)
+    c.index = torch.tensor([2, -7, 1 << 30], dtype=torch.int32)
+    assert not adapter_delta(c.x.cuda(), *c.device()).any()
+
+
+def test_strided_rows_and_output():
+    from energonai_b200.adapter import adapter_product
+    c = Case([4, 30], 256, 128, 16, 2, F16, seed=5)
+    wide, out = torch.zeros(34, 512, dtype=F16, device="cuda"), torch.zeros(34, 384, dtype=F16, device="cuda")
+    wide[:, 128:384] = c.x.cuda()
+    got = adapter_product(wide[:, 128:384], c.w.cuda(), *c.device(), out=out[:, 128:256])
+    assert torch.equal(got, adapter_product(c.x.cuda(), c.w.cuda(), *c.device()))
+    assert not out[:, :128].any() and not out[:, 256:].any()
+
+
+def test_replay_with_other_adapters():
+    from energonai_b200.adapter import adapter_product
+    c = Case([1] * 6, 512, 256, 16, 4, BF16, seed=6)
+    x, w, rest = c.x.cuda(), c.w.cuda(), c.device()
+    adapter_product(x, w, *rest)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = adapter_product(x, w, *rest)
+    for seed in range(3):
+        other = Case([1] * 6, 512, 256, 16, 4, BF16, seed=20 + seed)
+        x.copy_(other.x)
+        rest[3].copy_(other.index)
+        graph.replay()
+        assert torch.equal(y, adapter_product(x, w, *rest))
+
+
+def test_refusals():
+    from energonai_b200.adapter import adapter_delta, adapter_product
+    c = Case([1, 2], 64, 96, 8, 2, F16, seed=1)
+    x, w, (a, b, scales, index, starts, most_new) = c.x.cuda(), c.w.cuda(), c.device()
+    for bad, words in (((a[:, :, :32], b, scales, index, starts), "required"), ((a.bfloat16(), b, scales, index, starts), "type of x"), ((a, b, scales.half(), index, starts), "fp32 scale"),
+                       ((a, b, scales, index.long(), starts), "int32"), ((a, b, scales, index, starts[:2]), "int32"), ((a, b[:1], scales, index, starts), "required")):
+        with pytest.raises(RuntimeError, match=words):
+            adapter_delta(x, *bad, most_new)
+    with pytest.raises(RuntimeError, match="rank 4"):
+        adapter_delta(x, a[:, :4].contiguous(), b[:, :, :4].contiguous(), scales, index, starts, most_new)
+    with pytest.raises(RuntimeError, match="shared weight"):
+        adapter_product(x, w[:8], a, b, scales, index, starts, most_new)
+    with pytest.raises(RuntimeError, match="bias"):
+        adapter_product(x, w, a, b, scales, index, starts, most_new, bias=torch.zeros(96, device="cuda"))
