@@ -5,7 +5,6 @@
 #include "common.cuh"
 
 namespace eb {
-namespace {
 
 // Rows starts[b] .. starts[b + 1] of a packed batch are the last tokens of sequence b, which has lengths[b] positions
 // with them; position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].  Nothing that the
@@ -16,6 +15,8 @@ struct PagedBatch {
   long long table_ld;
   int batch, rows, table_cols, pages, page_shift;
 };
+
+namespace {
 
 struct PagedRows {
   int row0, count, past, length;       // first row, rows, positions in front of them, positions in all

@@ -15,7 +15,8 @@
 // row, which keeps all their bits.  A page's key scale multiplies its scores; the value scale z is added to the exponent,
 // 2^(s + log2 z - m), so that fp16 weights keep their precision where pages differ in magnitude, and taken out of the sum again.
 //
-// The reference m of a row is raised only when a score exceeds it by 2^8 (one vote per tile instead of a reduction).
+// The reference m of a row is raised only when a score exceeds it by 2^8 (one vote per tile instead of a reduction); fp16
+// weights are 2^6 times as large, up to 2^14, which leaves fewer of them below fp16's normal range.
 // Weights of bf16 caches are split into two bf16 pieces, which costs tensor time that is there and keeps
 // the result within its own rounding; fp16 weights are rounded once and the sum adds up the rounded ones.
 //
@@ -23,14 +24,14 @@
 // CTA take every fourth tile; partial rows are merged in order, across CTAs by a second launch.
 #include <type_traits>
 
-#include "paged.cuh"
+#include "paged_prompt.cuh"
 
 namespace eb {
 namespace {
 
 constexpr int kStepWarps = 4;
 constexpr float kLog2eStep = 1.4426950408889634f;
-constexpr float kGrow = 8.f;
+constexpr float kGrow = 8.f, kLiftHalf = 6.f;
 
 struct StepParams {
   PagedBatch batch;
@@ -87,6 +88,7 @@ template <typename T, bool EIGHT, int D, int NT>
 __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : NT == 1 ? (EIGHT ? 4 : 3) : 2) paged_step_kernel(const StepParams p) {
   using M = typename std::conditional<EIGHT, __half, T>::type;           // operand type of the products
   constexpr bool kSplitP = std::is_same<M, __nv_bfloat16>::value;
+  constexpr float kLift = kSplitP ? 0.f : kLiftHalf;
   constexpr int kRowsT = 8 * NT, kTiles = D / 16;
   constexpr int kKeyRegs = EIGHT ? D / 16 : D / 8;                       // registers per lane and key row
   constexpr int kValRegs = EIGHT ? D / 32 : D / 16;                      // ... and value row
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float w0 = pow2(s[n][2 * h] - m_ref[n][0]), w1 = pow2(s[n][2 * h + 1] - m_ref[n][1]);
+        const float w0 = pow2(s[n][2 * h] - (m_ref[n][0] - kLift)), w1 = pow2(s[n][2 * h + 1] - (m_ref[n][1] - kLift));
         const uint32_t w = pack2<M>(w0, w1);
         const float2 rounded = unpack2<M>(w);
         pf[n][h] = transposed(w);
@@ -412,26 +414,18 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
   }
 }
 
-// Merges the splits of a row, in order: a warp per row.
-template <typename T, int D, int NT> __global__ void __launch_bounds__(128) paged_merge_kernel(const StepParams p) {
-  constexpr int kRowsT = 8 * NT, kPer = D / 32;
-  griddep_wait();
-  griddep_launch();
-  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z, row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const PagedRows r = paged_rows(p.batch, b);
-  if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
-  const StepTile t = step_tile(p, r, rt, kRowsT);
-  if (row >= t.rows) return;
-  const int splits = min(p.splits, max(1, (t.hi - (t.lo & ~15) + p.chunk - 1) / p.chunk));
-  const float *in = p.part + (((long long)b * p.kv_heads + hk) * p.row_tiles + rt) * p.splits * kRowsT * (D + 2) + row * (D + 2);
+// A row of the output from its splits (D values, maximum, sum; `stride` floats apart), in order, by a warp.
+template <typename T, int D> __device__ __forceinline__ void merge_row(const float *in, int stride, int splits, T *out) {
+  constexpr int kPer = D / 32;
+  const int lane = threadIdx.x & 31;
   float m = -3.402823466e38f, l = 0.f, x[kPer];
-  for (int s = lane; s < splits; s += 32) m = fmaxf(m, in[(long long)s * kRowsT * (D + 2) + D]);
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, in[(long long)s * stride + D]);
   m = warp_max(m);
 #pragma unroll
   for (int e = 0; e < kPer; ++e) x[e] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) {
-    const float *one = in + (long long)s * kRowsT * (D + 2);
+    const float *one = in + (long long)s * stride;
     const float2 ml = *reinterpret_cast<const float2 *>(one + D);
     const float a = pow2(ml.x - m);
     l = fmaf(ml.y, a, l);
@@ -442,11 +436,42 @@ template <typename T, int D, int NT> __global__ void __launch_bounds__(128) page
       x[e + 1] = fmaf(v.y, a, x[e + 1]);
     }
   }
-  const int all = rt * kRowsT + row;
-  T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D + lane * kPer;
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t *>(out + e) = pack2<T>(x[e] * inv, x[e + 1] * inv);
+  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t *>(out + lane * kPer + e) = pack2<T>(x[e] * inv, x[e + 1] * inv);
+}
+
+template <typename T, int D, int NT> __global__ void __launch_bounds__(128) paged_merge_kernel(const StepParams p) {
+  constexpr int kRowsT = 8 * NT;
+  griddep_wait();
+  griddep_launch();
+  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z, row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const PagedRows r = paged_rows(p.batch, b);
+  if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
+  const StepTile t = step_tile(p, r, rt, kRowsT);
+  if (row >= t.rows) return;
+  const int splits = min(p.splits, max(1, (t.hi - (t.lo & ~15) + p.chunk - 1) / p.chunk)), all = rt * kRowsT + row;
+  const float *in = p.part + (((long long)b * p.kv_heads + hk) * p.row_tiles + rt) * p.splits * kRowsT * (D + 2) + row * (D + 2);
+  merge_row<T, D>(in, kRowsT * (D + 2), splits,
+                  reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D);
+}
+
+// The same for the prompt kernel's blocks of 256 rows.
+template <typename T, int D> __global__ void __launch_bounds__(128) paged_prompt_merge_kernel(const PromptParams p, int blocks) {
+  constexpr int kBlock = 256;
+  griddep_wait();
+  griddep_launch();
+  const int hk = blockIdx.y, b = blockIdx.z, all = blockIdx.x * 4 + (threadIdx.x >> 5), qb = all / kBlock;
+  const PagedRows r = paged_rows(p.batch, b);
+  const int count = r.count * p.group;
+  if (count <= p.few || all >= count) return;
+  // key tiles of the block's rows, as the prompt kernel counts them
+  const int first = p.window > 0 ? max(0, r.past + qb * kBlock / p.group - p.window + 1) : 0,
+            end = min(r.past + (min((qb + 1) * kBlock, count) - 1) / p.group + 1, p.batch.table_cols << p.batch.page_shift);
+  const int splits = min(p.splits, max(1, ((end + 127) / 128 - first / 128 + p.split_tiles - 1) / p.split_tiles));
+  const float *in = p.part + (((long long)b * p.kv_heads + hk) * blocks + qb) * p.splits * kBlock * (D + 2) + (long long)(all % kBlock) * (D + 2);
+  merge_row<T, D>(in, kBlock * (D + 2), splits,
+                  reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D);
 }
 
 template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParams &p, cudaStream_t st) {
@@ -481,6 +506,36 @@ size_t step_scratch(const StepPlan &s, int batch, int kv_heads, int head_dim) {
   return s.splits > 1 ? (size_t)batch * kv_heads * s.row_tiles * s.splits * 8 * s.tiles8 * (head_dim + 2) * sizeof(float) : 0;
 }
 
+// Sequences that bring at most so many rows (tokens x heads of a group) take the step kernel, the others the prompt kernel.
+constexpr int kFewRows = 64;
+
+struct PagedPlan {
+  bool prompt;
+  int step_rows;
+  StepPlan step;
+  PromptPlan tiles;
+  size_t step_bytes, prompt_bytes;
+};
+PagedPlan paged_plan(int batch, int kv_heads, int group, int head_dim, int most_new, int most_length, int window) {
+  PagedPlan s{};
+  const long long keys = step_keys(most_length, window, most_new);
+  const int rows = most_new * group;
+  s.prompt = rows > kFewRows;
+  s.step_rows = s.prompt ? kFewRows : rows;
+  s.step = step_plan(batch, kv_heads, s.step_rows, s.prompt ? step_keys(most_length, window, kFewRows) : keys);
+  s.step_bytes = step_scratch(s.step, batch, kv_heads, head_dim);
+  if (s.prompt) {
+    // a block's keys with a window: its own rows' and the window in front
+    s.tiles = prompt_plan(batch, kv_heads, rows, step_keys(most_length, window, 256 / group + 1));
+    s.prompt_bytes = s.tiles.splits > 1 ? (size_t)batch * kv_heads * s.tiles.blocks * s.tiles.splits * 256 * (head_dim + 2) * sizeof(float) : 0;
+  }
+  return s;
+}
+
+template <typename T, int D> void launch_prompt_merge(const PromptParams &p, const PromptPlan &s, cudaStream_t st) {
+  launch_pdl(paged_prompt_merge_kernel<T, D>, dim3(s.blocks * 64, p.kv_heads, p.batch.batch), dim3(128), 0, st, p, s.blocks);
+}
+
 }  // namespace
 }  // namespace eb
 
@@ -488,8 +543,9 @@ using namespace eb;
 
 extern "C" size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || most_new <= 0 || most_length <= 0 || window < 0 || heads % kv_heads) return 0;
-  const int rows = most_new * (heads / kv_heads);
-  return step_scratch(step_plan(batch, kv_heads, rows, step_keys(most_length, window, most_new)), batch, kv_heads, head_dim);
+  if ((long long)most_new * (heads / kv_heads) >= (1 << 30)) return 0;
+  const PagedPlan s = paged_plan(batch, kv_heads, heads / kv_heads, head_dim, most_new, most_length, window);
+  return s.step_bytes + s.prompt_bytes;
 }
 
 extern "C" int eb_paged_attention(const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int kv_heads, int head_dim,
@@ -514,18 +570,30 @@ extern "C" int eb_paged_attention(const void *q, long long ldq, void *out, long 
   if (most_length > reach) most_length = (int)reach;
   const int group = heads / kv_heads;
   EB_REQUIRE((long long)most_new * group < (1 << 30), "paged_attention: too many rows");
-  const StepPlan s = step_plan(batch, kv_heads, most_new * group, step_keys(most_length, window, most_new));
-  EB_REQUIRE((long long)kv_heads * s.row_tiles <= 65535, "paged_attention: %d row tiles of %d heads exceed the grid", s.row_tiles, kv_heads);
-  const size_t need = step_scratch(s, batch, kv_heads, head_dim);
+  const PagedPlan plan = paged_plan(batch, kv_heads, group, head_dim, most_new, most_length, window);
+  const StepPlan &s = plan.step;
+  EB_REQUIRE((long long)kv_heads * s.row_tiles <= 65535, "paged_attention: %d heads exceed the grid", kv_heads);
+  const size_t need = plan.step_bytes + plan.prompt_bytes;
   EB_REQUIRE(need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= need), "paged_attention: %zu bytes of scratch needed, %zu given", need, scratch_bytes);
   p.q = q; p.o = out; p.ldq = ldq; p.ldo = ldo; p.k_pages = k_pages; p.v_pages = v_pages; p.k_scale = k_scale; p.v_scale = v_scale;
-  p.kv_heads = kv_heads; p.group = group; p.window = window; p.few = 1 << 30; p.row_tiles = s.row_tiles; p.chunk = s.chunk; p.splits = s.splits;
-  p.scale_log2 = scale * kLog2eStep; p.part = need ? reinterpret_cast<float *>(scratch) : nullptr;
+  p.kv_heads = kv_heads; p.group = group; p.window = window; p.few = kFewRows; p.row_tiles = s.row_tiles; p.chunk = s.chunk; p.splits = s.splits;
+  p.scale_log2 = scale * kLog2eStep; p.part = plan.step_bytes ? reinterpret_cast<float *>(scratch) : nullptr;
   cudaStream_t st = as_stream(stream);
+  int rc;
 #define EB_STEP(T, E, D) (s.tiles8 == 1 ? launch_step<T, E, D, 1>(p, st) : launch_step<T, E, D, 2>(p, st))
 #define EB_STEP_D(T, E) (head_dim == 64 ? EB_STEP(T, E, 64) : EB_STEP(T, E, 128))
-  if (dtype == EB_F16) return k_scale ? EB_STEP_D(__half, true) : EB_STEP_D(__half, false);
-  return k_scale ? EB_STEP_D(__nv_bfloat16, true) : EB_STEP_D(__nv_bfloat16, false);
+  if (dtype == EB_F16) rc = k_scale ? EB_STEP_D(__half, true) : EB_STEP_D(__half, false);
+  else rc = k_scale ? EB_STEP_D(__nv_bfloat16, true) : EB_STEP_D(__nv_bfloat16, false);
 #undef EB_STEP_D
 #undef EB_STEP
+  if (rc != EB_OK || !plan.prompt) return rc;
+  PromptParams t{};
+  t.batch = p.batch; t.q = q; t.o = out; t.ldq = ldq; t.ldo = ldo; t.k_pages = k_pages; t.v_pages = v_pages; t.k_scale = k_scale; t.v_scale = v_scale;
+  t.kv_heads = kv_heads; t.group = group; t.window = window; t.few = kFewRows; t.scale_log2 = p.scale_log2;
+  t.part = plan.prompt_bytes ? reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(scratch) + plan.step_bytes) : nullptr;
+  t.splits = plan.tiles.splits; t.split_tiles = plan.tiles.split_tiles;
+  if ((rc = paged_prompt(t, plan.tiles, head_dim, dtype, st)) != EB_OK || !t.part) return rc;
+  if (dtype == EB_F16) head_dim == 64 ? launch_prompt_merge<__half, 64>(t, plan.tiles, st) : launch_prompt_merge<__half, 128>(t, plan.tiles, st);
+  else head_dim == 64 ? launch_prompt_merge<__nv_bfloat16, 64>(t, plan.tiles, st) : launch_prompt_merge<__nv_bfloat16, 128>(t, plan.tiles, st);
+  return check_launch("paged_attention");
 }

@@ -1,0 +1,575 @@
+// Attention of prompts and prompt chunks over a paged cache on the 5th-generation tensor cores (tcgen05 + TMEM): the
+// rows of a sequence that brings more than a few tokens, behind any cached past, 16-bit pages or e4m3 codes.
+//
+// The rows of a CTA are (token, query head of the group) pairs, so that heads which share a key / value head share its
+// tiles too: 256 rows, two row tiles of 128, walk the visible keys 128 at a time,
+//   S  = Q K^T   (128 x 128)     in tensor memory, columns [128 t, +128) for row tile t
+//   O += P V     (128 x D)       columns [256 + 128 t, +D)
+// with V as an N-major operand.  Warp 0 moves 16-bit pages by TMA (one box per page and 64 dimensions, 128-byte swizzle; boxes
+// of 16 and more rows are whole swizzle atoms and stack up to the tile), warp 1 issues the MMAs, warps 2-5 and 6-9
+// are the softmax of the row tiles, a thread per row; their order and the lazily raised reference of a row are those of
+// the dense prompt kernel.  Codes take four more warps instead of TMA: they load a tile's codes into registers while
+// the tile before is used, and store them as fp16 (exact) in the swizzled layout.  Queries of bf16 models then become
+// fp16 with a power of two per row, which keeps all their bits.  A page's key scale multiplies its scores, and the value
+// scale z enters the exponent, 2^(s + log2 z - m), and leaves the sum again: fp16 weights keep their precision where pages
+// differ in magnitude.  Both are one fused multiply-add per score, as without scales.
+//
+// Bound by the tensor core and, equally, by the special-function unit (a 256 x 128 tile takes 2048 cycles of either).
+// Few rows behind a long past do not fill the machine: the key tiles are then split over CTAs, whose rows are merged by
+// a second launch.
+//
+// Every mbarrier wait is bounded; a wait that runs out is recorded, the CTA's roles leave (each decision made
+// uniform over the warp first), copies in flight are given time to land, TMEM is freed and the kernel returns.
+#include <type_traits>
+
+#include "paged_prompt.cuh"
+#include "tc_ops.cuh"
+
+namespace eb {
+namespace {
+
+constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kConvertWarps = 4, kScaleRing = 4;
+constexpr float kRaise = 8.f;               // the reference of a row is raised when a score exceeds it by 2^8
+constexpr float kLiftHalf = 6.f;             // fp16 weights are 2^6 times as large, up to 2^14: fewer fall below the normal range
+constexpr float kNone = -3.402823466e38f;
+
+template <int D, bool EIGHT> struct PromptSmem {
+  static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128, kPBytes = 2 * kRows * 128;
+  static constexpr int kVStages = D > 64 ? 1 : 2;
+  static constexpr int kThreads = 64 + kRowTiles * 128 + (EIGHT ? kConvertWarps * 32 : 0);
+  static constexpr size_t kTotal = 1024 + 1024 + (size_t)kRowTiles * (kQBytes + kPBytes) + (2 + kVStages) * (size_t)kKBytes;
+};
+
+// Shared memory (1024-aligned): [1 KB: barriers, TMEM slot, abort flag, per 16 keys of the last four tiles: key scale, log2 of
+// the value scale and its inverse, and a word of those in no page][Q][K: 2 stages][V][P]
+template <typename T, bool EIGHT, int D>
+__global__ void __launch_bounds__(PromptSmem<D, EIGHT>::kThreads, 1)
+paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
+  using Smem = PromptSmem<D, EIGHT>;
+  using M = typename std::conditional<EIGHT, __half, T>::type;
+  constexpr int kSub = D / 64, kVStages = Smem::kVStages;
+  constexpr uint32_t kQBytes = Smem::kQBytes, kKBytes = Smem::kKBytes, kPBytes = Smem::kPBytes, kTmemCols = 512, kPvCol = 2 * kKeys;
+  constexpr float kLift = std::is_same<M, __half>::value ? kLiftHalf : 0.f;
+  constexpr int kBf16 = std::is_same<M, __nv_bfloat16>::value ? 1 : 0;
+  constexpr uint32_t kIdescS = tc_idesc(kKeys, kBf16), kIdescPV = tc_idesc(D, kBf16) | (1u << 16);     // bit 16: B is N-major
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = s32(smem_raw);
+  uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const uint32_t bar0 = s32(smem);
+  const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56, s_full = bar0 + 72, p_full = bar0 + 88,
+                 pv_full = bar0 + 104;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 256);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 264);
+  float *key_scale = reinterpret_cast<float *>(smem + 272), *value_log = key_scale + kScaleRing * 8, *value_inv = value_log + kScaleRing * 8;
+  uint32_t *no_page = reinterpret_cast<uint32_t *>(value_inv + kScaleRing * 8);
+  uint8_t *q_ptr = smem + 1024, *k_ptr = q_ptr + kRowTiles * kQBytes, *v_ptr = k_ptr + 2 * kKBytes, *p_ptr = v_ptr + kVStages * kKBytes;
+  const uint32_t q_addr = s32(q_ptr), k_addr = s32(k_ptr), v_addr = s32(v_ptr), p_addr = s32(p_ptr);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  const int blocks = gridDim.x / p.splits, split = blockIdx.x % p.splits, qb = blocks - 1 - blockIdx.x / p.splits, hk = blockIdx.y, b = blockIdx.z;    // the latest rows, which see most, first
+  const PagedRows r = paged_rows(p.batch, b);
+  const int all = r.count * p.group, q0 = qb * kCtaRows, reach = p.batch.table_cols << p.batch.page_shift;
+  if (all <= p.few || q0 >= all) return;
+  // Key tiles that each row tile walks, [ks, nt), none for one that lies behind the sequence's rows; the CTA's own are [jmin, nmax).
+  // Keys outside of [lo, hi) are seen by no row of the CTA.
+  int nt[kRowTiles], ks[kRowTiles], nmax = 0, jmin = 0x7fffffff, lo = 0x7fffffff, hi = 0;
+#pragma unroll
+  for (int t = 0; t < kRowTiles; ++t) {
+    const int a = q0 + t * kRows, z = min(a + kRows, all) - 1;
+    const int first = p.window > 0 ? max(0, r.past + a / p.group - p.window + 1) : 0, end = a < all ? min(r.past + z / p.group + 1, reach) : 0;
+    nt[t] = (end + kKeys - 1) / kKeys;
+    ks[t] = first / kKeys;
+    if (nt[t] > ks[t]) {
+      jmin = min(jmin, ks[t]);
+      nmax = max(nmax, nt[t]);
+      lo = min(lo, first);
+      hi = max(hi, end);
+    }
+  }
+  if (jmin > nmax) jmin = nmax;
+  if (p.splits > 1) {
+    jmin += split * p.split_tiles;
+    if (split > 0 && jmin >= nmax) return;
+    nmax = min(nmax, split == p.splits - 1 ? nmax : jmin + p.split_tiles);
+#pragma unroll
+    for (int t = 0; t < kRowTiles; ++t) {
+      ks[t] = max(ks[t], jmin);
+      nt[t] = min(nt[t], nmax);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kRowTiles; ++t)
+    if (nt[t] <= ks[t]) nt[t] = ks[t] = 0;                // (walks nothing)
+
+  if (threadIdx.x == 0) {
+    if (!EIGHT) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
+    }
+    bar_init(q_full, kRowTiles * 4);
+    for (int s = 0; s < 2; ++s) {
+      bar_init(k_full + 8 * s, EIGHT ? kConvertWarps : 1);
+      bar_init(k_empty + 8 * s, 1);
+      bar_init(v_full + 8 * s, EIGHT ? kConvertWarps : 1);
+      bar_init(v_empty + 8 * s, 1);
+      bar_init(s_full + 8 * s, 1);
+      bar_init(p_full + 8 * s, 4);
+      bar_init(pv_full + 8 * s, 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(tmem_slot)), "r"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch();                                       // (not before: a following kernel must not take the tensor memory first)
+  auto all_wait = [&](uint32_t bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag, where)) != 0; };
+
+  if (warp == 0) {
+    // ---------------- 16-bit pages: TMA, a lane per page of a tile ----------------
+    if (!EIGHT && nmax > jmin) {
+      const int per_tile = kKeys >> p.batch.page_shift, page_size = 1 << p.batch.page_shift;
+      auto page_of = [&](int j) {                          // page of this lane in tile j; one outside of the pool reads as zeros
+        const int key = j * kKeys + (lane << p.batch.page_shift);
+        return lane < per_tile && j < nmax && key < hi && key + page_size > lo ? paged_page(p.batch, b, key >> p.batch.page_shift) : -1;
+      };
+      const int outside = p.batch.pages * p.kv_heads;
+      auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t bar, int page) {
+        if (lane == 0) bar_expect_tx(bar, kKBytes);
+        __syncwarp();
+        if (lane < per_tile) {
+          const int block = page >= 0 ? page * p.kv_heads + hk : outside;
+#pragma unroll
+          for (int kb = 0; kb < kSub; ++kb) tma_load_3d(dst + kb * kKeys * 128 + (lane << p.batch.page_shift) * 128, map, bar, kb * 64, 0, block);
+        }
+      };
+      auto load_k = [&](int j, int page) -> bool {
+        const int i = j - jmin, st = i & 1;
+        if (i >= 2 && !all_wait(k_empty + 8 * st, ((i >> 1) - 1) & 1, 1)) return false;
+        // groups of 16 keys without a page, where some row could see them
+        const int key = j * kKeys + (lane << p.batch.page_shift), groups = page_size >> 4;
+        uint32_t mine = lane < per_tile && page < 0 && key < hi && key + page_size > lo ? ((1u << groups) - 1) << (lane * groups) : 0;
+        mine = __reduce_or_sync(0xffffffffu, mine);
+        if (lane == 0) no_page[i & (kScaleRing - 1)] = mine;
+        load(&tm_k, k_addr + st * kKBytes, k_full + 8 * st, page);
+        return true;
+      };
+      int now = page_of(jmin), next = page_of(jmin + 1);
+      bool ok = load_k(jmin, now);
+      for (int j = jmin; j < nmax && ok; ++j) {
+        const int i = j - jmin, vs = i % kVStages, vu = i / kVStages;
+        const int later = page_of(j + 2);
+        if (j + 1 < nmax && !load_k(j + 1, next)) break;
+        if (i >= kVStages && !all_wait(v_empty + 8 * vs, (vu - 1) & 1, 9)) break;
+        load(&tm_v, v_addr + vs * kKBytes, v_full + 8 * vs, now);
+        now = next;
+        next = later;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    // Per row tile the order is S(first), then for every key tile j, as soon as P(j) is written (which also says that S(j) has been
+    // read): S(j + 1), so that the softmax warps get their next scores as early as possible, then O += P(j) V(j).
+    if (nmax > jmin) {
+      auto last_reader = [&](int j) { return j >= ks[1] && j < nt[1] ? 1 : 0; };
+      auto issue_scores = [&](int t, int j) -> bool {
+        const int st = (j - jmin) & 1;
+        if (!all_wait(k_full + 8 * st, ((j - jmin) >> 1) & 1, 3)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int kb = 0; kb < kSub; ++kb) {
+          const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_warp(tmem + t * kKeys, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
+        }
+        tc_commit_warp(s_full + 8 * t);
+        if (t == last_reader(j)) tc_commit_warp(k_empty + 8 * st);
+        return true;
+      };
+      bool ok = all_wait(q_full, 0, 2);
+      for (int t = 0; t < kRowTiles && ok; ++t)
+        if (nt[t] > 0 && ks[t] == jmin) ok = issue_scores(t, jmin);
+      for (int j = jmin; j < nmax && ok; ++j) {
+        const int vs = (j - jmin) % kVStages, vu = (j - jmin) / kVStages;
+        bool seen_v = false;
+        for (int t = 0; t < kRowTiles && ok; ++t) {
+          if (nt[t] > 0 && ks[t] == j + 1) ok = issue_scores(t, j + 1);
+          if (j < ks[t] || j >= nt[t]) continue;
+          ok = ok && all_wait(p_full + 8 * t, (j - ks[t]) & 1, 5);
+          if (ok && j + 1 < nt[t]) ok = issue_scores(t, j + 1);
+          ok = ok && all_wait(v_full + 8 * vs, vu & 1, 10);
+          if (!ok) break;
+          if (!EIGHT && !seen_v && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
+            // value rows that no row sees may hold anything: a weight of 0 does not make them 0
+            for (int i = lane; i < kKeys * kSub * 8; i += 32) {
+              const int row = i / (kSub * 8), key = j * kKeys + row, c = i % (kSub * 8);
+              if (key < lo || key >= hi) *reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes + (c >> 3) * (kKeys * 128) + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+          seen_v = true;
+          tc_fence_after();
+#pragma unroll
+          for (int a2 = 0; a2 < 2; ++a2) {
+            const uint64_t a = tc_desc(p_addr + t * kPBytes + a2 * kRows * 128);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile
+              const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + (a2 * 4 + k) * 2048, kKeys * 128);
+              tc_mma_warp(tmem + kPvCol + t * kKeys, a + 2 * k, bd, kIdescPV, (j > ks[t] || a2 > 0 || k > 0) ? 1u : 0u);
+            }
+          }
+          tc_commit_warp(pv_full + 8 * t);
+          if (t == last_reader(j)) tc_commit_warp(v_empty + 8 * vs);
+        }
+      }
+    }
+  } else if (warp < 2 + kRowTiles * 4) {
+    // ---------------- softmax warps: 4 per row tile, thread = row ----------------
+    const int t = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane, at = q0 + t * kRows + row;
+    const bool there = at < all;
+    const int token = at / p.group, head = hk * p.group + at % p.group;
+    const int ntiles = nt[t], first_tile = ks[t];
+    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_pv = t_s + kPvCol;
+    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 8 * t, my_pv_full = pv_full + 8 * t;
+    uint8_t *p_row = p_ptr + t * kPBytes + row * 128;
+    float factor = p.scale_log2;                          // exponent of a score
+    {
+      // the row of Q, swizzled
+      const T *q = reinterpret_cast<const T *>(p.q) + (long long)(r.row0 + token) * p.ldq + (long long)head * D;
+      uint4 w[D / 8];
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) w[i] = there ? *reinterpret_cast<const uint4 *>(q + i * 8) : make_uint4(0, 0, 0, 0);
+      if constexpr (EIGHT && std::is_same<T, __nv_bfloat16>::value) {
+        float m = 0.f;
+        uint32_t *x = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          const float2 f = unpack2<__nv_bfloat16>(x[i]);
+          m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        // the largest magnitude to [2^14, 2^15): what falls out of fp16's range below is 2^-38 of it
+        const int e = min(max(14 - ((__float_as_int(m) >> 23) - 127), -100), 100);
+        const float up = __int_as_float((127 + e) << 23);
+        factor *= __int_as_float((127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) {
+          const float2 f = unpack2<__nv_bfloat16>(x[i]);
+          x[i] = pack2<__half>(f.x * up, f.y * up);
+        }
+      }
+      uint8_t *dst = q_ptr + t * kQBytes + row * 128;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4 *>(dst + (i >> 3) * (kRows * 128) + (((i & 7) ^ (row & 7)) << 4)) = w[i];
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(q_full);
+    }
+    const int pos = r.past + token;
+    const int vis_end = there ? min(pos + 1, reach) : 0, vis_begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;       // this row sees [vis_begin, vis_end)
+    float m_ref = kNone, l_run = 0.f;
+    bool alive = ntiles > 0;
+    for (int j = first_tile; j < ntiles && alive; ++j) {
+      const int key0 = j * kKeys, slot = (j - jmin) & (kScaleRing - 1);
+      // Work per chunk of 32 keys, decided for the warp as a whole: 0 = hidden from every row of the warp: P = 0; 1 = visible to
+      // every row, most chunks of a long prompt; 2 = per key.  (Rows behind the sequence's last see nothing, and leave it to the others.)
+      int cls[kKeys / 32];
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; ++c) {
+        const int kb = key0 + c * 32;
+        const bool hidden = __all_sync(0xffffffffu, kb >= vis_end || kb + 32 <= vis_begin);
+        const bool simple = __all_sync(0xffffffffu, !there || (kb >= vis_begin && kb + 32 <= vis_end));
+        cls[c] = hidden ? 0 : simple ? 1 : 2;
+      }
+      if (!all_wait(my_s_full, (j - first_tile) & 1, 7)) { alive = false; break; }
+      tc_fence_after();
+      uint32_t gone = 0;                                  // groups of 16 keys without a page
+      if (!EIGHT) {
+        gone = no_page[slot];
+        if (gone) {
+#pragma unroll
+          for (int c = 0; c < kKeys / 32; ++c)
+            if (cls[c] == 1 && (gone >> (2 * c)) & 3) cls[c] = 2;
+        }
+      }
+      // factor and summand of a group's exponents
+      auto group_factor = [&](int g) { return EIGHT ? factor * key_scale[slot * 8 + g] : factor; };
+      auto group_log = [&](int g) { return EIGHT ? value_log[slot * 8 + g] : 0.f; };
+      auto visible = [&](int key, int g) { return key < vis_end && key >= vis_begin && (EIGHT || !((gone >> g) & 1)); };
+      // pass 1: the largest exponent of this tile
+      float m_tile = kNone;
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; ++c) {
+        if (cls[c] == 0) continue;
+        float x[32];
+        tc_ld32(t_s + c * 32, x);
+        if (cls[c] == 2) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = visible(key0 + c * 32 + e, 2 * c + (e >> 4)) ? x[e] : -INFINITY;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float r0 = x[h * 16], r1 = x[h * 16 + 1], r2 = x[h * 16 + 2], r3 = x[h * 16 + 3];
+#pragma unroll
+          for (int e = 4; e < 16; e += 4) {
+            r0 = fmaxf(r0, x[h * 16 + e]);
+            r1 = fmaxf(r1, x[h * 16 + e + 1]);
+            r2 = fmaxf(r2, x[h * 16 + e + 2]);
+            r3 = fmaxf(r3, x[h * 16 + e + 3]);
+          }
+          m_tile = fmaxf(m_tile, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)), group_factor(2 * c + h), group_log(2 * c + h)));
+        }
+      }
+      // The previous tile's value product must be complete before P is overwritten (it reads P) and before the accumulated row
+      // is rescaled; it was issued right behind the scores just read, so this wait is normally over already.
+      if (j > first_tile && !all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8)) { alive = false; break; }
+      if (__any_sync(0xffffffffu, m_tile > m_ref + kRaise)) {
+        const float m_new = fmaxf(m_ref, m_tile), alpha = ex2(m_ref - m_new);
+        m_ref = m_new;
+        l_run *= alpha;
+        if (j > first_tile) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float x[32];
+            tc_ld32(t_pv + c * 32, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] *= alpha;
+            tc_st32(t_pv + c * 32, x);
+          }
+          tc_st_wait();
+        }
+      }
+      // pass 2: weights, as the 16-bit A operand of the second product (swizzled rows of 128 bytes)
+#pragma unroll
+      for (int c = 0; c < kKeys / 32; ++c) {
+        uint8_t *dst = p_row + (c >> 1) * (kRows * 128);
+        if (cls[c] == 0) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        float x[32];
+        tc_ld32(t_s + c * 32, x);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float f = group_factor(2 * c + h), a = group_log(2 * c + h) - (m_ref - kLift);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) fma2(x[h * 16 + e], x[h * 16 + e + 1], x[h * 16 + e], x[h * 16 + e + 1], f, f, a, a);
+          if (cls[c] == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[h * 16 + e] = visible(key0 + c * 32 + h * 16 + e, 2 * c + h) ? x[h * 16 + e] : -INFINITY;
+          }
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            x[h * 16 + e] = ex2(x[h * 16 + e]);
+            x[h * 16 + e + 1] = ex2(x[h * 16 + e + 1]);
+            add2(l0, l1, l0, l1, x[h * 16 + e], x[h * 16 + e + 1]);
+          }
+          l_run = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * c + h], l_run) : l_run + (l0 + l1);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float *y = x + h * 16 + g * 8;
+            *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + h * 2 + g) ^ (row & 7)) << 4)) =
+                make_uint4(pack2<M>(y[0], y[1]), pack2<M>(y[2], y[3]), pack2<M>(y[4], y[5]), pack2<M>(y[6], y[7]));
+          }
+        }
+      }
+      // P is complete for this warp's 32 rows: make it visible to the tensor core's reads.  The same arrival tells the issuer that S
+      // has been read and that the row has been rescaled.
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) bar_arrive(my_p_full);
+    }
+    const bool walked = ntiles > 0;
+    if (walked && alive && !all_wait(my_pv_full, (ntiles - 1 - first_tile) & 1, 11)) alive = false;
+    if (alive || !walked) {
+      tc_fence_after();
+      float *part = p.part ? p.part + ((((long long)b * p.kv_heads + hk) * blocks + qb) * p.splits + split) * kCtaRows * (D + 2) + (long long)(t * kRows + row) * (D + 2) : nullptr;
+      if (part && there) *reinterpret_cast<float2 *>(part + D) = make_float2(m_ref, l_run);
+      const float inv = part ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
+      T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + token) * p.ldo + (long long)head * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float x[32];
+        if (walked) {
+          tc_ld32(t_pv + c * 32, x);                 // warp-wide: rows behind the sequence's last are read too, and store nothing
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = 0.f;
+        }
+        if (!there) continue;
+        if (part) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2 *>(part + c * 32 + e) = make_float2(x[e], x[e + 1]);
+        } else {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const float *y = x + g * 8;
+            *reinterpret_cast<uint4 *>(out + c * 32 + g * 8) = make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv),
+                                                                          pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
+          }
+        }
+      }
+    }
+  } else if constexpr (EIGHT) {
+    // ---------------- e4m3 codes: registers one tile ahead, fp16 into shared memory ----------------
+    // Warp w has keys 32 w .. + 31 of a tile: a load takes kRowsPer rows, kLanesPer lanes of 16 codes each.
+    constexpr int kLanesPer = D / 16, kRowsPer = 32 / kLanesPer, kLoads = 32 / kRowsPer;
+    const int w = warp - 2 - kRowTiles * 4, sub = lane / kLanesPer, chunk = lane % kLanesPer;
+    const long long block_bytes = (long long)D << p.batch.page_shift;
+    const int in_page = (1 << p.batch.page_shift) - 1;
+    // lane 0 / 1 keep the pages of the warp's two groups of 16 keys
+    auto page_of = [&](int j) {
+      const int key = j * kKeys + w * 32 + (lane & 1) * 16;
+      return j < nmax && key < hi && key + 16 > lo ? paged_page(p.batch, b, key >> p.batch.page_shift) : -1;
+    };
+    uint4 kbuf[kLoads], vbuf[kLoads];
+    auto fetch = [&](const void *pool, uint4 (&buf)[kLoads], int j, int pages2) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = i * kRowsPer + sub, key = j * kKeys + w * 32 + row, page = __shfl_sync(0xffffffffu, pages2, row >> 4);
+        buf[i] = make_uint4(0, 0, 0, 0);
+        if (page >= 0 && key >= lo && key < hi)
+          buf[i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(pool) + ((long long)page * p.kv_heads + hk) * block_bytes + (key & in_page) * D + chunk * 16);
+      }
+    };
+    // 16 codes = two 16-byte chunks of fp16; the lanes of the second 64 dimensions store theirs the other way around, or pairs of
+    // lanes would meet in a bank
+    auto store = [&](uint8_t *tile, const uint4 (&buf)[kLoads]) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = w * 32 + i * kRowsPer + sub;
+        const uint4 lo8 = make_uint4(e4m3x2_to_half2(buf[i].x), e4m3x2_to_half2(buf[i].x >> 16), e4m3x2_to_half2(buf[i].y), e4m3x2_to_half2(buf[i].y >> 16));
+        const uint4 hi8 = make_uint4(e4m3x2_to_half2(buf[i].z), e4m3x2_to_half2(buf[i].z >> 16), e4m3x2_to_half2(buf[i].w), e4m3x2_to_half2(buf[i].w >> 16));
+        const bool swap = chunk >= 4;
+        uint8_t *dst = tile + (chunk >> 2) * (kKeys * 128) + row * 128;
+        const int c0 = (chunk & 3) * 2;
+        *reinterpret_cast<uint4 *>(dst + (((c0 + (swap ? 1 : 0)) ^ (row & 7)) << 4)) = swap ? hi8 : lo8;
+        *reinterpret_cast<uint4 *>(dst + (((c0 + (swap ? 0 : 1)) ^ (row & 7)) << 4)) = swap ? lo8 : hi8;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    auto scales = [&](int j, int page) {                   // lanes 0 and 1
+      if (lane < 2) {
+        const int at = ((j - jmin) & (kScaleRing - 1)) * 8 + w * 2 + lane;
+        const long long block = (long long)page * p.kv_heads + hk;
+        const float z = page >= 0 ? p.v_scale[block] : 0.f;
+        key_scale[at] = page >= 0 ? p.k_scale[block] : 1.f;
+        value_log[at] = page >= 0 ? __log2f(z) : -INFINITY;
+        value_inv[at] = page >= 0 ? 1.f / z : 0.f;
+      }
+      __syncwarp();
+    };
+    if (nmax > jmin) {
+      int k_pages = page_of(jmin), v_pages = k_pages, next = page_of(jmin + 1);
+      fetch(p.k_pages, kbuf, jmin, k_pages);
+      fetch(p.v_pages, vbuf, jmin, v_pages);
+      // K runs a tile ahead of V: its stage is released earlier
+      auto put_k = [&](int j) -> bool {
+        const int i = j - jmin, st = i & 1;
+        if (i >= 2 && !all_wait(k_empty + 8 * st, ((i >> 1) - 1) & 1, 1)) return false;
+        scales(j, k_pages);
+        store(k_ptr + st * kKBytes, kbuf);
+        if (lane == 0) bar_arrive(k_full + 8 * st);
+        k_pages = next;
+        next = page_of(j + 2);
+        fetch(p.k_pages, kbuf, j + 1, k_pages);
+        return true;
+      };
+      bool ok = put_k(jmin);
+      for (int j = jmin; j < nmax && ok; ++j) {
+        const int i = j - jmin, vs = i % kVStages, vu = i / kVStages;
+        const int following = k_pages;                     // (of tile j + 1)
+        if (j + 1 < nmax && !put_k(j + 1)) break;
+        if (i >= kVStages && !all_wait(v_empty + 8 * vs, (vu - 1) & 1, 9)) break;
+        store(v_ptr + vs * kKBytes, vbuf);
+        if (lane == 0) bar_arrive(v_full + 8 * vs);
+        v_pages = following;
+        fetch(p.v_pages, vbuf, j + 1, v_pages);
+      }
+    }
+  }
+
+  // ---------------- teardown ----------------
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    const unsigned long long t0 = gtimer();
+    while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+template <typename T, bool EIGHT, int D> int launch_prompt(const CUtensorMap &mk, const CUtensorMap &mv, const PromptParams &p, dim3 grid, cudaStream_t st) {
+  using Smem = PromptSmem<D, EIGHT>;
+  static_assert(Smem::kTotal <= 227 * 1024, "shared memory");
+  auto kern = paged_prompt_kernel<T, EIGHT, D>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem::kTotal) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(EB_ECUDA, "paged_attention: cannot reserve %zu bytes of shared memory", Smem::kTotal);
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  launch_pdl(kern, grid, dim3(Smem::kThreads), Smem::kTotal, st, mk, mv, p);
+  return check_launch("paged_attention");
+}
+
+}  // namespace
+
+int paged_tc_status(int *out4, bool clear) { return tc_status(out4, clear); }
+
+PromptPlan prompt_plan(int batch, int kv_heads, int rows_per_head, long long keys) {
+  PromptPlan s;
+  s.blocks = (rows_per_head + kCtaRows - 1) / kCtaRows;
+  const long long ctas = (long long)batch * kv_heads * s.blocks;
+  const int tiles = (int)((keys + 2 * kKeys - 2) / kKeys);                 // (the first tile may begin in front of the first key)
+  int splits = (int)(sm_count() / ctas);                                   // what one wave has room for, of at least eight tiles each
+  if (splits > tiles / 8) splits = tiles / 8;
+  if (splits < 1) splits = 1;
+  s.split_tiles = (tiles + splits - 1) / splits;
+  s.splits = (tiles + s.split_tiles - 1) / s.split_tiles;
+  if (s.splits < 1) s.splits = 1;
+  return s;
+}
+
+int paged_prompt(PromptParams p, const PromptPlan &s, int head_dim, int dtype, cudaStream_t st) {
+  const bool eight = p.k_scale != nullptr;
+  CUtensorMap mk{}, mv{};
+  if (!eight) {
+    const long long blocks = (long long)p.batch.pages * p.kv_heads, page = 1ll << p.batch.page_shift;
+    if (blocks >= (1ll << 31)) return fail(EB_EUNSUPPORTED, "paged_attention: %lld blocks exceed the tensor map", blocks);
+    if (int rc = tc_map3(&mk, p.k_pages, dtype, head_dim, page, blocks, head_dim, page * head_dim, (int)page)) return rc;
+    if (int rc = tc_map3(&mv, p.v_pages, dtype, head_dim, page, blocks, head_dim, page * head_dim, (int)page)) return rc;
+  }
+  p.splits = s.splits;
+  p.split_tiles = s.split_tiles;
+  const dim3 grid(s.blocks * s.splits, p.kv_heads, p.batch.batch);
+#define EB_PROMPT(T, E) (head_dim == 64 ? launch_prompt<T, E, 64>(mk, mv, p, grid, st) : launch_prompt<T, E, 128>(mk, mv, p, grid, st))
+  if (dtype == EB_F16) return eight ? EB_PROMPT(__half, true) : EB_PROMPT(__half, false);
+  return eight ? EB_PROMPT(__nv_bfloat16, true) : EB_PROMPT(__nv_bfloat16, false);
+#undef EB_PROMPT
+}
+
+}  // namespace eb

@@ -66,20 +66,24 @@ class Case:
             x = x * self.scale[which][ids].double()[..., None, None]
         return x.transpose(1, 2).flatten(0, 1)[:self.length[b]]
 
-    def attention(self, scale=None, window=0):
+    def attention(self, scale=None, window=0, prompt=1 << 30, missing=()):
         """(out, tolerance), [rows, heads*dim]; rows behind the last sequence are zero.
 
         The tolerance per element: the result's own rounding, u |o|; weights rounded to the products' type (fp16 2^-11; two bf16
         pieces 2^-16) once in the sum over values and, in effect, once in the sum of weights, 2 u_p sum w |v|; a score is a sum
         of `dim` products in fp32, at most 16 of which (one per 16 dimensions, truncated) are rounded into the accumulator, 2^-19
-        sum |q||k| scale, and its exponential is off by 2^-18 at most, both once above and once below."""
+        sum |q||k| scale, and its exponential is off by 2^-18 at most, both once above and once below.  fp16 weights are
+        held as 2^6 and more times their share of the row's largest weight; where they fall below fp16's normal range all the same, they are off by
+        2^-25, that is 2^-31 of a share at most: 2^-31 sum |v|.  A result below fp16's normal range is off by 2^-25.  Sequences with more than `prompt`
+        new tokens take the prompt kernel, whose bf16 weights over 16-bit pages are rounded once, 2^-8.  missing: table entries of pages
+        that are none."""
         scale = self.dim ** -0.5 if scale is None else scale
         out, tol = torch.zeros(self.rows, self.heads, self.dim, dtype=torch.float64), torch.zeros(self.rows, self.heads, self.dim, dtype=torch.float64)
         group = self.heads // self.kv_heads
-        u_p = 2.0 ** -11 if self.bits == 8 or self.dtype == torch.float16 else 2.0 ** -16
         for b, n in enumerate(self.new):
             if not n:
                 continue
+            u_p = 2.0 ** -11 if self.bits == 8 or self.dtype == torch.float16 else 2.0 ** -8 if n > prompt else 2.0 ** -16
             rows = slice(self.starts[b], self.starts[b] + n)
             k, v = (self.values(i, b).repeat_interleave(group, 1) for i in (0, 1))
             q = self.q[rows].double().view(n, self.heads, self.dim)
@@ -87,12 +91,18 @@ class Case:
             size = torch.einsum("ihd,jhd->hij", q.abs(), k.abs()) * scale
             pos, key = torch.arange(self.past[b], self.length[b])[:, None], torch.arange(self.length[b])[None]
             seen = (key <= pos) & ((key > pos - window) if window else torch.ones(()).bool())
+            for at in missing:
+                seen = seen & ((key < at * self.page) | (key >= (at + 1) * self.page))
             w = torch.softmax(s.masked_fill(~seen, -math.inf), -1)
             delta = 2.0 ** -19 * size.masked_fill(~seen, 0).amax(-1) + 2.0 ** -18
             o = torch.einsum("hij,jhd->ihd", w, v)
             size = torch.einsum("hij,jhd->ihd", w, v.abs())
             out[rows] = o
             tol[rows] = UNIT[self.dtype] * o.abs() + (2 * u_p + 2 * delta.T[..., None]) * size
+            if self.bits == 8 or self.dtype == torch.float16:
+                tol[rows] += 2.0 ** -31 * torch.einsum("hij,jhd->ihd", seen.expand(w.shape).double(), v.abs())
+            if self.dtype == torch.float16:
+                tol[rows] += 2.0 ** -25
         return out.flatten(1), tol.flatten(1)
 
     def turned(self, x, freq):

@@ -128,7 +128,38 @@ def test_attention_of_few_tokens(new, past, heads, kv_heads, dim, bits, dtype):
     (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
     for window in (0, 20) if max(past) < 2000 else (0, 700):
         got = paged_attention(q, *pools, tables, starts, lengths, most_new, max(c.length), window=window, k_scale=scales[0], v_scale=scales[1])
-        close(got, *c.attention(window=window), f"window {window}")
+        close(got, *c.attention(window=window, prompt=64 * kv_heads // heads), f"window {window}")
+
+
+PROMPTS = [([65], [0]), ([300, 64], [0, 5]), ([257, 1, 0, 90], [200, 1000, 3, 16]), ([1, 700], [0, 1]), ([128, 256, 129], [128, 0, 1]), ([70], [5000])]
+
+
+@pytest.mark.parametrize("dtype,bits", [(F16, 16), (BF16, 16), (F16, 8), (BF16, 8)])
+@pytest.mark.parametrize("new,past", PROMPTS)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (2, 2, 128), (8, 2, 128), (7, 1, 64), (6, 2, 128)])
+def test_attention_of_prompts(new, past, heads, kv_heads, dim, bits, dtype):
+    from energonai_b200.gemm import device_status
+    from energonai_b200.paged import paged_attention
+    page = (16, 32, 64, 128)[(heads + len(new) + max(new)) % 4]
+    c = Case(new, past, heads, kv_heads, dim, page, dtype, bits, seed=heads + sum(past) + max(new))
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    for window in (0, 1, 50, 333):
+        got = paged_attention(q, *pools, tables, starts, lengths, most_new, max(c.length), window=window, k_scale=scales[0], v_scale=scales[1])
+        want, tol = c.attention(window=window, prompt=64 * kv_heads // heads)
+        close(got, want, tol, f"window {window}")
+    assert device_status()[0] == 0
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_prompt_pages_that_are_none(bits):
+    """Keys of pages outside of the pool are not there for any row, in prompts too."""
+    from energonai_b200.paged import paged_attention
+    c = Case([200], [300], 2, 1, 128, 32, BF16, bits, seed=21)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device(bad=1 << 29)
+    for at, bad in ((0, -1), (3, 1 << 30), (9, c.pages)):
+        tables[0, at] = bad
+    got = paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1])
+    close(got, *c.attention(prompt=32, missing=(0, 3, 9)))
 
 
 @pytest.mark.parametrize("dtype,bits", [(BF16, 16), (BF16, 8), (F16, 8)])
@@ -136,11 +167,11 @@ def test_attention_of_few_tokens(new, past, heads, kv_heads, dim, bits, dtype):
 def test_attention_magnitudes(magnitude, bits, dtype):
     """Scores from almost equal to one-sided, queries far above and below fp16's normal range in bf16."""
     from energonai_b200.paged import paged_attention
-    c = Case([1, 3], [100, 50], 4, 2, 128, 16, dtype, bits, seed=4, magnitude=magnitude if dtype == BF16 or magnitude < 1e4 else 3e3)
+    c = Case([1, 3, 90], [100, 50, 40], 4, 2, 128, 16, dtype, bits, seed=4, magnitude=magnitude if dtype == BF16 or magnitude < 1e4 else 3e3)
     (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
     scale = 1 / magnitude if magnitude > 100 else 0.3
     got = paged_attention(q, *pools, tables, starts, lengths, most_new, scale=scale, k_scale=scales[0], v_scale=scales[1])
-    close(got, *c.attention(scale=scale))
+    close(got, *c.attention(scale=scale, prompt=32))
 
 
 def test_pages_of_very_different_scales():
