@@ -29,9 +29,19 @@ namespace eb {
 namespace {
 
 constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kConvertWarps = 4, kScaleRing = 4;
-constexpr float kRaise = 8.f;               // the reference of a row is raised when a score exceeds it by 2^8
+constexpr float kRaise = 8.f, kMostSum = 256.f;           // the reference of a row is raised when a tile's weights add up to more
 constexpr float kLiftHalf = 6.f;             // fp16 weights are 2^6 times as large, up to 2^14: fewer fall below the normal range
 constexpr float kNone = -3.402823466e38f;
+
+// tcgen05.wait::ld that the registers of two loads pass through: nothing reads them before
+__device__ __forceinline__ void tc_ld_wait_for(float (&a)[32], float (&b)[32]) {
+  tc_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    asm volatile("" : "+f"(a[i]), "+f"(a[i + 1]), "+f"(a[i + 2]), "+f"(a[i + 3]), "+f"(a[i + 4]), "+f"(a[i + 5]), "+f"(a[i + 6]), "+f"(a[i + 7]));
+    asm volatile("" : "+f"(b[i]), "+f"(b[i + 1]), "+f"(b[i + 2]), "+f"(b[i + 3]), "+f"(b[i + 4]), "+f"(b[i + 5]), "+f"(b[i + 6]), "+f"(b[i + 7]));
+  }
+}
 
 template <int D, bool EIGHT> struct PromptSmem {
   static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128, kPBytes = 2 * kRows * 128;
@@ -280,109 +290,152 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     bool alive = ntiles > 0;
     for (int j = first_tile; j < ntiles && alive; ++j) {
       const int key0 = j * kKeys, slot = (j - jmin) & (kScaleRing - 1);
-      // Work per chunk of 32 keys, decided for the warp as a whole: 0 = hidden from every row of the warp: P = 0; 1 = visible to
-      // every row, most chunks of a long prompt; 2 = per key.  (Rows behind the sequence's last see nothing, and leave it to the others.)
-      int cls[kKeys / 32];
-#pragma unroll
-      for (int c = 0; c < kKeys / 32; ++c) {
-        const int kb = key0 + c * 32;
-        const bool hidden = __all_sync(0xffffffffu, kb >= vis_end || kb + 32 <= vis_begin);
-        const bool simple = __all_sync(0xffffffffu, !there || (kb >= vis_begin && kb + 32 <= vis_end));
-        cls[c] = hidden ? 0 : simple ? 1 : 2;
-      }
+      uint32_t gone = 0;                                  // groups of 16 keys without a page
+      // Whether every row of the warp sees the whole tile: most tiles of a long prompt.  (Rows behind the sequence's last see nothing,
+      // and leave it to the others.)
+      const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kKeys <= vis_end));
       if (!all_wait(my_s_full, (j - first_tile) & 1, 7)) { alive = false; break; }
       tc_fence_after();
-      uint32_t gone = 0;                                  // groups of 16 keys without a page
-      if (!EIGHT) {
-        gone = no_page[slot];
-        if (gone) {
-#pragma unroll
-          for (int c = 0; c < kKeys / 32; ++c)
-            if (cls[c] == 1 && (gone >> (2 * c)) & 3) cls[c] = 2;
-        }
-      }
+      if (!EIGHT) gone = no_page[slot];
       // factor and summand of a group's exponents
       auto group_factor = [&](int g) { return EIGHT ? factor * key_scale[slot * 8 + g] : factor; };
       auto group_log = [&](int g) { return EIGHT ? value_log[slot * 8 + g] : 0.f; };
-      auto visible = [&](int key, int g) { return key < vis_end && key >= vis_begin && (EIGHT || !((gone >> g) & 1)); };
-      // pass 1: the largest exponent of this tile
-      float m_tile = kNone;
-#pragma unroll
-      for (int c = 0; c < kKeys / 32; ++c) {
-        if (cls[c] == 0) continue;
-        float x[32];
-        tc_ld32(t_s + c * 32, x);
-        if (cls[c] == 2) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = visible(key0 + c * 32 + e, 2 * c + (e >> 4)) ? x[e] : -INFINITY;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float r0 = x[h * 16], r1 = x[h * 16 + 1], r2 = x[h * 16 + 2], r3 = x[h * 16 + 3];
-#pragma unroll
-          for (int e = 4; e < 16; e += 4) {
-            r0 = fmaxf(r0, x[h * 16 + e]);
-            r1 = fmaxf(r1, x[h * 16 + e + 1]);
-            r2 = fmaxf(r2, x[h * 16 + e + 2]);
-            r3 = fmaxf(r3, x[h * 16 + e + 3]);
-          }
-          m_tile = fmaxf(m_tile, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)), group_factor(2 * c + h), group_log(2 * c + h)));
-        }
-      }
-      // The previous tile's value product must be complete before P is overwritten (it reads P) and before the accumulated row
-      // is rescaled; it was issued right behind the scores just read, so this wait is normally over already.
-      if (j > first_tile && !all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8)) { alive = false; break; }
-      if (__any_sync(0xffffffffu, m_tile > m_ref + kRaise)) {
-        const float m_new = fmaxf(m_ref, m_tile), alpha = ex2(m_ref - m_new);
-        m_ref = m_new;
-        l_run *= alpha;
-        if (j > first_tile) {
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float x[32];
-            tc_ld32(t_pv + c * 32, x);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] *= alpha;
-            tc_st32(t_pv + c * 32, x);
-          }
-          tc_st_wait();
-        }
-      }
-      // pass 2: weights, as the 16-bit A operand of the second product (swizzled rows of 128 bytes)
-#pragma unroll
-      for (int c = 0; c < kKeys / 32; ++c) {
-        uint8_t *dst = p_row + (c >> 1) * (kRows * 128);
-        if (cls[c] == 0) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        float x[32];
-        tc_ld32(t_s + c * 32, x);
+      // Weights of 32 keys: exponents, powers, sums, and the 16-bit operand of the second product, two to a register.  sum: of the weights
+      // as they are, l: without the value scale.
+      auto weigh = [&](float (&x)[32], int c, uint32_t (&w)[16], float &sum, float &l) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float f = group_factor(2 * c + h), a = group_log(2 * c + h) - (m_ref - kLift);
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) fma2(x[h * 16 + e], x[h * 16 + e + 1], x[h * 16 + e], x[h * 16 + e + 1], f, f, a, a);
-          if (cls[c] == 2) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[h * 16 + e] = visible(key0 + c * 32 + h * 16 + e, 2 * c + h) ? x[h * 16 + e] : -INFINITY;
-          }
           float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            x[h * 16 + e] = ex2(x[h * 16 + e]);
-            x[h * 16 + e + 1] = ex2(x[h * 16 + e + 1]);
-            add2(l0, l1, l0, l1, x[h * 16 + e], x[h * 16 + e + 1]);
+          for (int e = h * 16; e < h * 16 + 16; e += 2) {
+            fma2(x[e], x[e + 1], x[e], x[e + 1], f, f, a, a);
+            x[e] = ex2(x[e]);
+            x[e + 1] = ex2(x[e + 1]);
+            add2(l0, l1, l0, l1, x[e], x[e + 1]);
+            w[e / 2] = pack2<M>(x[e], x[e + 1]);
           }
-          l_run = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * c + h], l_run) : l_run + (l0 + l1);
+          sum += l0 + l1;
+          l = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * c + h], l) : sum;
+        }
+      };
+      auto put = [&](int c, const uint32_t (&w)[16]) {     // swizzled rows of 128 bytes
+        uint8_t *dst = p_row + (c >> 1) * (kRows * 128);
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float *y = x + h * 16 + g * 8;
-            *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + h * 2 + g) ^ (row & 7)) << 4)) =
-                make_uint4(pack2<M>(y[0], y[1]), pack2<M>(y[2], y[3]), pack2<M>(y[4], y[5]), pack2<M>(y[6], y[7]));
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+      };
+      // Before P is overwritten the previous tile's value product, which reads it, must be complete.  It was issued right behind the
+      // scores just read.
+      auto before_put = [&]() { return j == first_tile || all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8); };
+      bool done = false, tried = false;
+      if (whole && !gone && j > first_tile) {
+        // One pass, with the reference as it is.  No maximum is taken: where the tile's weights add up to no more than 2^8, none of
+        // them is above that.  Otherwise the tile is done again below.
+        float x0[32], x1[32], sum = 0.f, l = 0.f;
+        uint32_t w0[16], w1[16];
+        tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
+        tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
+        tc_ld_wait_for(x0, x1);
+        weigh(x0, 0, w0, sum, l);
+        tc_ld32_issue(t_s + 64, reinterpret_cast<uint32_t *>(x0));
+        weigh(x1, 1, w1, sum, l);
+        tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
+        if (!before_put()) { alive = false; break; }
+        put(0, w0);
+        put(1, w1);
+        tc_ld_wait_for(x0, x1);
+        weigh(x0, 2, w0, sum, l);
+        put(2, w0);
+        weigh(x1, 3, w1, sum, l);
+        put(3, w1);
+        done = __all_sync(0xffffffffu, sum <= kMostSum * (1 << (int)kLift));
+        tried = true;
+        if (done) l_run += l;
+      }
+      if (!done) {
+        // Two passes, chunk by chunk of 32 keys: 0 = hidden from every row of the warp: P = 0; 1 = visible to every row; 2 = per key.
+        auto visible = [&](int key, int g) { return key < vis_end && key >= vis_begin && (EIGHT || !((gone >> g) & 1)); };
+        auto kind = [&](int c) {
+          const int kb = key0 + c * 32;
+          if (__all_sync(0xffffffffu, kb >= vis_end || kb + 32 <= vis_begin)) return 0;
+          return __all_sync(0xffffffffu, !there || (kb >= vis_begin && kb + 32 <= vis_end)) && !((gone >> (2 * c)) & 3) ? 1 : 2;
+        };
+        float m_tile = kNone;
+#pragma unroll 1
+        for (int c = 0; c < kKeys / 32; ++c) {
+          const int what = kind(c);
+          if (what == 0) continue;
+          float x[32];
+          tc_ld32(t_s + c * 32, x);
+          if (what == 2) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = visible(key0 + c * 32 + e, 2 * c + (e >> 4)) ? x[e] : -INFINITY;
           }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float r0 = x[h * 16], r1 = x[h * 16 + 1], r2 = x[h * 16 + 2], r3 = x[h * 16 + 3];
+#pragma unroll
+            for (int e = 4; e < 16; e += 4) {
+              r0 = fmaxf(r0, x[h * 16 + e]);
+              r1 = fmaxf(r1, x[h * 16 + e + 1]);
+              r2 = fmaxf(r2, x[h * 16 + e + 2]);
+              r3 = fmaxf(r3, x[h * 16 + e + 3]);
+            }
+            m_tile = fmaxf(m_tile, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)), group_factor(2 * c + h), group_log(2 * c + h)));
+          }
+        }
+        if (!before_put()) { alive = false; break; }
+        // the reference is raised where some row exceeds it by 2^8 (or the one pass failed), and with it for all rows of the warp (tensor memory is read and written warp-wide)
+        if (__any_sync(0xffffffffu, m_tile > (tried ? m_ref : m_ref + kRaise))) {
+          const float m_new = fmaxf(m_ref, m_tile), alpha = ex2(m_ref - m_new);
+          m_ref = m_new;
+          l_run *= alpha;
+          if (j > first_tile) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              float x[32];
+              tc_ld32(t_pv + c * 32, x);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[e] *= alpha;
+              tc_st32(t_pv + c * 32, x);
+            }
+            tc_st_wait();
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < kKeys / 32; ++c) {
+          const int what = kind(c);
+          float x[32], sum = 0.f, l = 0.f;
+          uint32_t w[16];
+          if (what == 0) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e] = 0;
+          } else {
+            tc_ld32(t_s + c * 32, x);
+            if (what == 2) {
+              // (selected behind the multiply-add: a factor that underflows to 0 would make a NaN of an infinity)
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const bool v = visible(key0 + c * 32 + e, 2 * c + (e >> 4));
+                x[e] = v ? ex2(fmaf(x[e], group_factor(2 * c + (e >> 4)), group_log(2 * c + (e >> 4)) - (m_ref - kLift))) : 0.f;
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                float l0 = 0.f;
+#pragma unroll
+                for (int e = h * 16; e < h * 16 + 16; ++e) l0 += x[e];
+                l = EIGHT ? fmaf(l0, value_inv[slot * 8 + 2 * c + h], l) : l + l0;
+              }
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = pack2<M>(x[2 * e], x[2 * e + 1]);
+            } else {
+              weigh(x, c, w, sum, l);
+            }
+          }
+          l_run += l;
+          put(c, w);
         }
       }
       // P is complete for this warp's 32 rows: make it visible to the tensor core's reads.  The same arrival tells the issuer that S
