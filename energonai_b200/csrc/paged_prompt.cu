@@ -28,25 +28,44 @@
 namespace eb {
 namespace {
 
-constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kConvertWarps = 4, kScaleRing = 4;
+constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kConvertWarps = 4, kSoftmaxWarp = 4, kConvertWarp = kSoftmaxWarp + 4 * kRowTiles, kScaleRing = 4;
 constexpr float kRaise = 8.f, kMostSum = 256.f;           // the reference of a row is raised when a tile's weights add up to more
 constexpr float kLiftHalf = 6.f;             // fp16 weights are 2^6 times as large, up to 2^14: fewer fall below the normal range
 constexpr float kNone = -3.402823466e38f;
 
-// tcgen05.wait::ld that the registers of two loads pass through: nothing reads them before
-__device__ __forceinline__ void tc_ld_wait_for(float (&a)[32], float (&b)[32]) {
+// tcgen05.wait::ld that a load's registers pass through: nothing reads them before
+__device__ __forceinline__ void tc_ld_wait_for(float (&a)[32]) {
   tc_ld_wait();
 #pragma unroll
-  for (int i = 0; i < 32; i += 8) {
+  for (int i = 0; i < 32; i += 8)
     asm volatile("" : "+f"(a[i]), "+f"(a[i + 1]), "+f"(a[i + 2]), "+f"(a[i + 3]), "+f"(a[i + 4]), "+f"(a[i + 5]), "+f"(a[i + 6]), "+f"(a[i + 7]));
-    asm volatile("" : "+f"(b[i]), "+f"(b[i + 1]), "+f"(b[i + 2]), "+f"(b[i + 3]), "+f"(b[i + 4]), "+f"(b[i + 5]), "+f"(b[i + 6]), "+f"(b[i + 7]));
+}
+
+// bar_wait in line: a function of its own would tie the register counts of the roles together
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volatile int *abort_flag, int where) {
+  if (bar_try(bar, parity)) return true;
+  const unsigned long long t0 = gtimer();
+  for (unsigned it = 1;; ++it) {
+    if (bar_try(bar, parity)) return true;
+    if ((it & 63u) == 0) {
+      if (*abort_flag) return false;
+      if (gtimer() - t0 > kTcWaitNs) {
+        *abort_flag = 1;
+        if (atomicCAS(&g_tc_status[0], 0, EB_ETIMEDOUT) == 0) {
+          g_tc_status[1] = where;
+          g_tc_status[2] = blockIdx.x;
+          g_tc_status[3] = (int)parity;
+        }
+        return false;
+      }
+    }
   }
 }
 
 template <int D, bool EIGHT> struct PromptSmem {
   static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128, kPBytes = 2 * kRows * 128;
   static constexpr int kVStages = D > 64 ? 1 : 2;
-  static constexpr int kThreads = 64 + kRowTiles * 128 + (EIGHT ? kConvertWarps * 32 : 0);
+  static constexpr int kThreads = (kConvertWarp + (EIGHT ? kConvertWarps : 0)) * 32;
   static constexpr size_t kTotal = 1024 + 1024 + (size_t)kRowTiles * (kQBytes + kPBytes) + (2 + kVStages) * (size_t)kKBytes;
 };
 
@@ -141,8 +160,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_launch();                                       // (not before: a following kernel must not take the tensor memory first)
-  auto all_wait = [&](uint32_t bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag, where)) != 0; };
+  auto all_wait = [&](uint32_t bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, wait_inline(bar, parity, abort_flag, where)) != 0; };
 
+  // Registers: 128 per thread at launch with the converters' warpgroup; the softmax keeps 64 scores and 32 weights at a time.  The
+  // shares add up to what the launch has: 104 + 2 x 152 + 104 = 4 x 128.
+  if (EIGHT && warp < kSoftmaxWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
   if (warp == 0) {
     // ---------------- 16-bit pages: TMA, a lane per page of a tile ----------------
     if (!EIGHT && nmax > jmin) {
@@ -243,9 +265,10 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
       }
     }
-  } else if (warp < 2 + kRowTiles * 4) {
+  } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
+    if (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     // ---------------- softmax warps: 4 per row tile, thread = row ----------------
-    const int t = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane, at = q0 + t * kRows + row;
+    const int t = (warp - kSoftmaxWarp) >> 2, quarter = warp & 3, row = quarter * 32 + lane, at = q0 + t * kRows + row;
     const bool there = at < all;
     const int token = at / p.group, head = hk * p.group + at % p.group;
     const int ntiles = nt[t], first_tile = ks[t];
@@ -254,32 +277,47 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     uint8_t *p_row = p_ptr + t * kPBytes + row * 128;
     float factor = p.scale_log2;                          // exponent of a score
     {
-      // the row of Q, swizzled
-      const T *q = reinterpret_cast<const T *>(p.q) + (long long)(r.row0 + token) * p.ldq + (long long)head * D;
-      uint4 w[D / 8];
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) w[i] = there ? *reinterpret_cast<const uint4 *>(q + i * 8) : make_uint4(0, 0, 0, 0);
-      if constexpr (EIGHT && std::is_same<T, __nv_bfloat16>::value) {
+      // The warp's 32 rows of Q, swizzled, D / 8 lanes per row, straight to shared memory: with most of it taken, the first-level
+      // cache is too small for as many loads to registers (6 us instead of 2 in front of the first product).
+      constexpr bool kScaled = EIGHT && std::is_same<T, __nv_bfloat16>::value;
+      constexpr int kLanesPer = D / 8, kRowsPer = 32 / kLanesPer;
+      const int sub = lane / kLanesPer, chunk = lane % kLanesPer;
+      const uint32_t dst = (kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + (chunk >> 3) * (kRows * 128);
+#pragma unroll 4
+      for (int i = 0; i < 32 / kRowsPer; ++i) {
+        // (token and head of the row, computed by its own lane)
+        const int from = i * kRowsPer + sub, to = quarter * 32 + from, tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from);
+        const bool ok = q0 + t * kRows + to < all;
+        const T *src = reinterpret_cast<const T *>(p.q) + (ok ? (long long)(r.row0 + tk) * p.ldq + (long long)hd * D + chunk * 8 : 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + to * 128 + (((chunk & 7) ^ (to & 7)) << 4)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      if constexpr (kScaled) {
+        // queries of bf16 models wait in the memory of P to become fp16
+        const uint8_t *from = p_row;
+        uint8_t *to = q_ptr + t * kQBytes + row * 128;
         float m = 0.f;
-        uint32_t *x = reinterpret_cast<uint32_t *>(w);
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) {
-          const float2 f = unpack2<__nv_bfloat16>(x[i]);
-          m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          const uint4 w = *reinterpret_cast<const uint4 *>(from + (i >> 3) * (kRows * 128) + (((i & 7) ^ (row & 7)) << 4));
+          const float2 f0 = unpack2<T>(w.x), f1 = unpack2<T>(w.y), f2 = unpack2<T>(w.z), f3 = unpack2<T>(w.w);
+          m = fmaxf(fmaxf(fmaxf(m, fmaxf(fabsf(f0.x), fabsf(f0.y))), fmaxf(fabsf(f1.x), fabsf(f1.y))),
+                    fmaxf(fmaxf(fabsf(f2.x), fabsf(f2.y)), fmaxf(fabsf(f3.x), fabsf(f3.y))));
         }
         // the largest magnitude to [2^14, 2^15): what falls out of fp16's range below is 2^-38 of it
         const int e = min(max(14 - ((__float_as_int(m) >> 23) - 127), -100), 100);
         const float up = __int_as_float((127 + e) << 23);
         factor *= __int_as_float((127 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) {
-          const float2 f = unpack2<__nv_bfloat16>(x[i]);
-          x[i] = pack2<__half>(f.x * up, f.y * up);
+#pragma unroll 4
+        for (int i = 0; i < D / 8; ++i) {
+          const int at16 = (i >> 3) * (kRows * 128) + (((i & 7) ^ (row & 7)) << 4);
+          const uint4 w = *reinterpret_cast<const uint4 *>(from + at16);
+          const float2 f0 = unpack2<T>(w.x), f1 = unpack2<T>(w.y), f2 = unpack2<T>(w.z), f3 = unpack2<T>(w.w);
+          *reinterpret_cast<uint4 *>(to + at16) = make_uint4(pack2<__half>(f0.x * up, f0.y * up), pack2<__half>(f1.x * up, f1.y * up),
+                                                             pack2<__half>(f2.x * up, f2.y * up), pack2<__half>(f3.x * up, f3.y * up));
         }
       }
-      uint8_t *dst = q_ptr + t * kQBytes + row * 128;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4 *>(dst + (i >> 3) * (kRows * 128) + (((i & 7) ^ (row & 7)) << 4)) = w[i];
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) bar_arrive(q_full);
@@ -333,22 +371,24 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // One pass, with the reference as it is.  No maximum is taken: where the tile's weights add up to no more than 2^8, none of
         // them is above that.  Otherwise the tile is done again below.
         float x0[32], x1[32], sum = 0.f, l = 0.f;
-        uint32_t w0[16], w1[16];
+        uint32_t w[16];
         tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
+        tc_ld_wait_for(x0);
         tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
-        tc_ld_wait_for(x0, x1);
-        weigh(x0, 0, w0, sum, l);
+        weigh(x0, 0, w, sum, l);
+        tc_ld_wait_for(x1);
         tc_ld32_issue(t_s + 64, reinterpret_cast<uint32_t *>(x0));
-        weigh(x1, 1, w1, sum, l);
-        tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
         if (!before_put()) { alive = false; break; }
-        put(0, w0);
-        put(1, w1);
-        tc_ld_wait_for(x0, x1);
-        weigh(x0, 2, w0, sum, l);
-        put(2, w0);
-        weigh(x1, 3, w1, sum, l);
-        put(3, w1);
+        put(0, w);
+        weigh(x1, 1, w, sum, l);
+        put(1, w);
+        tc_ld_wait_for(x0);
+        tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
+        weigh(x0, 2, w, sum, l);
+        put(2, w);
+        tc_ld_wait_for(x1);
+        weigh(x1, 3, w, sum, l);
+        put(3, w);
         done = __all_sync(0xffffffffu, sum <= kMostSum * (1 << (int)kLift));
         tried = true;
         if (done) l_run += l;
@@ -476,23 +516,24 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
       }
     }
-  } else if constexpr (EIGHT) {
+  } else if (EIGHT && warp >= kConvertWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     // ---------------- e4m3 codes: registers one tile ahead, fp16 into shared memory ----------------
     // Warp w has keys 32 w .. + 31 of a tile: a load takes kRowsPer rows, kLanesPer lanes of 16 codes each.
-    constexpr int kLanesPer = D / 16, kRowsPer = 32 / kLanesPer, kLoads = 32 / kRowsPer;
-    const int w = warp - 2 - kRowTiles * 4, sub = lane / kLanesPer, chunk = lane % kLanesPer;
+    constexpr int kOwn = kKeys / kConvertWarps, kLanesPer = D / 16, kRowsPer = 32 / kLanesPer, kLoads = kOwn / kRowsPer, kGroups = kOwn / 16;
+    const int w = warp - kConvertWarp, sub = lane / kLanesPer, chunk = lane % kLanesPer;
     const long long block_bytes = (long long)D << p.batch.page_shift;
     const int in_page = (1 << p.batch.page_shift) - 1;
-    // lane 0 / 1 keep the pages of the warp's two groups of 16 keys
+    // lane l keeps the page of the warp's group l mod 2 of 16 keys
     auto page_of = [&](int j) {
-      const int key = j * kKeys + w * 32 + (lane & 1) * 16;
+      const int key = j * kKeys + w * kOwn + (lane & (kGroups - 1)) * 16;
       return j < nmax && key < hi && key + 16 > lo ? paged_page(p.batch, b, key >> p.batch.page_shift) : -1;
     };
     uint4 kbuf[kLoads], vbuf[kLoads];
-    auto fetch = [&](const void *pool, uint4 (&buf)[kLoads], int j, int pages2) {
+    auto fetch = [&](const void *pool, uint4 (&buf)[kLoads], int j, int group_pages) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = i * kRowsPer + sub, key = j * kKeys + w * 32 + row, page = __shfl_sync(0xffffffffu, pages2, row >> 4);
+        const int row = i * kRowsPer + sub, key = j * kKeys + w * kOwn + row, page = __shfl_sync(0xffffffffu, group_pages, row >> 4);
         buf[i] = make_uint4(0, 0, 0, 0);
         if (page >= 0 && key >= lo && key < hi)
           buf[i] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(pool) + ((long long)page * p.kv_heads + hk) * block_bytes + (key & in_page) * D + chunk * 16);
@@ -503,7 +544,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     auto store = [&](uint8_t *tile, const uint4 (&buf)[kLoads]) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = w * 32 + i * kRowsPer + sub;
+        const int row = w * kOwn + i * kRowsPer + sub;
         const uint4 lo8 = make_uint4(e4m3x2_to_half2(buf[i].x), e4m3x2_to_half2(buf[i].x >> 16), e4m3x2_to_half2(buf[i].y), e4m3x2_to_half2(buf[i].y >> 16));
         const uint4 hi8 = make_uint4(e4m3x2_to_half2(buf[i].z), e4m3x2_to_half2(buf[i].z >> 16), e4m3x2_to_half2(buf[i].w), e4m3x2_to_half2(buf[i].w >> 16));
         const bool swap = chunk >= 4;
@@ -515,9 +556,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     };
-    auto scales = [&](int j, int page) {                   // lanes 0 and 1
-      if (lane < 2) {
-        const int at = ((j - jmin) & (kScaleRing - 1)) * 8 + w * 2 + lane;
+    auto scales = [&](int j, int page) {
+      if (lane < kGroups) {
+        const int at = ((j - jmin) & (kScaleRing - 1)) * 8 + w * kGroups + lane;
         const long long block = (long long)page * p.kv_heads + hk;
         const float z = page >= 0 ? p.v_scale[block] : 0.f;
         key_scale[at] = page >= 0 ? p.k_scale[block] : 1.f;
