@@ -33,12 +33,14 @@ constexpr float kRaise = 8.f, kMostSum = 256.f;           // the reference of a 
 constexpr float kLiftHalf = 6.f;             // fp16 weights are 2^6 times as large, up to 2^14: fewer fall below the normal range
 constexpr float kNone = -3.402823466e38f;
 
-// tcgen05.wait::ld that a load's registers pass through: nothing reads them before
-__device__ __forceinline__ void tc_ld_wait_for(float (&a)[32]) {
+// tcgen05.wait::ld that the registers of two loads pass through: nothing reads them before
+__device__ __forceinline__ void tc_ld_wait_for(float (&a)[32], float (&b)[32]) {
   tc_ld_wait();
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < 32; i += 8) {
     asm volatile("" : "+f"(a[i]), "+f"(a[i + 1]), "+f"(a[i + 2]), "+f"(a[i + 3]), "+f"(a[i + 4]), "+f"(a[i + 5]), "+f"(a[i + 6]), "+f"(a[i + 7]));
+    asm volatile("" : "+f"(b[i]), "+f"(b[i + 1]), "+f"(b[i + 2]), "+f"(b[i + 3]), "+f"(b[i + 4]), "+f"(b[i + 5]), "+f"(b[i + 6]), "+f"(b[i + 7]));
+  }
 }
 
 // bar_wait in line: a function of its own would tie the register counts of the roles together
@@ -87,7 +89,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bar0 = s32(smem);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56, s_full = bar0 + 72, p_full = bar0 + 88,
-                 pv_full = bar0 + 104;
+                 pv_full = bar0 + 104, s_free = bar0 + 120;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 256);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 264);
   float *key_scale = reinterpret_cast<float *>(smem + 272), *value_log = key_scale + kScaleRing * 8, *value_inv = value_log + kScaleRing * 8;
@@ -140,11 +142,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     bar_init(q_full, kRowTiles * 4);
     for (int s = 0; s < 2; ++s) {
       bar_init(k_full + 8 * s, EIGHT ? kConvertWarps : 1);
-      bar_init(k_empty + 8 * s, 1);
+      bar_init(k_empty + 8 * s, kRowTiles);
       bar_init(v_full + 8 * s, EIGHT ? kConvertWarps : 1);
-      bar_init(v_empty + 8 * s, 1);
+      bar_init(v_empty + 8 * s, kRowTiles);
       bar_init(s_full + 8 * s, 1);
       bar_init(p_full + 8 * s, 4);
+      bar_init(s_free + 8 * s, 4);
       bar_init(pv_full + 8 * s, 1);
     }
     *abort_flag = 0;
@@ -206,65 +209,68 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         next = later;
       }
     }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    // Per row tile the order is S(first), then for every key tile j, as soon as P(j) is written (which also says that S(j) has been
-    // read): S(j + 1), so that the softmax warps get their next scores as early as possible, then O += P(j) V(j).
-    if (nmax > jmin) {
-      auto last_reader = [&](int j) { return j >= ks[1] && j < nt[1] ? 1 : 0; };
-      auto issue_scores = [&](int t, int j) -> bool {
-        const int st = (j - jmin) & 1;
-        if (!all_wait(k_full + 8 * st, ((j - jmin) >> 1) & 1, 3)) return false;
+  } else if (warp <= kRowTiles) {
+    // ---------------- MMA issuers: a warp per row tile ----------------
+    // S(first), then for every key tile j: S(j + 1), as soon as S(j) has been read, so that the softmax warps find their next scores
+    // ready, and O += P(j) V(j), as soon as P(j) is written.  Both warps hand back every stage, those of tiles that theirs does not
+    // walk too, each when it is full (an earlier arrival would count for the stage's use before).
+    const int t = warp - 1, first = t == 0 ? ks[0] : ks[1], end = t == 0 ? nt[0] : nt[1];
+    auto pass = [&](int j) -> bool {                       // a tile that this row tile does not walk
+      const int i = j - jmin, vs = i % kVStages;
+      if (!all_wait(k_full + 8 * (i & 1), (i >> 1) & 1, 3)) return false;
+      if (lane == 0) bar_arrive(k_empty + 8 * (i & 1));
+      if (!all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10)) return false;
+      if (lane == 0) bar_arrive(v_empty + 8 * vs);
+      return true;
+    };
+    auto issue_scores = [&](int j) -> bool {
+      const int st = (j - jmin) & 1;
+      if (!all_wait(k_full + 8 * st, ((j - jmin) >> 1) & 1, 3)) return false;
+      tc_fence_after();
+#pragma unroll
+      for (int kb = 0; kb < kSub; ++kb) {
+        const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_warp(tmem + t * kKeys, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
+      }
+      tc_commit_warp(s_full + 8 * t);
+      tc_commit_warp(k_empty + 8 * st);
+      return true;
+    };
+    bool ok = true;
+    if (end > first) {
+      for (int j = jmin; j < first && ok; ++j) ok = pass(j);
+      ok = ok && all_wait(q_full, 0, 2) && issue_scores(first);
+      for (int j = first; j < end && ok; ++j) {
+        const int i = j - jmin, vs = i % kVStages;
+        if (j + 1 < end) ok = all_wait(s_free + 8 * t, (j - first) & 1, 4) && issue_scores(j + 1);
+        ok = ok && all_wait(p_full + 8 * t, (j - first) & 1, 5) && all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10);
+        if (!ok) break;
+        if (!EIGHT && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
+          // value rows that no row sees may hold anything, and a weight of 0 does not make them 0 (both warps may write these zeros)
+          for (int n = lane; n < kKeys * kSub * 8; n += 32) {
+            const int row = n / (kSub * 8), key = j * kKeys + row, c = n % (kSub * 8);
+            if (key < lo || key >= hi) *reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes + (c >> 3) * (kKeys * 128) + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
         tc_fence_after();
 #pragma unroll
-        for (int kb = 0; kb < kSub; ++kb) {
-          const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128);
+        for (int a2 = 0; a2 < 2; ++a2) {
+          const uint64_t a = tc_desc(p_addr + t * kPBytes + a2 * kRows * 128);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_warp(tmem + t * kKeys, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
-        }
-        tc_commit_warp(s_full + 8 * t);
-        if (t == last_reader(j)) tc_commit_warp(k_empty + 8 * st);
-        return true;
-      };
-      bool ok = all_wait(q_full, 0, 2);
-      for (int t = 0; t < kRowTiles && ok; ++t)
-        if (nt[t] > 0 && ks[t] == jmin) ok = issue_scores(t, jmin);
-      for (int j = jmin; j < nmax && ok; ++j) {
-        const int vs = (j - jmin) % kVStages, vu = (j - jmin) / kVStages;
-        bool seen_v = false;
-        for (int t = 0; t < kRowTiles && ok; ++t) {
-          if (nt[t] > 0 && ks[t] == j + 1) ok = issue_scores(t, j + 1);
-          if (j < ks[t] || j >= nt[t]) continue;
-          ok = ok && all_wait(p_full + 8 * t, (j - ks[t]) & 1, 5);
-          if (ok && j + 1 < nt[t]) ok = issue_scores(t, j + 1);
-          ok = ok && all_wait(v_full + 8 * vs, vu & 1, 10);
-          if (!ok) break;
-          if (!EIGHT && !seen_v && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
-            // value rows that no row sees may hold anything: a weight of 0 does not make them 0
-            for (int i = lane; i < kKeys * kSub * 8; i += 32) {
-              const int row = i / (kSub * 8), key = j * kKeys + row, c = i % (kSub * 8);
-              if (key < lo || key >= hi) *reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes + (c >> 3) * (kKeys * 128) + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
+          for (int k = 0; k < 4; ++k) {
+            // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile
+            const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + (a2 * 4 + k) * 2048, kKeys * 128);
+            tc_mma_warp(tmem + kPvCol + t * kKeys, a + 2 * k, bd, kIdescPV, (j > first || a2 > 0 || k > 0) ? 1u : 0u);
           }
-          seen_v = true;
-          tc_fence_after();
-#pragma unroll
-          for (int a2 = 0; a2 < 2; ++a2) {
-            const uint64_t a = tc_desc(p_addr + t * kPBytes + a2 * kRows * 128);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile
-              const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + (a2 * 4 + k) * 2048, kKeys * 128);
-              tc_mma_warp(tmem + kPvCol + t * kKeys, a + 2 * k, bd, kIdescPV, (j > ks[t] || a2 > 0 || k > 0) ? 1u : 0u);
-            }
-          }
-          tc_commit_warp(pv_full + 8 * t);
-          if (t == last_reader(j)) tc_commit_warp(v_empty + 8 * vs);
         }
+        tc_commit_warp(pv_full + 8 * t);
+        tc_commit_warp(v_empty + 8 * vs);
       }
     }
+    for (int j = max(end, jmin); j < nmax && ok; ++j) ok = pass(j);
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
     if (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     // ---------------- softmax warps: 4 per row tile, thread = row ----------------
@@ -273,7 +279,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int token = at / p.group, head = hk * p.group + at % p.group;
     const int ntiles = nt[t], first_tile = ks[t];
     const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_pv = t_s + kPvCol;
-    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 8 * t, my_pv_full = pv_full + 8 * t;
+    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 8 * t, my_pv_full = pv_full + 8 * t, my_s_free = s_free + 8 * t;
     uint8_t *p_row = p_ptr + t * kPBytes + row * 128;
     float factor = p.scale_log2;                          // exponent of a score
     {
@@ -338,6 +344,20 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       // factor and summand of a group's exponents
       auto group_factor = [&](int g) { return EIGHT ? factor * key_scale[slot * 8 + g] : factor; };
       auto group_log = [&](int g) { return EIGHT ? value_log[slot * 8 + g] : 0.f; };
+      auto largest = [&](const float (&x)[32], int c) {    // exponent of 32 keys
+        float m = kNone;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float r0 = x[h * 16], r1 = x[h * 16 + 1];
+#pragma unroll
+          for (int e = h * 16 + 2; e < h * 16 + 14; e += 4) {
+            r0 = fmaxf(r0, fmaxf(x[e], x[e + 1]));         // (one instruction for three)
+            r1 = fmaxf(r1, fmaxf(x[e + 2], x[e + 3]));
+          }
+          m = fmaxf(m, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(x[h * 16 + 14], x[h * 16 + 15])), group_factor(2 * c + h), group_log(2 * c + h)));
+        }
+        return m;
+      };
       // Weights of 32 keys: exponents, powers, sums, and the 16-bit operand of the second product, two to a register.  sum: of the weights
       // as they are, l: without the value scale.
       auto weigh = [&](float (&x)[32], int c, uint32_t (&w)[16], float &sum, float &l) {
@@ -368,30 +388,34 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       auto before_put = [&]() { return j == first_tile || all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8); };
       bool done = false, tried = false;
       if (whole && !gone && j > first_tile) {
-        // One pass, with the reference as it is.  No maximum is taken: where the tile's weights add up to no more than 2^8, none of
-        // them is above that.  Otherwise the tile is done again below.
+        // One pass, with the reference as it is: where the first half's weights add up to no more than 2^8, none of them is above that, and of
+        // the second half the maximum is taken.  Otherwise the tile is done again below.
         float x0[32], x1[32], sum = 0.f, l = 0.f;
-        uint32_t w[16];
+        uint32_t w0[16], w1[16];
         tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
-        tc_ld_wait_for(x0);
         tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
-        weigh(x0, 0, w, sum, l);
-        tc_ld_wait_for(x1);
+        tc_ld_wait_for(x0, x1);
+        weigh(x0, 0, w0, sum, l);
         tc_ld32_issue(t_s + 64, reinterpret_cast<uint32_t *>(x0));
-        if (!before_put()) { alive = false; break; }
-        put(0, w);
-        weigh(x1, 1, w, sum, l);
-        put(1, w);
-        tc_ld_wait_for(x0);
+        weigh(x1, 1, w1, sum, l);
         tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
-        weigh(x0, 2, w, sum, l);
-        put(2, w);
-        tc_ld_wait_for(x1);
-        weigh(x1, 3, w, sum, l);
-        put(3, w);
-        done = __all_sync(0xffffffffu, sum <= kMostSum * (1 << (int)kLift));
+        tc_ld_wait_for(x0, x1);
+        // the other half's weights stay below 2^8 too: nothing will be done again, and the next scores may come
+        done = __all_sync(0xffffffffu, sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise);
+        if (done) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) bar_arrive(my_s_free);
+          if (!before_put()) { alive = false; break; }
+          put(0, w0);
+          put(1, w1);
+          weigh(x0, 2, w0, sum, l);
+          put(2, w0);
+          weigh(x1, 3, w1, sum, l);
+          put(3, w1);
+          l_run += l;
+        }
         tried = true;
-        if (done) l_run += l;
       }
       if (!done) {
         // Two passes, chunk by chunk of 32 keys: 0 = hidden from every row of the warp: P = 0; 1 = visible to every row; 2 = per key.
@@ -412,18 +436,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
             for (int e = 0; e < 32; ++e) x[e] = visible(key0 + c * 32 + e, 2 * c + (e >> 4)) ? x[e] : -INFINITY;
           }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float r0 = x[h * 16], r1 = x[h * 16 + 1], r2 = x[h * 16 + 2], r3 = x[h * 16 + 3];
-#pragma unroll
-            for (int e = 4; e < 16; e += 4) {
-              r0 = fmaxf(r0, x[h * 16 + e]);
-              r1 = fmaxf(r1, x[h * 16 + e + 1]);
-              r2 = fmaxf(r2, x[h * 16 + e + 2]);
-              r3 = fmaxf(r3, x[h * 16 + e + 3]);
-            }
-            m_tile = fmaxf(m_tile, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(r2, r3)), group_factor(2 * c + h), group_log(2 * c + h)));
-          }
+          m_tile = fmaxf(m_tile, largest(x, c));
         }
         if (!before_put()) { alive = false; break; }
         // the reference is raised where some row exceeds it by 2^8 (or the one pass failed), and with it for all rows of the warp (tensor memory is read and written warp-wide)
@@ -477,9 +490,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           l_run += l;
           put(c, w);
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(my_s_free);
       }
-      // P is complete for this warp's 32 rows: make it visible to the tensor core's reads.  The same arrival tells the issuer that S
-      // has been read and that the row has been rescaled.
+      // P is complete for this warp's 32 rows (and these are rescaled): make it visible to the tensor core's reads.
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
