@@ -165,9 +165,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   griddep_launch();                                       // (not before: a following kernel must not take the tensor memory first)
   auto all_wait = [&](uint32_t bar, uint32_t parity, int where) { return __all_sync(0xffffffffu, wait_inline(bar, parity, abort_flag, where)) != 0; };
 
-  // Registers: 128 per thread at launch with the converters' warpgroup; the softmax keeps 64 scores and 32 weights at a time.  The
-  // shares add up to what the launch has: 104 + 2 x 152 + 104 = 4 x 128.
-  if (EIGHT && warp < kSoftmaxWarp) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  // Registers go where 64 scores and their weights are kept: of 128 per thread at launch with the converters' warpgroup 80 + 2 x 168 + 96,
+  // of 168 without it 120 + 2 x 192.  (The launch checks that the kernel got them.)
+  if (warp < kSoftmaxWarp) {
+    if (EIGHT) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+  }
   if (warp == 0) {
     // ---------------- 16-bit pages: TMA, a lane per page of a tile ----------------
     if (!EIGHT && nmax > jmin) {
@@ -272,7 +275,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     for (int j = max(end, jmin); j < nmax && ok; ++j) ok = pass(j);
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
-    if (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    if (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     // ---------------- softmax warps: 4 per row tile, thread = row ----------------
     const int t = (warp - kSoftmaxWarp) >> 2, quarter = warp & 3, row = quarter * 32 + lane, at = q0 + t * kRows + row;
     const bool there = at < all;
@@ -334,15 +338,27 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     bool alive = ntiles > 0;
     for (int j = first_tile; j < ntiles && alive; ++j) {
       const int key0 = j * kKeys, slot = (j - jmin) & (kScaleRing - 1);
-      uint32_t gone = 0;                                  // groups of 16 keys without a page
-      // Whether every row of the warp sees the whole tile: most tiles of a long prompt.  (Rows behind the sequence's last see nothing,
-      // and leave it to the others.)
-      const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kKeys <= vis_end));
       if (!all_wait(my_s_full, (j - first_tile) & 1, 7)) { alive = false; break; }
       tc_fence_after();
-      if (!EIGHT) gone = no_page[slot];
-      // factor and summand of a group's exponents
-      auto group_factor = [&](int g) { return EIGHT ? factor * key_scale[slot * 8 + g] : factor; };
+      // groups of 16 keys without a page
+      const uint32_t gone = EIGHT ? 0 : no_page[slot];
+      // Which of 32 keys this row sees.  (Rows behind the sequence's last count as seeing all, which leaves it to the others.)
+      auto seen = [&](int c) {
+        const int end = vis_end - (key0 + c * 32), begin = vis_begin - (key0 + c * 32);
+        uint32_t bits = end >= 32 ? 0xffffffffu : end <= 0 ? 0u : (1u << end) - 1u;
+        if (begin > 0) bits &= begin >= 32 ? 0u : ~((1u << begin) - 1u);
+        if (!EIGHT && gone) bits &= ((gone >> (2 * c)) & 1 ? 0u : 0xffffu) | ((gone >> (2 * c)) & 2 ? 0u : 0xffff0000u);
+        return there ? bits : 0xffffffffu;
+      };
+      // most tiles of a long prompt: every row sees every key
+      const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kKeys <= vis_end)) && !gone;
+      auto hide = [&](float (&x)[32], int c) {
+        const uint32_t bits = seen(c);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1 ? x[e] : -INFINITY;
+      };
+      // factor and summand of a group's exponents (the factor is never 0, which would make a NaN of a hidden score)
+      auto group_factor = [&](int g) { return EIGHT ? fmaxf(factor * key_scale[slot * 8 + g], 1e-37f) : factor; };
       auto group_log = [&](int g) { return EIGHT ? value_log[slot * 8 + g] : 0.f; };
       auto largest = [&](const float (&x)[32], int c) {    // exponent of 32 keys
         float m = kNone;
@@ -383,11 +399,26 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
       };
-      // Before P is overwritten the previous tile's value product, which reads it, must be complete.  It was issued right behind the
-      // scores just read.
+      // Before P is overwritten the previous tile's value product, which reads it, must be complete.
       auto before_put = [&]() { return j == first_tile || all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8); };
-      bool done = false, tried = false;
-      if (whole && !gone && j > first_tile) {
+      auto release = [&]() {                               // S has been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) bar_arrive(my_s_free);
+      };
+      // The tile, with and without hidden keys: false if a wait ran out.
+      auto tile = [&](auto plain) -> bool {
+        constexpr bool kPlain = decltype(plain)::value;
+        if (!kPlain && j == first_tile) {
+          // the first reference: the first tile's maximum
+#pragma unroll 1
+          for (int c = 0; c < kKeys / 32; ++c) {
+            float x[32];
+            tc_ld32(t_s + c * 32, x);
+            hide(x, c);
+            m_ref = fmaxf(m_ref, largest(x, c));
+          }
+        }
         // One pass, with the reference as it is: where the first half's weights add up to no more than 2^8, none of them is above that, and of
         // the second half the maximum is taken.  Otherwise the tile is done again below.
         float x0[32], x1[32], sum = 0.f, l = 0.f;
@@ -395,18 +426,18 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
         tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
         tc_ld_wait_for(x0, x1);
+        if (!kPlain) hide(x0, 0);
         weigh(x0, 0, w0, sum, l);
         tc_ld32_issue(t_s + 64, reinterpret_cast<uint32_t *>(x0));
+        if (!kPlain) hide(x1, 1);
         weigh(x1, 1, w1, sum, l);
         tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
         tc_ld_wait_for(x0, x1);
-        // the other half's weights stay below 2^8 too: nothing will be done again, and the next scores may come
-        done = __all_sync(0xffffffffu, sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise);
-        if (done) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) bar_arrive(my_s_free);
-          if (!before_put()) { alive = false; break; }
+        if (!kPlain) hide(x0, 2);
+        if (!kPlain) hide(x1, 3);
+        if (__all_sync(0xffffffffu, !there || (sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise))) {
+          release();
+          if (!before_put()) return false;
           put(0, w0);
           put(1, w1);
           weigh(x0, 2, w0, sum, l);
@@ -414,86 +445,45 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
           weigh(x1, 3, w1, sum, l);
           put(3, w1);
           l_run += l;
-        }
-        tried = true;
-      }
-      if (!done) {
-        // Two passes, chunk by chunk of 32 keys: 0 = hidden from every row of the warp: P = 0; 1 = visible to every row; 2 = per key.
-        auto visible = [&](int key, int g) { return key < vis_end && key >= vis_begin && (EIGHT || !((gone >> g) & 1)); };
-        auto kind = [&](int c) {
-          const int kb = key0 + c * 32;
-          if (__all_sync(0xffffffffu, kb >= vis_end || kb + 32 <= vis_begin)) return 0;
-          return __all_sync(0xffffffffu, !there || (kb >= vis_begin && kb + 32 <= vis_end)) && !((gone >> (2 * c)) & 3) ? 1 : 2;
-        };
-        float m_tile = kNone;
+        } else {
+          // The reference is raised, for all rows of the warp (tensor memory is read and written warp-wide).
+          float m_new = m_ref;
 #pragma unroll 1
-        for (int c = 0; c < kKeys / 32; ++c) {
-          const int what = kind(c);
-          if (what == 0) continue;
-          float x[32];
-          tc_ld32(t_s + c * 32, x);
-          if (what == 2) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] = visible(key0 + c * 32 + e, 2 * c + (e >> 4)) ? x[e] : -INFINITY;
+          for (int c = 0; c < kKeys / 32; ++c) {
+            tc_ld32(t_s + c * 32, x0);
+            if (!kPlain) hide(x0, c);
+            m_new = fmaxf(m_new, largest(x0, c));
           }
-          m_tile = fmaxf(m_tile, largest(x, c));
-        }
-        if (!before_put()) { alive = false; break; }
-        // the reference is raised where some row exceeds it by 2^8 (or the one pass failed), and with it for all rows of the warp (tensor memory is read and written warp-wide)
-        if (__any_sync(0xffffffffu, m_tile > (tried ? m_ref : m_ref + kRaise))) {
-          const float m_new = fmaxf(m_ref, m_tile), alpha = ex2(m_ref - m_new);
+          if (!before_put()) return false;
+          const float alpha = ex2(m_ref - m_new);
           m_ref = m_new;
           l_run *= alpha;
           if (j > first_tile) {
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
-              float x[32];
-              tc_ld32(t_pv + c * 32, x);
+              tc_ld32(t_pv + c * 32, x0);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] *= alpha;
-              tc_st32(t_pv + c * 32, x);
+              for (int e = 0; e < 32; ++e) x0[e] *= alpha;
+              tc_st32(t_pv + c * 32, x0);
             }
             tc_st_wait();
           }
-        }
+          l = 0.f;
+          sum = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < kKeys / 32; ++c) {
-          const int what = kind(c);
-          float x[32], sum = 0.f, l = 0.f;
-          uint32_t w[16];
-          if (what == 0) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w[e] = 0;
-          } else {
-            tc_ld32(t_s + c * 32, x);
-            if (what == 2) {
-              // (selected behind the multiply-add: a factor that underflows to 0 would make a NaN of an infinity)
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const bool v = visible(key0 + c * 32 + e, 2 * c + (e >> 4));
-                x[e] = v ? ex2(fmaf(x[e], group_factor(2 * c + (e >> 4)), group_log(2 * c + (e >> 4)) - (m_ref - kLift))) : 0.f;
-              }
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float l0 = 0.f;
-#pragma unroll
-                for (int e = h * 16; e < h * 16 + 16; ++e) l0 += x[e];
-                l = EIGHT ? fmaf(l0, value_inv[slot * 8 + 2 * c + h], l) : l + l0;
-              }
-#pragma unroll
-              for (int e = 0; e < 16; ++e) w[e] = pack2<M>(x[2 * e], x[2 * e + 1]);
-            } else {
-              weigh(x, c, w, sum, l);
-            }
+          for (int c = 0; c < kKeys / 32; ++c) {
+            tc_ld32(t_s + c * 32, x0);
+            if (!kPlain) hide(x0, c);
+            weigh(x0, c, w0, sum, l);
+            put(c, w0);
           }
           l_run += l;
-          put(c, w);
+          release();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(my_s_free);
-      }
+        return true;
+      };
+      if (!(whole && j > first_tile ? tile(std::true_type{}) : tile(std::false_type{}))) { alive = false; break; }
       // P is complete for this warp's 32 rows (and these are rescaled): make it visible to the tensor core's reads.
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -532,7 +522,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       }
     }
   } else if (EIGHT && warp >= kConvertWarp) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ---------------- e4m3 codes: registers one tile ahead, fp16 into shared memory ----------------
     // Warp w has keys 32 w .. + 31 of a tile: a load takes kRowsPer rows, kLanesPer lanes of 16 codes each.
     constexpr int kOwn = kKeys / kConvertWarps, kLanesPer = D / 16, kRowsPer = 32 / kLanesPer, kLoads = kOwn / kRowsPer, kGroups = kOwn / 16;
@@ -638,6 +628,11 @@ template <typename T, bool EIGHT, int D> int launch_prompt(const CUtensorMap &mk
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem::kTotal) != cudaSuccess) {
       cudaGetLastError();
       return fail(EB_ECUDA, "paged_attention: cannot reserve %zu bytes of shared memory", Smem::kTotal);
+    }
+    cudaFuncAttributes attr{};
+    if (cudaFuncGetAttributes(&attr, kern) != cudaSuccess || attr.numRegs != (EIGHT ? 128 : 168)) {
+      cudaGetLastError();
+      return fail(EB_EUNSUPPORTED, "paged_attention: the kernel was built with %d registers, its roles share out %d", attr.numRegs, EIGHT ? 128 : 168);
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
