@@ -2,15 +2,16 @@
 // sequence's adapter, for the rows of a packed batch.  The projection beside it adds delta to its fp32 sums as a
 // residual, so that the result is rounded once (and delta, the smaller part, before).
 //
-// Two launches.  The first has x A^T: bound by reading x and the adapters that occur; a CTA takes 16 rows of one
-// sequence and a part of the columns, its warps take slices of that part, a lane loads 16 bytes of its row straight
-// into the fragments of mma.sync (the contraction runs over columns in any order), partial sums go to shared memory and,
-// where the columns are split over CTAs, to scratch, summed in order by the second launch.  That one has the
+// Two launches.  The first has x A^T: bound by reading x and the adapters that occur.  With up to 16 rows per sequence a CTA takes them and
+// a part of the columns, its warps take slices of that part, and a lane loads 16 bytes of its row straight
+// into the fragments of mma.sync (the contraction runs over columns in any order); the warps' sums meet in shared memory.  Longer sequences
+// go 64 rows at a time through shared memory, or every 16 rows would read the adapter again.  Where the columns are split over CTAs,
+// partial sums go to scratch, summed in order by the second launch.  That one has the
 // product with B^T: bound by writing delta.  The low-rank row stays fp32 between the two and enters the product as two
 // 16-bit pieces: it costs tensor time that is there, and no rounding.
 #include <type_traits>
 
-#include "common.cuh"
+#include "attention_mma.cuh"
 
 namespace eb {
 namespace {
@@ -29,13 +30,20 @@ struct AdapterParams {
 
 template <typename T> __device__ __forceinline__ void mma_low(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// two numbers as two 16-bit pieces each
+template <typename T> __device__ __forceinline__ void two_pieces(float x, float y, uint32_t &hi, uint32_t &lo) {
+  hi = pack2<T>(x, y);
+  const float2 f = unpack2<T>(hi);
+  lo = pack2<T>(x - f.x, y - f.y);
 }
 
 // Rows and adapter of sequence b; b = batch: the rows behind the last sequence, without one.
@@ -105,21 +113,91 @@ template <typename T, int NR> __global__ void __launch_bounds__(kAdapterWarps * 
   }
 }
 
-// delta[row][n] = s sum_r low[row][r] B[n][r].  KR: steps of 16 ranks.  MANY: the warps take 16 rows each of 64, else they
-// take turns over the columns of 16 rows.
-template <typename T, int KR, bool MANY> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_delta_kernel(const AdapterParams p) {
+// The same for many rows: 64 rows of a sequence, a split's columns in steps of 64 through shared memory (x and A, each read once per
+// CTA), four steps in flight.  RT: tiles of 16 ranks.
+constexpr int kLowRows = 64, kLowStep = 64, kLowStages = 4;
+template <int RT> struct LowSmem {
+  static constexpr int kX = kLowRows * kLowStep * 2, kA = RT * 16 * kLowStep * 2, kStage = kX + kA, kTotal = kLowStages * kStage;
+};
+template <typename T, int RT> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_low_many_kernel(const AdapterParams p) {
+  using S = LowSmem<RT>;
+  extern __shared__ __align__(128) uint8_t low_smem[];
+  griddep_wait();
+  griddep_launch();
+  const int split = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const AdapterRows r = adapter_rows(p, b);
+  const int t0 = blockIdx.x * kLowRows;
+  if (r.adapter < 0 || t0 >= r.count) return;
+  const int rows = min(kLowRows, r.count - t0), row0 = r.row0 + t0;
+  const T *x = reinterpret_cast<const T *>(p.x) + (long long)row0 * p.ldx, *a = reinterpret_cast<const T *>(p.a) + (long long)r.adapter * p.rank * p.width;
+  const int begin = split * p.per_split, end = min(p.width, begin + p.per_split), steps = (end - begin + kLowStep - 1) / kLowStep;
+  const uint32_t base = smem_u32(low_smem);
+  // 8 lanes per row of 64 columns; chunks XOR-swizzled with the row
+  auto fetch = [&](int i) {
+    if (i < steps) {
+      const uint32_t xs = base + (i % kLowStages) * S::kStage, as = xs + S::kX;
+      const int k0 = begin + i * kLowStep, chunk = threadIdx.x & 7, col = k0 + chunk * 8;
+      const bool in = col < end;
+#pragma unroll
+      for (int n = 0; n < kLowRows / 16; ++n) {
+        const int row = n * 16 + (threadIdx.x >> 3);
+        const bool ok = in && row < rows;
+        cp_async16(xs + tile_off<kLowStep>(row, chunk), ok ? x + (long long)row * p.ldx + col : x, ok);
+      }
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        const int row = n * 16 + (threadIdx.x >> 3);
+        const bool ok = in && row < p.rank;
+        cp_async16(as + tile_off<kLowStep>(row, chunk), ok ? a + (long long)row * p.width + col : a, ok);
+      }
+    }
+    cp_async_commit();
+  };
+  float acc[2 * RT][4];
+#pragma unroll
+  for (int n = 0; n < 2 * RT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  for (int i = 0; i < kLowStages - 1; ++i) fetch(i);
+  for (int i = 0; i < steps; ++i) {
+    cp_async_wait<kLowStages - 2>();
+    __syncthreads();
+    fetch(i + kLowStages - 1);                             // (into the stage that all warps are done with)
+    const uint32_t xs = base + (i % kLowStages) * S::kStage, as = xs + S::kX;
+    const int mrow = warp * 16 + (lane & 15), half = lane >> 4;
+#pragma unroll
+    for (int k = 0; k < kLowStep / 16; ++k) {
+      uint32_t xa[4], w[RT][4];                            // ranks 16 n .. + 7 and + 8 .. + 15, columns of the step's halves
+      ldmatrix_x4(xa, xs + tile_off<kLowStep>(mrow, 2 * k + half));
+#pragma unroll
+      for (int n = 0; n < RT; ++n) ldmatrix_x4(w[n], as + tile_off<kLowStep>(n * 16 + (lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        mma_low<T>(acc[2 * n], xa[0], xa[1], xa[2], xa[3], w[n][0], w[n][1]);
+        mma_low<T>(acc[2 * n + 1], xa[0], xa[1], xa[2], xa[3], w[n][2], w[n][3]);
+      }
+    }
+  }
+  float *low = p.low + ((long long)split * p.rows + row0) * p.rank;
+#pragma unroll
+  for (int n = 0; n < 2 * RT; ++n) {
+    const int k = n * 8 + 2 * c, r0 = warp * 16 + g;
+    if (k >= p.rank) continue;
+    if (r0 < rows) *reinterpret_cast<float2 *>(low + (long long)r0 * p.rank + k) = make_float2(acc[n][0], acc[n][1]);
+    if (r0 + 8 < rows) *reinterpret_cast<float2 *>(low + (long long)(r0 + 8) * p.rank + k) = make_float2(acc[n][2], acc[n][3]);
+  }
+}
+
+// delta[row][n] = s sum_r low[row][r] B[n][r], 16 rows of a sequence, the warps take turns over the columns.  KR: steps of 16 ranks.
+template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_delta_kernel(const AdapterParams p) {
   griddep_wait();
   griddep_launch();
   const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const AdapterRows r = adapter_rows(p, b);
-  constexpr int kRowsCta = MANY ? kAdapterWarps * kRowTile : kRowTile;
-  const int begin = blockIdx.y * p.chunk, end = min(p.columns, begin + p.chunk);
+  const int begin = blockIdx.y * p.chunk, end = min(p.columns, begin + p.chunk), first = begin + warp * 32, step = kAdapterWarps * 32;
   T *delta = reinterpret_cast<T *>(p.delta);
   // (the rows behind the last sequence may be more than the grid has tiles for)
-  for (int t0 = blockIdx.x * kRowsCta + (MANY ? warp * kRowTile : 0); t0 < r.count; t0 += gridDim.x * kRowsCta) {
+  for (int t0 = blockIdx.x * kRowTile; t0 < r.count; t0 += gridDim.x * kRowTile) {
     const int rows = min(kRowTile, r.count - t0), row0 = r.row0 + t0;
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
-    const int first = begin + (MANY ? 0 : warp * 32), step = MANY ? 32 : kAdapterWarps * 32;
     if (r.adapter < 0) {
       for (int n0 = first; n0 < end; n0 += step)
         if (n0 + c * 8 < end) {
@@ -128,37 +206,10 @@ template <typename T, int KR, bool MANY> __global__ void __launch_bounds__(kAdap
         }
       continue;
     }
-    const float s = p.scales[r.adapter];
-    // low-rank rows g and g + 8, ranks 16 k + 4 c .. + 3: two pieces each
-    uint32_t hi[KR][4], lo[KR][4];
-#pragma unroll
-    for (int k = 0; k < KR; ++k)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k * 16 + c * 4 < p.rank && g + 8 * h < rows)
-          for (int q = 0; q < p.splits; ++q) {
-            const float4 one = *reinterpret_cast<const float4 *>(p.low + ((long long)q * p.rows + row0 + g + 8 * h) * p.rank + k * 16 + c * 4);
-            v.x += one.x;
-            v.y += one.y;
-            v.z += one.z;
-            v.w += one.w;
-          }
-        v.x *= s;
-        v.y *= s;
-        v.z *= s;
-        v.w *= s;
-        hi[k][h] = pack2<T>(v.x, v.y);
-        hi[k][h + 2] = pack2<T>(v.z, v.w);
-        const float2 f0 = unpack2<T>(hi[k][h]), f1 = unpack2<T>(hi[k][h + 2]);
-        lo[k][h] = pack2<T>(v.x - f0.x, v.y - f0.y);
-        lo[k][h + 2] = pack2<T>(v.z - f1.x, v.w - f1.y);
-      }
     const T *bm = reinterpret_cast<const T *>(p.b) + (long long)r.adapter * p.columns * p.rank + c * 4;
-    for (int n0 = first; n0 < end; n0 += step) {
-      // column i of tile t is n0 + 8 (i / 2) + 2 t + i % 2: lane c ends up with 8 columns that follow one another
-      float acc[4][4];
-      uint2 w[4][KR];
+    // column i of tile t is n0 + 8 (i / 2) + 2 t + i % 2: lane c ends up with 8 columns that follow one another
+    uint2 w[4][KR];
+    auto fetch = [&](int n0) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int n = n0 + g / 2 * 8 + 2 * t + g % 2;
@@ -166,6 +217,32 @@ template <typename T, int KR, bool MANY> __global__ void __launch_bounds__(kAdap
         for (int k = 0; k < KR; ++k)
           w[t][k] = n < end && k * 16 + c * 4 < p.rank ? __ldg(reinterpret_cast<const uint2 *>(bm + (long long)n * p.rank + k * 16)) : make_uint2(0, 0);
       }
+    };
+    fetch(first);
+    const float s = p.scales[r.adapter];
+    // low-rank rows g and g + 8, ranks 16 k + 4 c .. + 3: two pieces each
+    uint32_t hi[KR][4], lo[KR][4];
+    {
+      float4 v[KR][2] = {};
+      for (int q = 0; q < p.splits; ++q)                   // (a split's loads together)
+#pragma unroll
+        for (int k = 0; k < KR; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (k * 16 + c * 4 < p.rank && g + 8 * h < rows) {
+              const float4 one = *reinterpret_cast<const float4 *>(p.low + ((long long)q * p.rows + row0 + g + 8 * h) * p.rank + k * 16 + c * 4);
+              v[k][h] = make_float4(v[k][h].x + one.x, v[k][h].y + one.y, v[k][h].z + one.z, v[k][h].w + one.w);
+            }
+#pragma unroll
+      for (int k = 0; k < KR; ++k)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          two_pieces<T>(v[k][h].x * s, v[k][h].y * s, hi[k][h], lo[k][h]);
+          two_pieces<T>(v[k][h].z * s, v[k][h].w * s, hi[k][h + 2], lo[k][h + 2]);
+        }
+    }
+    for (int n0 = first; n0 < end; n0 += step) {
+      float acc[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
@@ -175,6 +252,7 @@ template <typename T, int KR, bool MANY> __global__ void __launch_bounds__(kAdap
           mma_low<T>(acc[t], hi[k][0], hi[k][1], hi[k][2], hi[k][3], w[t][k].x, w[t][k].y);
         }
       }
+      fetch(n0 + step);                                    // (the next columns, while these are stored)
       if (n0 + c * 8 < end) {
         if (g < rows)
           *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(pack2<T>(acc[0][0], acc[0][1]), pack2<T>(acc[1][0], acc[1][1]), pack2<T>(acc[2][0], acc[2][1]), pack2<T>(acc[3][0], acc[3][1]));
@@ -185,48 +263,186 @@ template <typename T, int KR, bool MANY> __global__ void __launch_bounds__(kAdap
   }
 }
 
+// The same for 64 rows of a sequence, 16 per warp; B comes through shared memory, 128 columns at a time, two steps ahead.  (Loaded to
+// registers by every warp, 8 bytes of eight rows at a time, it kept the first-level cache busy for 48 us where this takes 19:
+// 6144 columns, rank 64, 4000 rows.)  The rows of 32 columns lie in the order in which the tiles use them, so that a tile's
+// eight rows follow one another; their chunks of 16 bytes are XOR-swizzled.
+constexpr int kDeltaCols = 128, kDeltaStages = 3;
+template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_delta_many_kernel(const AdapterParams p) {
+  constexpr int kChunks = 2 * KR, kRowBytes = 32 * KR, kStage = kDeltaCols * kRowBytes;
+  extern __shared__ __align__(128) uint8_t delta_smem[];
+  griddep_wait();
+  griddep_launch();
+  const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const AdapterRows r = adapter_rows(p, b);
+  const int begin = blockIdx.y * p.chunk, end = min(p.columns, begin + p.chunk), steps = (end - begin + kDeltaCols - 1) / kDeltaCols;
+  const uint32_t base = smem_u32(delta_smem);
+  T *delta = reinterpret_cast<T *>(p.delta);
+  // chunk of row i of a tile's eight
+  auto swizzled = [](int i, int chunk) { return KR == 1 ? chunk ^ (i >> 2) : KR == 2 ? chunk ^ (i >> 1) : chunk ^ i; };
+  for (int t0 = blockIdx.x * kLowRows; t0 < r.count; t0 += gridDim.x * kLowRows) {
+    const int rows = min(kRowTile, r.count - t0 - warp * kRowTile), row0 = r.row0 + t0 + warp * kRowTile;      // (of this warp; none: <= 0)
+    T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
+    if (r.adapter < 0) {
+      for (int n0 = begin; n0 < end; n0 += 32)
+        if (n0 + c * 8 < end) {
+          if (g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
+          if (g + 8 < rows) *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(0, 0, 0, 0);
+        }
+      continue;
+    }
+    const T *bm = reinterpret_cast<const T *>(p.b) + (long long)r.adapter * p.columns * p.rank;
+    auto fetch = [&](int i) {
+      if (i < steps) {
+        const uint32_t at = base + (i % kDeltaStages) * kStage;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < kDeltaCols * kChunks; e += kAdapterWarps * 32) {
+          const int col = e / kChunks, chunk = e % kChunks, n = begin + i * kDeltaCols + col, in = col & 31;
+          const int tile = (in & 7) >> 1, row = (in >> 3) * 2 + (in & 1);
+          const bool ok = n < end && chunk * 8 < p.rank;
+          cp_async16(at + ((col & ~31) + tile * 8 + row) * kRowBytes + swizzled(row, chunk) * 16, ok ? bm + (long long)n * p.rank + chunk * 8 : bm, ok);
+        }
+      }
+      cp_async_commit();
+    };
+    __syncthreads();                                       // (the stages of the rows before are done with)
+    for (int i = 0; i < kDeltaStages - 1; ++i) fetch(i);
+    const float s = p.scales[r.adapter];
+    // The low-rank rows, summed over the splits in order by whoever comes across 4 ranks of a row, then as two pieces each through shared
+    // memory to the fragments.  (Each lane gathering its own fragments took 10 us.)
+    constexpr int kPieces = kLowRows * kRowBytes;
+    const uint32_t at_hi = base + kDeltaStages * kStage, at_lo = at_hi + kPieces;
+    uint8_t *pieces = delta_smem + kDeltaStages * kStage;
+    const int all = min(kLowRows, r.count - t0), quads = p.rank / 4;
+    for (int e = threadIdx.x; e < kLowRows * KR * 4; e += kAdapterWarps * 32) {
+      const int row = e / (KR * 4), quad = e % (KR * 4);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < all && quad < quads) {
+        const float4 *from = reinterpret_cast<const float4 *>(p.low + ((long long)r.row0 + t0 + row) * p.rank) + quad;
+#pragma unroll 4
+        for (int q = 0; q < p.splits; ++q) {
+          const float4 one = from[(long long)q * p.rows * quads];
+          v = make_float4(v.x + one.x, v.y + one.y, v.z + one.z, v.w + one.w);
+        }
+      }
+      uint2 hi2, lo2;
+      two_pieces<T>(v.x * s, v.y * s, hi2.x, lo2.x);
+      two_pieces<T>(v.z * s, v.w * s, hi2.y, lo2.y);
+      const int to = row * kRowBytes + swizzled(row & 7, quad >> 1) * 16 + (quad & 1) * 8;
+      *reinterpret_cast<uint2 *>(pieces + to) = hi2;
+      *reinterpret_cast<uint2 *>(pieces + kPieces + to) = lo2;
+    }
+    __syncthreads();
+    uint32_t hi[KR][4], lo[KR][4];
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+      const int row = warp * kRowTile + (lane & 15), to = row * kRowBytes + swizzled(row & 7, 2 * k + (lane >> 4)) * 16;
+      ldmatrix_x4(hi[k], at_hi + to);
+      ldmatrix_x4(lo[k], at_lo + to);
+    }
+    for (int i = 0; i < steps; ++i) {
+      cp_async_wait<kDeltaStages - 2>();
+      __syncthreads();
+      fetch(i + kDeltaStages - 1);
+      const uint32_t at = base + (i % kDeltaStages) * kStage;
+      for (int n0 = 0; n0 < kDeltaCols; n0 += 32) {
+        float acc[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        constexpr int kTogether = KR < 4 ? KR : 4;           // steps whose operands are loaded before the first product
+#pragma unroll
+        for (int k0 = 0; k0 < KR; k0 += kTogether) {
+          uint32_t w[kTogether][2][4];                     // tiles t and t + 1, ranks 16 k .. + 7 and + 8 .. + 15 each
+#pragma unroll
+          for (int k = 0; k < kTogether; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              ldmatrix_x4(w[k][t], at + (n0 + (2 * t + (lane >> 4)) * 8 + (lane & 7)) * kRowBytes + swizzled(lane & 7, 2 * (k0 + k) + ((lane >> 3) & 1)) * 16);
+          // (four products that do not wait for one another, then the next four on the same sums)
+#pragma unroll
+          for (int k = 0; k < kTogether; ++k) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              mma_low<T>(acc[t], lo[k0 + k][0], lo[k0 + k][1], lo[k0 + k][2], lo[k0 + k][3], w[k][t / 2][2 * (t & 1)], w[k][t / 2][2 * (t & 1) + 1]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              mma_low<T>(acc[t], hi[k0 + k][0], hi[k0 + k][1], hi[k0 + k][2], hi[k0 + k][3], w[k][t / 2][2 * (t & 1)], w[k][t / 2][2 * (t & 1) + 1]);
+          }
+        }
+        const int n = begin + i * kDeltaCols + n0;
+        if (n + c * 8 < end) {
+          if (g < rows)
+            *reinterpret_cast<uint4 *>(out0 + n) = make_uint4(pack2<T>(acc[0][0], acc[0][1]), pack2<T>(acc[1][0], acc[1][1]), pack2<T>(acc[2][0], acc[2][1]), pack2<T>(acc[3][0], acc[3][1]));
+          if (g + 8 < rows)
+            *reinterpret_cast<uint4 *>(out1 + n) = make_uint4(pack2<T>(acc[0][2], acc[0][3]), pack2<T>(acc[1][2], acc[1][3]), pack2<T>(acc[2][2], acc[2][3]), pack2<T>(acc[3][2], acc[3][3]));
+        }
+      }
+    }
+  }
+}
+
 struct AdapterPlan {
+  bool many;
   int tiles, splits, per_split;
 };
 AdapterPlan adapter_plan(int batch, int most_new, int width) {
   AdapterPlan s;
-  s.tiles = (most_new + kRowTile - 1) / kRowTile;
+  s.many = most_new > kRowTile;
+  const int rows = s.many ? kLowRows : kRowTile, turn = s.many ? kLowStep : kAdapterWarps * 32;
+  s.tiles = (most_new + rows - 1) / rows;
   const long long ctas = (long long)s.tiles * batch;
-  const int turns = (width + kAdapterWarps * 32 - 1) / (kAdapterWarps * 32);          // of the warps over all columns
-  int want = (int)((2ll * sm_count() + ctas - 1) / ctas);
-  if (want > turns / 4) want = turns / 4 > 0 ? turns / 4 : 1;
+  const int turns = (width + turn - 1) / turn, least = s.many ? 8 : 4;                  // turns of the CTA over its columns, at least
+  int want = (int)(((s.many ? 3ll : 2ll) * sm_count() + ctas - 1) / ctas);
+  if (want > turns / least) want = turns / least > 0 ? turns / least : 1;
   const int per = (turns + want - 1) / want;
   s.splits = (turns + per - 1) / per;
-  s.per_split = per * kAdapterWarps * 32;
+  s.per_split = per * turn;
   return s;
 }
 
-template <typename T, int NR> void launch_low(const AdapterParams &p, const AdapterPlan &s, cudaStream_t st) {
-  launch_pdl(adapter_low_kernel<T, NR>, dim3(s.tiles, s.splits, p.batch), dim3(kAdapterWarps * 32), 0, st, p);
+template <typename T, int NR> int launch_low(const AdapterParams &p, const AdapterPlan &s, cudaStream_t st) {
+  const dim3 grid(s.tiles, s.splits, p.batch), block(kAdapterWarps * 32);
+  if (!s.many) {
+    launch_pdl(adapter_low_kernel<T, NR>, grid, block, 0, st, p);
+    return EB_OK;
+  }
+  constexpr int RT = (NR + 1) / 2, kSmem = LowSmem<RT>::kTotal;
+  auto kern = adapter_low_many_kernel<T, RT>;
+  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(EB_ECUDA, "adapter_delta: cannot reserve %d bytes of shared memory", kSmem);
+  }
+  launch_pdl(kern, grid, block, kSmem, st, p);
+  return EB_OK;
 }
-template <typename T, int KR> void launch_delta(AdapterParams p, int most_new, cudaStream_t st) {
-  const bool many = most_new > kRowTile;
-  const int rows = many ? kAdapterWarps * kRowTile : kRowTile, tiles = (most_new + rows - 1) / rows;
+template <typename T, int KR> int launch_delta(AdapterParams p, const AdapterPlan &s, cudaStream_t st) {
   // columns per CTA: enough CTAs for four on every multiprocessor, no fewer columns than a turn of the warps
-  const long long ctas = (long long)tiles * p.batch;
-  const int turn = many ? 32 : kAdapterWarps * 32, turns = (p.columns + turn - 1) / turn;
+  const long long ctas = (long long)s.tiles * p.batch;
+  const int turns = (p.columns + kDeltaCols - 1) / kDeltaCols;
   const long long want = (4ll * sm_count() + ctas - 1) / ctas;
   const int parts = (int)(want < turns ? want : turns);
-  p.chunk = (turns + parts - 1) / parts * turn;
-  const dim3 grid(tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch + 1);
-  if (many) launch_pdl(adapter_delta_kernel<T, KR, true>, grid, dim3(kAdapterWarps * 32), 0, st, p);
-  else launch_pdl(adapter_delta_kernel<T, KR, false>, grid, dim3(kAdapterWarps * 32), 0, st, p);
+  p.chunk = (turns + parts - 1) / parts * kDeltaCols;
+  static_assert(kDeltaCols == kAdapterWarps * 32, "a turn of either form");
+  const dim3 grid(s.tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch + 1), block(kAdapterWarps * 32);
+  if (!s.many) {
+    launch_pdl(adapter_delta_kernel<T, KR>, grid, block, 0, st, p);
+    return EB_OK;
+  }
+  constexpr int kSmem = (kDeltaStages * kDeltaCols + 2 * kLowRows) * 32 * KR;
+  auto kern = adapter_delta_many_kernel<T, KR>;
+  if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(EB_ECUDA, "adapter_delta: cannot reserve %d bytes of shared memory", kSmem);
+  }
+  launch_pdl(kern, grid, block, kSmem, st, p);
+  return EB_OK;
 }
-template <typename T> int launch_adapter(const AdapterParams &p, const AdapterPlan &s, int most_new, cudaStream_t st) {
-  if (p.rank <= 8) launch_low<T, 1>(p, s, st);
-  else if (p.rank <= 16) launch_low<T, 2>(p, s, st);
-  else if (p.rank <= 32) launch_low<T, 4>(p, s, st);
-  else if (p.rank <= 64) launch_low<T, 8>(p, s, st);
-  else launch_low<T, 16>(p, s, st);
-  if (p.rank <= 16) launch_delta<T, 1>(p, most_new, st);
-  else if (p.rank <= 32) launch_delta<T, 2>(p, most_new, st);
-  else if (p.rank <= 64) launch_delta<T, 4>(p, most_new, st);
-  else launch_delta<T, 8>(p, most_new, st);
+template <typename T> int launch_adapter(const AdapterParams &p, const AdapterPlan &s, cudaStream_t st) {
+  int rc = p.rank <= 8 ? launch_low<T, 1>(p, s, st) : p.rank <= 16 ? launch_low<T, 2>(p, s, st) : p.rank <= 32 ? launch_low<T, 4>(p, s, st)
+                 : p.rank <= 64 ? launch_low<T, 8>(p, s, st) : launch_low<T, 16>(p, s, st);
+  if (rc != EB_OK) return rc;
+  rc = p.rank <= 16 ? launch_delta<T, 1>(p, s, st) : p.rank <= 32 ? launch_delta<T, 2>(p, s, st) : p.rank <= 64 ? launch_delta<T, 4>(p, s, st) : launch_delta<T, 8>(p, s, st);
+  if (rc != EB_OK) return rc;
   return check_launch("adapter_delta");
 }
 
@@ -259,5 +475,5 @@ extern "C" int eb_adapter_delta(const void *x, long long ldx, const void *a, con
   p.x = x; p.a = a; p.b = b; p.scales = scales; p.index = index; p.starts = starts; p.delta = delta; p.low = reinterpret_cast<float *>(scratch);
   p.ldx = ldx; p.ldd = ldd; p.rows = rows; p.width = width; p.columns = columns; p.rank = rank; p.count = adapters; p.batch = batch;
   p.splits = s.splits; p.per_split = s.per_split;
-  return dtype == EB_F16 ? launch_adapter<__half>(p, s, most_new, as_stream(stream)) : launch_adapter<__nv_bfloat16>(p, s, most_new, as_stream(stream));
+  return dtype == EB_F16 ? launch_adapter<__half>(p, s, as_stream(stream)) : launch_adapter<__nv_bfloat16>(p, s, as_stream(stream));
 }

@@ -41,7 +41,7 @@ struct StepParams {
   const void *k_pages, *v_pages;
   const float *k_scale, *v_scale;
   int kv_heads, group, window, few;      // few: sequences with more rows (tokens x group) than this are left to the prompt kernel
-  int row_tiles, chunk;                  // tiles of query rows, keys per CTA
+  int row_tiles, tile_rows, chunk;       // tiles of query rows, rows of a tile (of the largest one), keys per CTA
   float scale_log2;
   float *part;                           // [batch][kv_heads][row tiles][splits][rows][D + 2], or null: one split
   int splits;
@@ -414,17 +414,20 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
   }
 }
 
-// A row of the output from its splits (D values, maximum, sum; `stride` floats apart), in order, by a warp.
+// A row of the output from its splits (D values, maximum, sum; `stride` floats apart) by the four warps of a CTA: each adds up
+// every fourth split, in order, then the warps' sums are added in order.
+constexpr int kMergeWarps = 4;
 template <typename T, int D> __device__ __forceinline__ void merge_row(const float *in, int stride, int splits, T *out) {
   constexpr int kPer = D / 32;
-  const int lane = threadIdx.x & 31;
+  __shared__ float sums[kMergeWarps][D + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float m = -3.402823466e38f, l = 0.f, x[kPer];
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, in[(long long)s * stride + D]);
   m = warp_max(m);
 #pragma unroll
   for (int e = 0; e < kPer; ++e) x[e] = 0.f;
 #pragma unroll 8
-  for (int s = 0; s < splits; ++s) {
+  for (int s = warp; s < splits; s += kMergeWarps) {
     const float *one = in + (long long)s * stride;
     const float2 ml = *reinterpret_cast<const float2 *>(one + D);
     const float a = pow2(ml.x - m);
@@ -436,16 +439,28 @@ template <typename T, int D> __device__ __forceinline__ void merge_row(const flo
       x[e + 1] = fmaf(v.y, a, x[e + 1]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t *>(out + lane * kPer + e) = pack2<T>(x[e] * inv, x[e + 1] * inv);
+  for (int e = 0; e < kPer; ++e) sums[warp][lane * kPer + e] = x[e];
+  if (lane == 0) sums[warp][D] = l;
+  __syncthreads();
+  if (threadIdx.x < D / 2) {
+    float y0 = 0.f, y1 = 0.f, all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+      y0 += sums[w][2 * threadIdx.x];
+      y1 += sums[w][2 * threadIdx.x + 1];
+      all += sums[w][D];
+    }
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    *reinterpret_cast<uint32_t *>(out + 2 * threadIdx.x) = pack2<T>(y0 * inv, y1 * inv);
+  }
 }
 
 template <typename T, int D, int NT> __global__ void __launch_bounds__(128) paged_merge_kernel(const StepParams p) {
   constexpr int kRowsT = 8 * NT;
   griddep_wait();
   griddep_launch();
-  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z, row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z, row = blockIdx.x;
   const PagedRows r = paged_rows(p.batch, b);
   if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
   const StepTile t = step_tile(p, r, rt, kRowsT);
@@ -461,7 +476,7 @@ template <typename T, int D> __global__ void __launch_bounds__(128) paged_prompt
   constexpr int kBlock = 256;
   griddep_wait();
   griddep_launch();
-  const int hk = blockIdx.y, b = blockIdx.z, all = blockIdx.x * 4 + (threadIdx.x >> 5), qb = all / kBlock;
+  const int hk = blockIdx.y, b = blockIdx.z, all = blockIdx.x, qb = all / kBlock;
   const PagedRows r = paged_rows(p.batch, b);
   const int count = r.count * p.group;
   if (count <= p.few || all >= count) return;
@@ -476,7 +491,7 @@ template <typename T, int D> __global__ void __launch_bounds__(128) paged_prompt
 
 template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParams &p, cudaStream_t st) {
   launch_pdl(paged_step_kernel<T, EIGHT, D, NT>, dim3(p.splits, p.kv_heads * p.row_tiles, p.batch.batch), dim3(kStepWarps * 32), 0, st, p);
-  if (p.part) launch_pdl(paged_merge_kernel<T, D, NT>, dim3(2 * NT, p.kv_heads * p.row_tiles, p.batch.batch), dim3(128), 0, st, p);
+  if (p.part) launch_pdl(paged_merge_kernel<T, D, NT>, dim3(p.tile_rows, p.kv_heads * p.row_tiles, p.batch.batch), dim3(128), 0, st, p);
   return check_launch("paged_attention");
 }
 
@@ -488,7 +503,7 @@ StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys) {
   StepPlan s;
   s.tiles8 = rows_per_head > 8 ? 2 : 1;
   s.row_tiles = (rows_per_head + 8 * s.tiles8 - 1) / (8 * s.tiles8);
-  const long long units = (long long)batch * kv_heads * s.row_tiles, want = (8ll * sm_count() + units - 1) / units;
+  const long long units = (long long)batch * kv_heads * s.row_tiles, want = (4ll * sm_count() + units - 1) / units;
   keys += 15;                                               // (the first tile may begin in front of the first key)
   long long chunk = (keys + want - 1) / want, least = (keys + 511) / 512;
   if (chunk < 256) chunk = 256;
@@ -533,7 +548,7 @@ PagedPlan paged_plan(int batch, int kv_heads, int group, int head_dim, int most_
 }
 
 template <typename T, int D> void launch_prompt_merge(const PromptParams &p, const PromptPlan &s, cudaStream_t st) {
-  launch_pdl(paged_prompt_merge_kernel<T, D>, dim3(s.blocks * 64, p.kv_heads, p.batch.batch), dim3(128), 0, st, p, s.blocks);
+  launch_pdl(paged_prompt_merge_kernel<T, D>, dim3(s.blocks * 256, p.kv_heads, p.batch.batch), dim3(128), 0, st, p, s.blocks);
 }
 
 }  // namespace
@@ -576,7 +591,7 @@ extern "C" int eb_paged_attention(const void *q, long long ldq, void *out, long 
   const size_t need = plan.step_bytes + plan.prompt_bytes;
   EB_REQUIRE(need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= need), "paged_attention: %zu bytes of scratch needed, %zu given", need, scratch_bytes);
   p.q = q; p.o = out; p.ldq = ldq; p.ldo = ldo; p.k_pages = k_pages; p.v_pages = v_pages; p.k_scale = k_scale; p.v_scale = v_scale;
-  p.kv_heads = kv_heads; p.group = group; p.window = window; p.few = kFewRows; p.row_tiles = s.row_tiles; p.chunk = s.chunk; p.splits = s.splits;
+  p.kv_heads = kv_heads; p.group = group; p.window = window; p.few = kFewRows; p.row_tiles = s.row_tiles; p.tile_rows = plan.step_rows < 8 * s.tiles8 ? plan.step_rows : 8 * s.tiles8; p.chunk = s.chunk; p.splits = s.splits;
   p.scale_log2 = scale * kLog2eStep; p.part = plan.step_bytes ? reinterpret_cast<float *>(scratch) : nullptr;
   cudaStream_t st = as_stream(stream);
   int rc;

@@ -406,21 +406,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         __syncwarp();
         if (lane == 0) bar_arrive(my_s_free);
       };
-      // The tile, with and without hidden keys: false if a wait ran out.
-      auto tile = [&](auto plain) -> bool {
+      // One pass, with the reference as it is, with or without hidden keys: where the first half's weights add up to no more than 2^8,
+      // none of them is above that, and of the second half the maximum is taken.  Otherwise the tile is done again below.
+      enum { kOut, kDone, kAgain };
+      auto pass = [&](auto plain) -> int {
         constexpr bool kPlain = decltype(plain)::value;
-        if (!kPlain && j == first_tile) {
-          // the first reference: the first tile's maximum
-#pragma unroll 1
-          for (int c = 0; c < kKeys / 32; ++c) {
-            float x[32];
-            tc_ld32(t_s + c * 32, x);
-            hide(x, c);
-            m_ref = fmaxf(m_ref, largest(x, c));
-          }
-        }
-        // One pass, with the reference as it is: where the first half's weights add up to no more than 2^8, none of them is above that, and of
-        // the second half the maximum is taken.  Otherwise the tile is done again below.
         float x0[32], x1[32], sum = 0.f, l = 0.f;
         uint32_t w0[16], w1[16];
         tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
@@ -435,55 +425,61 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         tc_ld_wait_for(x0, x1);
         if (!kPlain) hide(x0, 2);
         if (!kPlain) hide(x1, 3);
-        if (__all_sync(0xffffffffu, !there || (sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise))) {
-          release();
-          if (!before_put()) return false;
-          put(0, w0);
-          put(1, w1);
-          weigh(x0, 2, w0, sum, l);
-          put(2, w0);
-          weigh(x1, 3, w1, sum, l);
-          put(3, w1);
-          l_run += l;
-        } else {
-          // The reference is raised, for all rows of the warp (tensor memory is read and written warp-wide).
-          float m_new = m_ref;
-#pragma unroll 1
-          for (int c = 0; c < kKeys / 32; ++c) {
-            tc_ld32(t_s + c * 32, x0);
-            if (!kPlain) hide(x0, c);
-            m_new = fmaxf(m_new, largest(x0, c));
-          }
-          if (!before_put()) return false;
-          const float alpha = ex2(m_ref - m_new);
-          m_ref = m_new;
-          l_run *= alpha;
-          if (j > first_tile) {
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              tc_ld32(t_pv + c * 32, x0);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x0[e] *= alpha;
-              tc_st32(t_pv + c * 32, x0);
-            }
-            tc_st_wait();
-          }
-          l = 0.f;
-          sum = 0.f;
-#pragma unroll 1
-          for (int c = 0; c < kKeys / 32; ++c) {
-            tc_ld32(t_s + c * 32, x0);
-            if (!kPlain) hide(x0, c);
-            weigh(x0, c, w0, sum, l);
-            put(c, w0);
-          }
-          l_run += l;
-          release();
-        }
-        return true;
+        if (!__all_sync(0xffffffffu, !there || (sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise))) return kAgain;
+        release();
+        if (!before_put()) return kOut;
+        put(0, w0);
+        put(1, w1);
+        weigh(x0, 2, w0, sum, l);
+        put(2, w0);
+        weigh(x1, 3, w1, sum, l);
+        put(3, w1);
+        l_run += l;
+        return kDone;
       };
-      if (!(whole && j > first_tile ? tile(std::true_type{}) : tile(std::false_type{}))) { alive = false; break; }
+      int how = kAgain;
+      if (j > first_tile) how = whole ? pass(std::true_type{}) : pass(std::false_type{});
+      if (how == kAgain) {
+        // The first tile, and where the reference has to be raised, for all rows of the warp (tensor memory is read and written warp-wide):
+        // a pass for the maximum, one for the weights.
+        float m_new = m_ref;
+#pragma unroll 1
+        for (int c = 0; c < kKeys / 32; ++c) {
+          float x[32];
+          tc_ld32(t_s + c * 32, x);
+          if (!whole) hide(x, c);
+          m_new = fmaxf(m_new, largest(x, c));
+        }
+        how = before_put() ? kDone : kOut;
+        const float alpha = ex2(m_ref - m_new);
+        m_ref = m_new;
+        l_run *= alpha;
+        if (j > first_tile && how == kDone) {
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float x[32];
+            tc_ld32(t_pv + c * 32, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] *= alpha;
+            tc_st32(t_pv + c * 32, x);
+          }
+          tc_st_wait();
+        }
+        float sum = 0.f, l = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < kKeys / 32; ++c) {
+          float x[32];
+          uint32_t w[16];
+          tc_ld32(t_s + c * 32, x);
+          if (!whole) hide(x, c);
+          weigh(x, c, w, sum, l);
+          put(c, w);
+        }
+        l_run += l;
+        release();
+      }
+      if (how == kOut) { alive = false; break; }
       // P is complete for this warp's 32 rows (and these are rescaled): make it visible to the tensor core's reads.
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
