@@ -1,11 +1,18 @@
 """Python entry to the low-rank adapters of many requests (eb_adapter_delta) beside a shared projection."""
+import functools
+
 import torch
 
-from ._lib import lib, check, dtype_code, ptr, stream_ptr
+from ._lib import lib, check, dtype_code
 from .gemm import gemm
-from .paged import _one_device, _rows
+from .paged import _one_device, _rows, _stream_of
 
 MAX_RANK = 128
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(*sizes):
+    return lib().eb_adapter_scratch_bytes(*sizes)
 
 
 def adapter_delta(x, a, b, scales, index, starts, most_new):
@@ -13,23 +20,27 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
     i = index[s] for the rows starts[s] to starts[s + 1] - 1 of sequence s (at most most_new).  a [adapters, rank, width], b
     [adapters, columns, rank], scales fp32 [adapters]; index int32 [batch], negative for none; starts int32 [batch + 1].  rank is
     a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows behind the last sequence get zeros."""
-    _one_device("adapter_delta", x, a, b, scales, index, starts)
-    if a.dim() != 3 or b.dim() != 3 or x.dim() != 2 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.shape[2] != x.shape[1]:
+    device = _one_device("adapter_delta", x, a, b, scales, index, starts)
+    dtype, shape, of, to = x.dtype, x.shape, a.shape, b.shape
+    if len(of) != 3 or len(to) != 3 or len(shape) != 2 or of[0] != to[0] or of[1] != to[2] or of[2] != shape[1]:
         raise RuntimeError("adapter_delta: x [rows, width], a [adapters, rank, width] and b [adapters, columns, rank] required")
-    if a.dtype != x.dtype or b.dtype != x.dtype or not a.is_contiguous() or not b.is_contiguous():
+    if a.dtype is not dtype or b.dtype is not dtype or not a.is_contiguous() or not b.is_contiguous():
         raise RuntimeError("adapter_delta: adapters are contiguous and of the type of x")
-    adapters, rank, width = a.shape
-    if scales.dtype != torch.float32 or tuple(scales.shape) != (adapters,) or not scales.is_contiguous():
+    adapters, rank, width = of
+    if scales.dtype is not torch.float32 or scales.shape != (adapters,) or not scales.is_contiguous():
         raise RuntimeError("adapter_delta: one fp32 scale per adapter")
-    if any(t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() for t in (index, starts)) or starts.numel() != index.numel() + 1 or index.numel() == 0:
+    batch = index.numel()
+    if index.dtype is not torch.int32 or starts.dtype is not torch.int32 or index.dim() != 1 or starts.shape != (batch + 1,) or batch == 0 or not (
+            index.is_contiguous() and starts.is_contiguous()):
         raise RuntimeError("adapter_delta: int32 index [batch] and starts [batch + 1] required")
-    rows, columns, batch = x.shape[0], b.shape[1], index.numel()
-    ldx = _rows("adapter_delta", x, width, x.dtype)
-    delta = torch.empty((rows, columns), dtype=x.dtype, device=x.device)
-    nbytes = lib().eb_adapter_scratch_bytes(rows, width, rank, batch, int(most_new))
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None       # (of this call: captured calls share none)
-    check(lib().eb_adapter_delta(ptr(x), ldx, ptr(a), ptr(b), ptr(scales), ptr(index), ptr(starts), ptr(delta), columns, rows, width, columns, rank, adapters,
-                                 batch, int(most_new), dtype_code(x.dtype), ptr(scratch), nbytes, stream_ptr()), "adapter_delta", launches=2)
+    rows, columns, most_new = shape[0], to[1], int(most_new)
+    ldx = _rows("adapter_delta", x, width, dtype)
+    delta = x.new_empty((rows, columns))
+    nbytes = _scratch_bytes(rows, width, rank, batch, most_new)
+    scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None       # (of this call: captured calls share none)
+    check(lib().eb_adapter_delta(x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), index.data_ptr(), starts.data_ptr(), delta.data_ptr(), columns,
+                                 rows, width, columns, rank, adapters, batch, most_new, dtype_code(dtype), None if scratch is None else scratch.data_ptr(),
+                                 nbytes, _stream_of(device)), "adapter_delta", launches=2)
     return delta
 
 

@@ -224,6 +224,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
     uint32_t hi[KR][4], lo[KR][4];
     {
       float4 v[KR][2] = {};
+#pragma unroll 4
       for (int q = 0; q < p.splits; ++q)                   // (a split's loads together)
 #pragma unroll
         for (int k = 0; k < KR; ++k)
@@ -392,7 +393,7 @@ AdapterPlan adapter_plan(int batch, int most_new, int width) {
   s.tiles = (most_new + rows - 1) / rows;
   const long long ctas = (long long)s.tiles * batch;
   const int turns = (width + turn - 1) / turn, least = s.many ? 8 : 4;                  // turns of the CTA over its columns, at least
-  int want = (int)(((s.many ? 3ll : 2ll) * sm_count() + ctas - 1) / ctas);
+  int want = (int)(((s.many ? 3ll : 4ll) * sm_count() + ctas - 1) / ctas);
   if (want > turns / least) want = turns / least > 0 ? turns / least : 1;
   const int per = (turns + want - 1) / want;
   s.splits = (turns + per - 1) / per;

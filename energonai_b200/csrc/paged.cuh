@@ -49,8 +49,10 @@ __device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
 }
 
 // Host side of the checks that all entry points make of a packed batch.
-inline int paged_check(const char *what, PagedBatch &p, const int32_t *tables, long long table_ld, const int32_t *starts, const int32_t *lengths, int batch,
-                       int rows, int table_cols, int pages, int page_size) {
+inline int paged_check(const char *what, PagedBatch &p, const eb_paged &c, int rows) {
+  const int32_t *tables = c.tables, *starts = c.starts, *lengths = c.lengths;
+  const long long table_ld = c.table_ld;
+  const int batch = c.batch, table_cols = c.table_cols, pages = c.pages, page_size = c.page_size;
   EB_REQUIRE(tables && starts && lengths, "%s: null pointer", what);
   EB_REQUIRE(batch > 0 && batch <= 65535 && rows > 0 && table_cols > 0 && table_ld >= table_cols && pages > 0, "%s: bad sizes", what);
   EB_REQUIRE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "%s: pages of %d positions not supported (16, 32, 64 or 128)", what,

@@ -563,13 +563,17 @@ extern "C" size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_
   return s.step_bytes + s.prompt_bytes;
 }
 
-extern "C" int eb_paged_attention(const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int kv_heads, int head_dim,
-                                  const void *k_pages, const void *v_pages, const float *k_scale, const float *v_scale, int pages, int page_size,
-                                  const int32_t *tables, long long table_ld, int table_cols, const int32_t *starts, const int32_t *lengths, int batch,
-                                  int most_new, int most_length, int window, float scale, int dtype, void *scratch, size_t scratch_bytes, void *stream) {
+extern "C" int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,
+                                  void *scratch, size_t scratch_bytes, void *stream) {
+  EB_REQUIRE(cache, "paged_attention: null pointer");
+  const int batch = cache->batch, kv_heads = cache->kv_heads, head_dim = cache->head_dim, page_size = cache->page_size, dtype = cache->dtype,
+            table_cols = cache->table_cols;
+  int most_new = cache->most_new, most_length = cache->most_length;
+  const void *k_pages = cache->k_pages, *v_pages = cache->v_pages;
+  const float *k_scale = cache->k_scale, *v_scale = cache->v_scale;
   if (rows == 0 || batch == 0 || most_new == 0) return EB_OK;
   StepParams p{};
-  if (int rc = paged_check("paged_attention", p.batch, tables, table_ld, starts, lengths, batch, rows, table_cols, pages, page_size)) return rc;
+  if (int rc = paged_check("paged_attention", p.batch, *cache, rows)) return rc;
   EB_REQUIRE(dtype == EB_F16 || dtype == EB_BF16, "paged_attention: fp16 or bf16 only (dtype %d)", dtype);
   EB_REQUIRE(head_dim == 64 || head_dim == 128, "paged_attention: head_dim %d not supported (64 or 128)", head_dim);
   EB_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && (long long)heads * head_dim < (1 << 28), "paged_attention: %d heads do not share %d key / value heads", heads, kv_heads);

@@ -6,9 +6,12 @@ in slot p mod page_size of page tables[b, p // page_size].  Pools are [pages, kv
 activations' type or torch.float8_e4m3fn with fp32 scales [pages, kv_heads] (value = code * scale).  starts, lengths and
 tables are int32 on the device; a captured call may be replayed with other contents, within most_new new tokens per
 sequence and most_length positions."""
+import functools
+import struct
+
 import torch
 
-from ._lib import lib, check, dtype_code, ptr, stream_ptr, require_cuda
+from ._lib import lib, check, dtype_code, require_cuda
 
 PAGE_SIZES = (16, 32, 64, 128)
 HEAD_DIMS = (64, 128)
@@ -53,37 +56,65 @@ def paged_batch(new, lengths, tables, pages, page_size, device="cuda"):
     return i32([list(t) + [-1] * (cols - len(t)) for t in tables]), i32(starts), i32(list(lengths)), max(new), max(1, max(lengths))
 
 
+_device_here = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _one_device(what, *tensors):
-    require_cuda(*tensors)
-    here = torch.cuda.current_device()
-    if any(t is not None and t.device.index != here for t in tensors):
-        raise RuntimeError(f"{what}: all tensors must be on the current device (cuda:{here})")
+    """All tensors (or None) are on the current device; returns its number."""
+    on = {t.get_device() for t in tensors if t is not None}
+    if on != {_device_here()} if -1 not in on else True:
+        require_cuda(*tensors)
+        raise RuntimeError(f"{what}: all tensors must be on the current device (cuda:{_device_here()})")
+    return on.pop()
 
 
 def _rows(what, t, width, dtype):
-    if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] != width or t.dtype != dtype or (t.shape[0] > 1 and t.stride(0) < width):
-        raise RuntimeError(f"{what}: rows of {width} contiguous columns of {dtype} required, not {tuple(t.shape)} of {t.dtype}")
-    return t.stride(0) if t.shape[0] > 1 else width
+    """Row stride of [rows, width]."""
+    shape = t.shape
+    if len(shape) == 2 and shape[1] == width and t.dtype is dtype:
+        ld, one = t.stride()
+        if one == 1 or width == 1:
+            if shape[0] <= 1:
+                return width
+            if ld >= width:
+                return ld
+    raise RuntimeError(f"{what}: rows of {width} contiguous columns of {dtype} required, not {tuple(shape)} of {t.dtype}")
 
 
-def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale):
-    """Checks pools and batch; returns (kv_heads, head_dim, arguments from `pages` on to `batch`)."""
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+# struct eb_paged of the header
+_paged = struct.Struct("@7Pq10i")
+
+
+def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length):
+    """Checks pools and batch; returns (kv_heads, head_dim, positions that the tables address, struct eb_paged)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise RuntimeError(f"{what}: pools are contiguous [pages, kv_heads, page_size, head_dim], alike for keys and values")
-    pages, kv_heads, page_size, head_dim = k_pages.shape
-    held = torch.float8_e4m3fn if k_scale is not None else dtype
-    if k_pages.dtype != held or v_pages.dtype != held:
-        raise RuntimeError(f"{what}: pools of {held} required" + ("" if k_scale is not None else " (8-bit pools go with scales)"))
-    if (k_scale is None) != (v_scale is None) or any(s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (pages, kv_heads) or not s.is_contiguous())
-                                                     for s in (k_scale, v_scale)):
-        raise RuntimeError(f"{what}: scales are contiguous fp32 [pages, kv_heads], for keys and for values")
-    if any(t.dtype != torch.int32 for t in (tables, starts, lengths)) or tables.dim() != 2 or tables.stride(1) != 1 or lengths.shape != tables.shape[:1] or tuple(
-            starts.shape) != (tables.shape[0] + 1,) or not starts.is_contiguous() or not lengths.is_contiguous():
+    pages, kv_heads, page_size, head_dim = shape
+    if k_scale is None and v_scale is None:
+        held, ks, vs = dtype, 0, 0
+    else:
+        held = torch.float8_e4m3fn
+        if k_scale is None or v_scale is None or any(s.dtype is not torch.float32 or s.shape != shape[:2] or not s.is_contiguous() for s in (k_scale, v_scale)):
+            raise RuntimeError(f"{what}: scales are contiguous fp32 [pages, kv_heads], for keys and for values")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    if k_pages.dtype is not held or v_pages.dtype is not held:
+        raise RuntimeError(f"{what}: pools of {held} required" + ("" if ks else " (8-bit pools go with scales)"))
+    i32, of = torch.int32, tables.shape
+    if tables.dtype is not i32 or starts.dtype is not i32 or lengths.dtype is not i32 or len(of) != 2 or lengths.shape != of[:1] or starts.shape != (
+            of[0] + 1,) or not starts.is_contiguous() or not lengths.is_contiguous():
         raise RuntimeError(f"{what}: int32 tables [batch, pages], starts [batch + 1] and lengths [batch] required")
-    if tables.shape[0] == 0 or tables.shape[1] == 0 or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
-        raise RuntimeError(f"{what}: tables of one or more rows and columns required")
-    return kv_heads, head_dim, (pages, page_size, ptr(tables), tables.stride(0) if tables.shape[0] > 1 else tables.shape[1], tables.shape[1], ptr(starts),
-                                ptr(lengths), tables.shape[0])
+    batch, cols = of
+    ld, one = tables.stride()
+    if batch == 1:
+        ld = cols
+    if batch == 0 or cols == 0 or (one != 1 and cols > 1) or ld < cols:
+        raise RuntimeError(f"{what}: int32 tables of one or more rows of contiguous columns required")
+    reach = cols * page_size
+    most_length = reach if most_length is None else min(int(most_length), reach)
+    return kv_heads, head_dim, most_length, _paged.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), ld, pages,
+                                                        page_size, kv_heads, head_dim, cols, batch, int(most_new), most_length, dtype_code(dtype), 0)
 
 
 def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, freq=None, k_scale=None, v_scale=None, q_out=None):
@@ -92,23 +123,34 @@ def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, f
     ranges of one projection.  Returns the turned queries (in q_out, which may be q, or a new tensor; without freq: q itself
     unless q_out is given).  k_scale / v_scale belong to 8-bit pools and are updated: a page's scale grows to what its largest
     value needs, and the codes that it holds already are rounded to the new one."""
-    _one_device("paged_append", q, k, v, k_pages, v_pages, tables, starts, lengths, freq, k_scale, v_scale, q_out)
-    kv_heads, head_dim, where = _cache("paged_append", q.dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale)
-    rows = q.shape[0]
-    if q.dim() != 2 or q.shape[1] % (kv_heads * head_dim) or k.shape[0] != rows or v.shape[0] != rows:
+    device = _one_device("paged_append", q, k, v, k_pages, v_pages, tables, starts, lengths, freq, k_scale, v_scale, q_out)
+    dtype = q.dtype
+    kv_heads, head_dim, _, cache = _cache("paged_append", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, None)
+    shape, width = q.shape, kv_heads * head_dim
+    if len(shape) != 2 or shape[1] % width or k.shape[0] != shape[0] or v.shape[0] != shape[0]:
         raise RuntimeError("paged_append: one row of q, k and v per token, query heads in equal groups")
-    ldq, ldk, ldv = (_rows("paged_append", t, w, q.dtype) for t, w in ((q, q.shape[1]), (k, kv_heads * head_dim), (v, kv_heads * head_dim)))
-    if freq is not None and (freq.dtype != torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * freq.numel() > head_dim):
-        raise RuntimeError("paged_append: frequencies are fp32, one for each leading pair of a head")
-    if freq is not None and q_out is None:
-        q_out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=q.device)
-    ldo = _rows("paged_append", q_out, q.shape[1], q.dtype) if q_out is not None else 0
-    if q_out is not None and q_out.shape[0] != rows:
-        raise RuntimeError("paged_append: one row of q_out per token")
-    check(lib().eb_paged_append(ptr(q), ldq, ptr(k), ldk, ptr(v), ldv, ptr(q_out), ldo, rows, q.shape[1] // head_dim, kv_heads, head_dim, ptr(freq),
-                                freq.numel() if freq is not None else 0, ptr(k_pages), ptr(v_pages), ptr(k_scale), ptr(v_scale), *where, int(most_new),
-                                dtype_code(q.dtype), stream_ptr()), "paged_append")
+    rows, columns = shape
+    ldq, ldk, ldv = _rows("paged_append", q, columns, dtype), _rows("paged_append", k, width, dtype), _rows("paged_append", v, width, dtype)
+    pairs = 0
+    if freq is not None:
+        pairs = freq.numel()
+        if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * pairs > head_dim:
+            raise RuntimeError("paged_append: frequencies are fp32, one for each leading pair of a head")
+        if q_out is None:
+            q_out = q.new_empty((rows, columns))
+    ldo = 0
+    if q_out is not None:
+        ldo = _rows("paged_append", q_out, columns, dtype)
+        if q_out.shape[0] != rows:
+            raise RuntimeError("paged_append: one row of q_out per token")
+    check(lib().eb_paged_append(cache, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, None if q_out is None else q_out.data_ptr(), ldo, rows,
+                                columns // head_dim, None if freq is None else freq.data_ptr(), pairs, _stream_of(device)), "paged_append")
     return q if q_out is None else q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(*sizes):
+    return lib().eb_paged_attention_scratch_bytes(*sizes)
 
 
 def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most_length=None, scale=None, window=0, k_scale=None, v_scale=None, out=None):
@@ -116,23 +158,25 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     already: single tokens, a few per sequence, prompts and chunks of prompts, or all of them in one batch.  window > 0:
     the row at position p sees the positions above p - window only.  most_length: no sequence is longer (None: what the
     tables address).  Returns out [rows, heads*head_dim]; rows behind the last sequence are left as they are."""
-    _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)
-    kv_heads, head_dim, where = _cache("paged_attention", q.dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale)
-    if q.dim() != 2 or q.shape[1] % (kv_heads * head_dim):
+    device = _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)
+    dtype, shape = q.dtype, q.shape
+    kv_heads, head_dim, most_length, cache = _cache("paged_attention", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length)
+    if len(shape) != 2 or shape[1] % (kv_heads * head_dim):
         raise RuntimeError("paged_attention: q is [rows, heads*head_dim], query heads in equal groups")
-    rows, heads, batch = q.shape[0], q.shape[1] // head_dim, tables.shape[0]
-    ldq = _rows("paged_attention", q, q.shape[1], q.dtype)
+    rows, columns = shape
+    heads = columns // head_dim
+    ldq = _rows("paged_attention", q, columns, dtype)
     if out is None:
-        out = torch.empty((rows, q.shape[1]), dtype=q.dtype, device=q.device)
-    ldo = _rows("paged_attention", out, q.shape[1], q.dtype)
-    if out.shape[0] != rows:
-        raise RuntimeError("paged_attention: one row of out per row of q")
-    reach = tables.shape[1] * k_pages.shape[2]
-    most_length = reach if most_length is None else min(int(most_length), reach)
-    most_new, window = min(int(most_new), rows), 0 if int(window) >= reach else int(window)
-    nbytes = lib().eb_paged_attention_scratch_bytes(batch, heads, kv_heads, head_dim, most_new, most_length, window)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None       # (of this call: captured calls share none)
-    check(lib().eb_paged_attention(ptr(q), ldq, ptr(out), ldo, rows, heads, kv_heads, head_dim, ptr(k_pages), ptr(v_pages), ptr(k_scale), ptr(v_scale), *where,
-                                   most_new, most_length, window, float(head_dim ** -0.5 if scale is None else scale), dtype_code(q.dtype),
-                                   ptr(scratch), nbytes, stream_ptr()), "paged_attention", launches=2 if nbytes else 1)
+        out, ldo = q.new_empty((rows, columns)), columns
+    else:
+        ldo = _rows("paged_attention", out, columns, dtype)
+        if out.shape[0] != rows:
+            raise RuntimeError("paged_attention: one row of out per row of q")
+    window = int(window)
+    if window >= most_length:
+        window = 0                                          # (every key is inside)
+    nbytes = _scratch_bytes(tables.shape[0], heads, kv_heads, head_dim, min(int(most_new), rows), most_length, window)
+    scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None       # (of this call: captured calls share none)
+    check(lib().eb_paged_attention(cache, q.data_ptr(), ldq, out.data_ptr(), ldo, rows, heads, window, float(head_dim ** -0.5 if scale is None else scale),
+                                   None if scratch is None else scratch.data_ptr(), nbytes, _stream_of(device)), "paged_attention", launches=2 if nbytes else 1)
     return out

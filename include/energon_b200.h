@@ -892,11 +892,18 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
 /* Many sequences at once, each with a length of its own, keys and values in pages of page_size (16, 32, 64 or 128)
  * positions: pools [pages][kv_heads][page_size][head_dim], in `dtype` (fp16 or bf16) or, with scales [pages][kv_heads],
  * as e4m3 codes (value = code * scale).  Rows starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the
- * new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, so that row i of n_b has
- * position lengths[b] - n_b + i.  Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
+ * new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, at most most_length, so that row i
+ * of n_b has position lengths[b] - n_b + i.  Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
  * starts, lengths and tables live on the device and may change between replays of a captured call.  Pages that are none
  * (outside of the pool or behind the table's columns) hold nothing: nothing is written to them and nothing read.
  * head_dim is 64 or 128; heads / kv_heads query heads share a key / value head.  No counterpart in the reference. */
+typedef struct eb_paged {
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;       /* both or neither */
+  const int32_t *tables, *starts, *lengths;
+  int64_t table_ld;
+  int32_t pages, page_size, kv_heads, head_dim, table_cols, batch, most_new, most_length, dtype, reserved;
+} eb_paged;
 
 /* New tokens into the cache: for i < pairs (z_2i, z_2i+1) of every query and key head turned by the angle
  * position * freq[i] (taken in 64 bits), queries to q_out (NULL: left alone; may be q), keys and values to their pages.  With
@@ -904,21 +911,16 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
  * 448, or the one that it had if that is larger and the page holds earlier positions of the sequence, whose codes are then
  * rounded to the new scale; infinities and NaN become NaN.  Slots in front of and behind the new rows, other pages and rows
  * of q_out behind the last sequence are left as they were.  A page that this call writes belongs to one sequence. */
-EB_API int eb_paged_append(const void *q, long long ldq, const void *k, long long ldk, const void *v, long long ldv, void *q_out, long long ldo,
-                    int rows, int heads, int kv_heads, int head_dim, const float *freq, int pairs, void *k_pages, void *v_pages,
-                    float *k_scale, float *v_scale, int pages, int page_size, const int32_t *tables, long long table_ld, int table_cols,
-                    const int32_t *starts, const int32_t *lengths, int batch, int most_new, int dtype, void *stream);
+EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, const void *k, long long ldk, const void *v, long long ldv, void *q_out,
+                    long long ldo, int rows, int heads, const float *freq, int pairs, void *stream);
 
 /* Causal attention of the new tokens over the cache (which holds them already): the row at position p sees the positions
  * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros; rows of `out` behind the last
- * sequence are left as they were.  No lengths[b] is above most_length.  Slots that no row sees may hold anything.
+ * sequence are left as they were.  Slots that no row sees may hold anything.
  * scratch: eb_paged_attention_scratch_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the
  * device need scratch of their own. */
-EB_API int eb_paged_attention(const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int kv_heads, int head_dim,
-                       const void *k_pages, const void *v_pages, const float *k_scale, const float *v_scale, int pages, int page_size,
-                       const int32_t *tables, long long table_ld, int table_cols, const int32_t *starts, const int32_t *lengths, int batch,
-                       int most_new, int most_length, int window, float scale, int dtype, void *scratch, size_t scratch_bytes,
-                       void *stream);
+EB_API int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,
+                       void *scratch, size_t scratch_bytes, void *stream);
 EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window);
 
 /* Low-rank adapters of many requests: for the rows starts[b] to starts[b + 1] - 1 (at most most_new) of each sequence, with

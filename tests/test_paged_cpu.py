@@ -45,12 +45,24 @@ def test_cpu_tensors_are_rejected():
 FAKE = 1 << 20                 # an aligned address that nothing is read from: every call below is refused before a launch
 
 
+class Paged(ctypes.Structure):
+    """struct eb_paged of the header."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k_pages", "v_pages", "k_scale", "v_scale", "tables", "starts", "lengths")] + [("table_ld", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("pages", "page_size", "kv_heads", "head_dim", "table_cols", "batch", "most_new", "most_length", "dtype", "reserved")]
+
+
+def cache_of(a):
+    names = [n for n, _ in Paged._fields_]
+    return Paged(**{n: a.pop(n) for n in names if n in a}), a
+
+
 def append_call(**change):
     a = dict(q=FAKE, ldq=512, k=FAKE, ldk=256, v=FAKE, ldv=256, q_out=FAKE, ldo=512, rows=4, heads=8, kv_heads=4, head_dim=64, freq=FAKE, pairs=32, k_pages=FAKE,
              v_pages=FAKE, k_scale=FAKE, v_scale=FAKE, pages=9, page_size=16, tables=FAKE, table_ld=3, table_cols=3, starts=FAKE, lengths=FAKE, batch=2, most_new=4,
-             dtype=_lib.F16, stream=None)
+             most_length=48, dtype=_lib.F16, stream=None)
     a.update(change)
-    return _lib.lib().eb_paged_append(*a.values())
+    cache, a = cache_of(a)
+    return _lib.lib().eb_paged_append(ctypes.addressof(cache), *a.values())
 
 
 @pytest.mark.parametrize("change,words", [(dict(k=None), "null"), (dict(tables=None), "null"), (dict(dtype=_lib.F32), "fp16 or bf16"), (dict(head_dim=80), "head_dim 80"),
@@ -63,11 +75,12 @@ def test_append_refuses(change, words):
 
 
 def attention_call(**change):
-    a = dict(q=FAKE, ldq=512, out=FAKE, ldo=512, rows=4, heads=8, kv_heads=4, head_dim=64, k_pages=FAKE, v_pages=FAKE, k_scale=None, v_scale=None, pages=9, page_size=16,
-             tables=FAKE, table_ld=300, table_cols=300, starts=FAKE, lengths=FAKE, batch=2, most_new=4, most_length=4800, window=0, scale=0.125, dtype=_lib.F16,
+    a = dict(q=FAKE, ldq=512, out=FAKE, ldo=512, rows=4, heads=8, window=0, scale=0.125, kv_heads=4, head_dim=64, k_pages=FAKE, v_pages=FAKE, k_scale=None, v_scale=None, pages=9, page_size=16,
+             tables=FAKE, table_ld=300, table_cols=300, starts=FAKE, lengths=FAKE, batch=2, most_new=4, most_length=4800, dtype=_lib.F16,
              scratch=FAKE, scratch_bytes=1 << 30, stream=None)
     a.update(change)
-    return _lib.lib().eb_paged_attention(*a.values())
+    cache, a = cache_of(a)
+    return _lib.lib().eb_paged_attention(ctypes.addressof(cache), *a.values())
 
 
 @pytest.mark.parametrize("change,words", [(dict(q=None), "null"), (dict(out=None), "null"), (dict(dtype=_lib.F32), "fp16 or bf16"), (dict(head_dim=96), "head_dim 96"),
@@ -90,3 +103,23 @@ def test_scratch_grows_with_the_splits():
     assert need(1, 8, 8, 128, 1, 100000, 0) > 0
     assert need(1, 8, 8, 128, 1, 100000, 128) == 0                        # a window is short
     assert ctypes.sizeof(ctypes.c_size_t) == 8
+
+
+def test_the_cache_struct_matches_the_header(tmp_path):
+    """The bytes that the Python entry packs, and the structure above, have the size and field offsets that a C compiler gives the declaration."""
+    import shutil
+    import subprocess
+    from energonai_b200 import paged
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no C compiler")
+    names = [n for n, _ in Paged._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(['#include <stdio.h>', '#include <stddef.h>', f'#include "{_lib.HEADER}"', 'int main(void) {', '  printf("%zu\\n", sizeof(eb_paged));']
+                             + [f'  printf("%zu\\n", offsetof(eb_paged, {n}));' for n in names] + ['  return 0;', '}']))
+    subprocess.run([gcc, "-std=c99", "-Wall", "-Werror", str(src), "-o", str(exe)], check=True)
+    size, *offsets = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert ctypes.sizeof(Paged) == size == paged._paged.size
+    assert [getattr(Paged, n).offset for n in names] == offsets
+    packed = Paged.from_buffer_copy(paged._paged.pack(*range(1, len(names) + 1)))
+    assert [getattr(packed, n) for n in names] == list(range(1, len(names) + 1))
