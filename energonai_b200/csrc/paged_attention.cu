@@ -59,11 +59,11 @@ __device__ __forceinline__ float pow2(float x) {
 }
 template <typename T> __device__ __forceinline__ void mma_tile(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -102,6 +102,84 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
   const StepTile t = step_tile(p, r, rt, kRowsT);
   const int lo = (t.lo & ~15) + split * p.chunk, hi = split == p.splits - 1 ? t.hi : min(t.hi, lo + p.chunk);
   if (split > 0 && lo >= hi) return;
+
+  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
+    l_run[n][0] = l_run[n][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
+  }
+
+  constexpr long long kRowBytes = EIGHT ? D : 2 * D;
+  const long long block_bytes = kRowBytes << p.batch.page_shift;
+  const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.k_pages), *vp = reinterpret_cast<const uint8_t *>(p.v_pages);
+  const int blocks = hi > lo ? (hi - lo + 15) / 16 : 0, mine = blocks > warp ? (blocks - warp + kStepWarps - 1) / kStepWarps : 0;
+  // lane l holds the page of this warp's tile 32 n + l (and its scales), and of the next 32
+  struct Ids {
+    int id;
+    float ks, vs;
+  };
+  auto fetch_ids = [&](int i0) {
+    Ids x{-1, 1.f, 1.f};
+    if (i0 + lane < mine) x.id = paged_page(p.batch, b, (lo + (warp + (i0 + lane) * kStepWarps) * 16) >> p.batch.page_shift);
+    if (EIGHT && x.id >= 0) {
+      x.ks = p.k_scale[(long long)x.id * p.kv_heads + hk];
+      x.vs = p.v_scale[(long long)x.id * p.kv_heads + hk];
+    }
+    return x;
+  };
+  uint32_t kr[2][kKeyRegs], vr[4][kValRegs];
+  // address of the 16 rows of tile i (null: no such page)
+  auto tile_at = [&](const uint8_t *pool, int i, int id) {
+    const int key = lo + (warp + i * kStepWarps) * 16;
+    return pool + ((long long)id * p.kv_heads + hk) * block_bytes + (key & ((1 << p.batch.page_shift) - 1)) * kRowBytes;
+  };
+  auto load_keys = [&](int i, int id) {
+    const uint8_t *x = tile_at(kp, i, id) + g * kRowBytes + c * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < kKeyRegs / 4; ++j) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(x + h * 8 * kRowBytes + j * 64));
+        kr[h][4 * j] = w.x;
+        kr[h][4 * j + 1] = w.y;
+        kr[h][4 * j + 2] = w.z;
+        kr[h][4 * j + 3] = w.w;
+      }
+  };
+  // value rows 2c, 2c + 1, 2c + 8, 2c + 9; dimensions by g
+  auto load_values = [&](int i, int id) {
+    const uint8_t *x = tile_at(vp, i, id) + 2 * c * kRowBytes;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint8_t *y = x + ((h & 1) + (h >> 1) * 8) * kRowBytes;
+      if constexpr (kValRegs == 2) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(y + g * 8));
+        vr[h][0] = w.x;
+        vr[h][1] = w.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < kValRegs / 4; ++j) {
+          const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(y + j * 128 + g * 16));
+          vr[h][4 * j] = w.x;
+          vr[h][4 * j + 1] = w.y;
+          vr[h][4 * j + 2] = w.z;
+          vr[h][4 * j + 3] = w.w;
+        }
+      }
+    }
+  };
+  Ids ids = fetch_ids(0), ids_next = fetch_ids(32);
+  int id = __shfl_sync(0xffffffffu, ids.id, 0);
+  float k_now = __shfl_sync(0xffffffffu, ids.ks, 0), v_now = __shfl_sync(0xffffffffu, ids.vs, 0);
+  if (mine > 0 && id >= 0) {
+    load_keys(0, id);
+    load_values(0, id);
+  }
 
   // ---- queries: fragments of the second operand, k index permuted like the keys ----
   uint32_t qf[NT][kTiles][2];
@@ -160,89 +238,18 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
     for (int e = 0; e < 2; ++e) row_pos[n][e] = t.past + (rt * kRowsT + n * 8 + 2 * c + e) / p.group;
   const int first_pos = t.past + rt * kRowsT / p.group, last_pos = t.past + (rt * kRowsT + t.rows - 1) / p.group;
 
-  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
-    l_run[n][0] = l_run[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
-  }
-
-  constexpr long long kRowBytes = EIGHT ? D : 2 * D;
-  const long long block_bytes = kRowBytes << p.batch.page_shift;
-  const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.k_pages), *vp = reinterpret_cast<const uint8_t *>(p.v_pages);
-  const int blocks = hi > lo ? (hi - lo + 15) / 16 : 0, mine = blocks > warp ? (blocks - warp + kStepWarps - 1) / kStepWarps : 0;
-  // lane l holds the page of this warp's tile 32 n + l (and its scales)
-  int ids = -1;
-  float ks = 1.f, vs = 1.f;
-  auto fetch_ids = [&](int i0) {
-    ids = -1;
-    if (i0 + lane < mine) ids = paged_page(p.batch, b, (lo + (warp + (i0 + lane) * kStepWarps) * 16) >> p.batch.page_shift);
-    if (EIGHT && ids >= 0) {
-      ks = p.k_scale[(long long)ids * p.kv_heads + hk];
-      vs = p.v_scale[(long long)ids * p.kv_heads + hk];
-    }
-  };
-  uint32_t kr[2][kKeyRegs], vr[4][kValRegs];
-  // address of the 16 rows of tile i (null: no such page)
-  auto tile_at = [&](const uint8_t *pool, int i, int id) {
-    const int key = lo + (warp + i * kStepWarps) * 16;
-    return pool + ((long long)id * p.kv_heads + hk) * block_bytes + (key & ((1 << p.batch.page_shift) - 1)) * kRowBytes;
-  };
-  auto load_keys = [&](int i, int id) {
-    const uint8_t *x = tile_at(kp, i, id) + g * kRowBytes + c * 16;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < kKeyRegs / 4; ++j) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(x + h * 8 * kRowBytes + j * 64));
-        kr[h][4 * j] = w.x;
-        kr[h][4 * j + 1] = w.y;
-        kr[h][4 * j + 2] = w.z;
-        kr[h][4 * j + 3] = w.w;
-      }
-  };
-  // value rows 2c, 2c + 1, 2c + 8, 2c + 9; dimensions by g
-  auto load_values = [&](int i, int id) {
-    const uint8_t *x = tile_at(vp, i, id) + 2 * c * kRowBytes;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint8_t *y = x + ((h & 1) + (h >> 1) * 8) * kRowBytes;
-      if constexpr (kValRegs == 2) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(y + g * 8));
-        vr[h][0] = w.x;
-        vr[h][1] = w.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kValRegs / 4; ++j) {
-          const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(y + j * 128 + g * 16));
-          vr[h][4 * j] = w.x;
-          vr[h][4 * j + 1] = w.y;
-          vr[h][4 * j + 2] = w.z;
-          vr[h][4 * j + 3] = w.w;
-        }
-      }
-    }
-  };
-  fetch_ids(0);
-  int id = __shfl_sync(0xffffffffu, ids, 0);
-  float k_now = __shfl_sync(0xffffffffu, ks, 0), v_now = __shfl_sync(0xffffffffu, vs, 0);
-  if (mine > 0 && id >= 0) {
-    load_keys(0, id);
-    load_values(0, id);
-  }
   for (int i = 0; i < mine; ++i) {
     const int key0 = lo + (warp + i * kStepWarps) * 16, id_now = id;
     const float ks_now = k_now, vs_now = v_now;
     if (i + 1 < mine) {
-      if (((i + 1) & 31) == 0) fetch_ids(i + 1);
-      id = __shfl_sync(0xffffffffu, ids, (i + 1) & 31);
+      if (((i + 1) & 31) == 0) {
+        ids = ids_next;
+        ids_next = fetch_ids(i + 33);
+      }
+      id = __shfl_sync(0xffffffffu, ids.id, (i + 1) & 31);
       if (EIGHT) {
-        k_now = __shfl_sync(0xffffffffu, ks, (i + 1) & 31);
-        v_now = __shfl_sync(0xffffffffu, vs, (i + 1) & 31);
+        k_now = __shfl_sync(0xffffffffu, ids.ks, (i + 1) & 31);
+        v_now = __shfl_sync(0xffffffffu, ids.vs, (i + 1) & 31);
       }
     }
     const bool more = i + 1 < mine && id >= 0;
@@ -254,9 +261,11 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
       continue;
     }
     // ---- scores ----
-    float s[NT][4];
+    float s[NT][4], s2[NT][4];                                           // (two chains of dependent products)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
     for (int k = 0; k < kTiles; ++k) {
       uint32_t a0, a1, a2, a3;
@@ -272,7 +281,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
         a3 = kr[1][2 * k + 1];
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_tile<M>(s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+      for (int n = 0; n < NT; ++n) mma_tile<M>((k & 1) ? s2[n] : s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
     }
     if (more) load_keys(i + 1, id);
     const float v_log = EIGHT ? __log2f(vs_now) : 0.f, v_inv = EIGHT ? 1.f / vs_now : 1.f;
@@ -282,7 +291,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float v = EIGHT ? fmaf(s[n][e], factor[n][e & 1] * ks_now, v_log) : s[n][e] * factor[n][e & 1];
+        const float x = s[n][e] + s2[n][e];
+        float v = EIGHT ? fmaf(x, factor[n][e & 1] * ks_now, v_log) : x * factor[n][e & 1];
         if (!whole) {
           const int key = key0 + g + (e >> 1) * 8, pos = row_pos[n][e & 1];
           if (key >= hi || key > pos || (p.window > 0 && key <= pos - p.window)) v = -INFINITY;
@@ -389,27 +399,38 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
       }
     }
   __syncthreads();
-  for (int i = threadIdx.x; i < t.rows * (D / 2); i += kStepWarps * 32) {
-    const int row = i / (D / 2), d = 2 * (i % (D / 2));
-    float m = red[0][row][D], l = 0.f, x = 0.f, y = 0.f;
+  // two columns of a row, of this CTA's warps
+  struct Sum {
+    float m, l, x, y;
+  };
+  auto of_warps = [&](int row, int d) {
+    Sum r{red[0][row][D], 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 1; w < kStepWarps; ++w) m = fmaxf(m, red[w][row][D]);
+    for (int w = 1; w < kStepWarps; ++w) r.m = fmaxf(r.m, red[w][row][D]);
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w) {
-      const float a = pow2(red[w][row][D] - m);
-      l = fmaf(red[w][row][D + 1], a, l);
-      x = fmaf(red[w][row][d], a, x);
-      y = fmaf(red[w][row][d + 1], a, y);
+      const float a = pow2(red[w][row][D] - r.m);
+      r.l = fmaf(red[w][row][D + 1], a, r.l);
+      r.x = fmaf(red[w][row][d], a, r.x);
+      r.y = fmaf(red[w][row][d + 1], a, r.y);
     }
+    return r;
+  };
+  auto write = [&](int row, int d, const Sum &v) {
+    const int all = rt * kRowsT + row;
+    T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D + d;
+    const float inv = v.l == 0.f ? 0.f : 1.f / v.l;
+    *reinterpret_cast<uint32_t *>(out) = pack2<T>(v.x * inv, v.y * inv);
+  };
+  for (int i = threadIdx.x; i < t.rows * (D / 2); i += kStepWarps * 32) {
+    const int row = i / (D / 2), d = 2 * (i % (D / 2));
+    const Sum v = of_warps(row, d);
     if (p.part) {
       float *out = p.part + ((((long long)b * p.kv_heads + hk) * p.row_tiles + rt) * p.splits + split) * kRowsT * (D + 2) + row * (D + 2);
-      *reinterpret_cast<float2 *>(out + d) = make_float2(x, y);
-      if (d == 0) *reinterpret_cast<float2 *>(out + D) = make_float2(m, l);
+      *reinterpret_cast<float2 *>(out + d) = make_float2(v.x, v.y);
+      if (d == 0) *reinterpret_cast<float2 *>(out + D) = make_float2(v.m, v.l);
     } else {
-      const int all = rt * kRowsT + row;
-      T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D + d;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      *reinterpret_cast<uint32_t *>(out) = pack2<T>(x * inv, y * inv);
+      write(row, d, v);
     }
   }
 }
@@ -495,6 +516,7 @@ template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParam
   return check_launch("paged_attention");
 }
 
+constexpr int kMostKeys = 8192, kLeastKeys = 256;
 // How the step form cuts a call: query rows per tile, tiles, keys per CTA, splits.
 struct StepPlan {
   int tiles8, row_tiles, chunk, splits;
@@ -503,11 +525,17 @@ StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys) {
   StepPlan s;
   s.tiles8 = rows_per_head > 8 ? 2 : 1;
   s.row_tiles = (rows_per_head + 8 * s.tiles8 - 1) / (8 * s.tiles8);
-  const long long units = (long long)batch * kv_heads * s.row_tiles, want = (4ll * sm_count() + units - 1) / units;
+  const long long units = (long long)batch * kv_heads * s.row_tiles, sms = sm_count();
+  // Two CTAs per multiprocessor and more stream fast enough without splits; fewer are split to four per multiprocessor.  No CTA
+  // gets more than kMostKeys keys (a long sequence among short ones would keep the call waiting) nor fewer than kLeastKeys.  (64 sequences
+  // of 2048 to 4095 keys, 8 key / value heads: 87 us without splits, 96 with two, 86 with four.  A cluster per row that merges in shared
+  // memory was slower than a second launch at every size, 146 us there: clusters wait for room side by side.)
+  const long long want = units >= 2 * sms ? 1 : (4 * sms + units - 1) / units;
   keys += 15;                                               // (the first tile may begin in front of the first key)
-  long long chunk = (keys + want - 1) / want, least = (keys + 511) / 512;
-  if (chunk < 256) chunk = 256;
-  if (chunk < least) chunk = least;
+  long long chunk = (keys + want - 1) / want;
+  if (chunk > kMostKeys) chunk = kMostKeys;
+  if (chunk < kLeastKeys) chunk = kLeastKeys;
+  if (chunk < (keys + 511) / 512) chunk = (keys + 511) / 512;
   chunk = (chunk + 63) / 64 * 64;
   s.splits = (int)((keys + chunk - 1) / chunk);
   s.chunk = (int)chunk;
