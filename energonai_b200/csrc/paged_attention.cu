@@ -3,13 +3,13 @@
 // once per key / value head and serves all query heads that share it.
 //
 // Both products are mma.sync tiles with the cached rows on the long side: S^T = K Q^T (16 keys x 8 query rows) and
-// O^T += V^T P^T (16 dimensions x 8 query rows), so that 8 query rows (token, head of the group) fill a tile.  A
-// warp takes 16 keys at a time, straight from global memory into the fragments of its lanes: the contraction of S
-// runs over dimensions in any order and that of O over keys in any order, so each lane loads 16 bytes where they lie
-// and the queries are laid out to match; 8 lanes cover a row, every sector is used, and neither
-// shared memory nor a barrier stands between memory and the tensor core.  P^T comes from S^T by an 8 x 8 transpose
-// within the warp.  The next keys are requested as soon as the scores are done, the next values behind the second
-// product; 12 to 16 warps per multiprocessor keep 50 KB and more in flight.
+// O^T += V^T P^T (16 dimensions x 8 query rows), so that 8 query rows (token, head of the group) fill a tile.  A warp takes
+// 16 keys at a time, which lie in one page, through a small ring of tiles of its own in shared memory (asynchronous copies of 16 bytes, no
+// barrier between warps, 16 warps per multiprocessor).  The contraction of S runs over dimensions in any order and that of O
+// over keys in any order, so each lane reads 16 bytes where they lie, as the fragments of the products need them, and the queries
+// are laid out to match; the chunks are swizzled so that these reads meet in no bank.  P^T comes from S^T by an 8 x 8
+// transpose within the warp.  Tried and slower, for 64 sequences of 2048 to 4095 keys in e4m3, 8 heads of 128 (76 us): keys and values straight to
+// registers, one tile ahead (88 us); bulk copies into unswizzled rings, twice as deep with 12 warps (93 us).
 //
 // e4m3 codes become fp16 (exact), whatever the model's type: queries of bf16 models go to fp16 with a power of two per
 // row, which keeps all their bits.  A page's key scale multiplies its scores; the value scale z is added to the exponent,
@@ -24,6 +24,7 @@
 // CTA take every fourth tile; partial rows are merged in order, across CTAs by a second launch.
 #include <type_traits>
 
+#include "attention_mma.cuh"
 #include "paged_prompt.cuh"
 
 namespace eb {
@@ -84,15 +85,19 @@ __device__ __forceinline__ StepTile step_tile(const StepParams &p, const PagedRo
 }
 
 // T: type of queries and output; EIGHT: e4m3 pages; NT: tiles of 8 query rows
-template <typename T, bool EIGHT, int D, int NT>
-__global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) : NT == 1 ? (EIGHT ? 4 : 3) : 2) paged_step_kernel(const StepParams p) {
+template <bool EIGHT, int D, int NT> struct StepShape {
+  static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : 3) : NT == 1 ? (EIGHT ? 4 : 3) : 2;      // resident per multiprocessor
+};
+template <typename T, bool EIGHT, int D, int NT, int STAGES>
+__global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCtas) paged_step_kernel(const StepParams p) {
   using M = typename std::conditional<EIGHT, __half, T>::type;           // operand type of the products
   constexpr bool kSplitP = std::is_same<M, __nv_bfloat16>::value;
   constexpr float kLift = kSplitP ? 0.f : kLiftHalf;
   constexpr int kRowsT = 8 * NT, kTiles = D / 16;
   constexpr int kKeyRegs = EIGHT ? D / 16 : D / 8;                       // registers per lane and key row
   constexpr int kValRegs = EIGHT ? D / 32 : D / 16;                      // ... and value row
-  __shared__ float red[kStepWarps][kRowsT][D + 2];
+  extern __shared__ __align__(128) uint8_t smem[];
+  float (*red)[kRowsT][D + 2] = reinterpret_cast<float (*)[kRowsT][D + 2]>(smem);      // behind the key loop: [warps][rows][D + 2]
   griddep_wait();
   griddep_launch();
   const int split = blockIdx.x, hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z;
@@ -103,19 +108,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
   const int lo = (t.lo & ~15) + split * p.chunk, hi = split == p.splits - 1 ? t.hi : min(t.hi, lo + p.chunk);
   if (split > 0 && lo >= hi) return;
 
-  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
-    l_run[n][0] = l_run[n][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
-  }
-
-  constexpr long long kRowBytes = EIGHT ? D : 2 * D;
-  const long long block_bytes = kRowBytes << p.batch.page_shift;
+  constexpr int kRowBytes = EIGHT ? D : 2 * D, kChunks = kRowBytes / 16, kHalf = 16 * kRowBytes, kTile = 2 * kHalf;
+  const long long block_bytes = (long long)kRowBytes << p.batch.page_shift;
   const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.k_pages), *vp = reinterpret_cast<const uint8_t *>(p.v_pages);
   const int blocks = hi > lo ? (hi - lo + 15) / 16 : 0, mine = blocks > warp ? (blocks - warp + kStepWarps - 1) / kStepWarps : 0;
   // lane l holds the page of this warp's tile 32 n + l (and its scales), and of the next 32
@@ -132,54 +126,34 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
     }
     return x;
   };
-  uint32_t kr[2][kKeyRegs], vr[4][kValRegs];
-  // address of the 16 rows of tile i (null: no such page)
-  auto tile_at = [&](const uint8_t *pool, int i, int id) {
-    const int key = lo + (warp + i * kStepWarps) * 16;
-    return pool + ((long long)id * p.kv_heads + hk) * block_bytes + (key & ((1 << p.batch.page_shift) - 1)) * kRowBytes;
-  };
-  auto load_keys = [&](int i, int id) {
-    const uint8_t *x = tile_at(kp, i, id) + g * kRowBytes + c * 16;
+  Ids ids = fetch_ids(0), ids_next = fetch_ids(32);
+  // The warp's ring of tiles.  Chunks of 16 bytes are swizzled so that neither the keys' reads (rows g, chunks c + 4 j) nor the values'
+  // (rows 2 c + h, chunks g) meet in a bank.
+  uint8_t *ring = smem + warp * STAGES * kTile;
+  const uint32_t ring_at = smem_u32(ring);
+  auto swizzle = [](int row) { return kChunks >= 8 ? ((row >> 1) & 3) << 1 ^ (row & 1) << 2 : (row >> 1) & 3; };
+  // tile i of this warp, whose page is held by lane i mod 32 of `from` (a page that is none: nothing is requested)
+  auto request = [&](int i, int id) {
+    if (i < mine && id >= 0) {
+      const int key = lo + (warp + i * kStepWarps) * 16;
+      const long long at = ((long long)id * p.kv_heads + hk) * block_bytes + (key & ((1 << p.batch.page_shift) - 1)) * kRowBytes + lane * 16;
+      const uint32_t to = ring_at + (i % STAGES) * kTile;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < kKeyRegs / 4; ++j) {
-        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(x + h * 8 * kRowBytes + j * 64));
-        kr[h][4 * j] = w.x;
-        kr[h][4 * j + 1] = w.y;
-        kr[h][4 * j + 2] = w.z;
-        kr[h][4 * j + 3] = w.w;
-      }
-  };
-  // value rows 2c, 2c + 1, 2c + 8, 2c + 9; dimensions by g
-  auto load_values = [&](int i, int id) {
-    const uint8_t *x = tile_at(vp, i, id) + 2 * c * kRowBytes;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint8_t *y = x + ((h & 1) + (h >> 1) * 8) * kRowBytes;
-      if constexpr (kValRegs == 2) {
-        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(y + g * 8));
-        vr[h][0] = w.x;
-        vr[h][1] = w.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < kValRegs / 4; ++j) {
-          const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(y + j * 128 + g * 16));
-          vr[h][4 * j] = w.x;
-          vr[h][4 * j + 1] = w.y;
-          vr[h][4 * j + 2] = w.z;
-          vr[h][4 * j + 3] = w.w;
-        }
+      for (int n = 0; n < kHalf / 512; ++n) {
+        const int row = (n * 32 + lane) / kChunks, chunk = (n * 32 + lane) % kChunks;
+        const uint32_t off = row * kRowBytes + (chunk ^ swizzle(row)) * 16;
+        cp_async16(to + off, kp + at + n * 512, true);
+        cp_async16(to + kHalf + off, vp + at + n * 512, true);
       }
     }
+    cp_async_commit();
   };
-  Ids ids = fetch_ids(0), ids_next = fetch_ids(32);
-  int id = __shfl_sync(0xffffffffu, ids.id, 0);
-  float k_now = __shfl_sync(0xffffffffu, ids.ks, 0), v_now = __shfl_sync(0xffffffffu, ids.vs, 0);
-  if (mine > 0 && id >= 0) {
-    load_keys(0, id);
-    load_values(0, id);
-  }
+  auto id_of = [&](int i, int base) {                      // page of tile i, with the windows that begin at tile `base`
+    const int x = __shfl_sync(0xffffffffu, ids.id, i & 31), y = __shfl_sync(0xffffffffu, ids_next.id, i & 31);
+    return i - base < 32 ? x : y;
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) request(i, id_of(i, 0));
 
   // ---- queries: fragments of the second operand, k index permuted like the keys ----
   uint32_t qf[NT][kTiles][2];
@@ -238,53 +212,55 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
     for (int e = 0; e < 2; ++e) row_pos[n][e] = t.past + (rt * kRowsT + n * 8 + 2 * c + e) / p.group;
   const int first_pos = t.past + rt * kRowsT / p.group, last_pos = t.past + (rt * kRowsT + t.rows - 1) / p.group;
 
+  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
+    l_run[n][0] = l_run[n][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
+  }
+
   for (int i = 0; i < mine; ++i) {
-    const int key0 = lo + (warp + i * kStepWarps) * 16, id_now = id;
-    const float ks_now = k_now, vs_now = v_now;
-    if (i + 1 < mine) {
-      if (((i + 1) & 31) == 0) {
-        ids = ids_next;
-        ids_next = fetch_ids(i + 33);
-      }
-      id = __shfl_sync(0xffffffffu, ids.id, (i + 1) & 31);
-      if (EIGHT) {
-        k_now = __shfl_sync(0xffffffffu, ids.ks, (i + 1) & 31);
-        v_now = __shfl_sync(0xffffffffu, ids.vs, (i + 1) & 31);
-      }
+    const int key0 = lo + (warp + i * kStepWarps) * 16;
+    if (i > 0 && (i & 31) == 0) {
+      ids = ids_next;
+      ids_next = fetch_ids(i + 32);
     }
-    const bool more = i + 1 < mine && id >= 0;
-    if (id_now < 0) {                                                    // (a page that is none: nothing to see)
-      if (more) {
-        load_keys(i + 1, id);
-        load_values(i + 1, id);
-      }
-      continue;
-    }
+    const int id = __shfl_sync(0xffffffffu, ids.id, i & 31);
+    const float ks = EIGHT ? __shfl_sync(0xffffffffu, ids.ks, i & 31) : 1.f, vs = EIGHT ? __shfl_sync(0xffffffffu, ids.vs, i & 31) : 1.f;
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();                                          // (tile i is there, and all lanes have read tile i - 1, whose memory the next request takes)
+    request(i + STAGES - 1, id_of(i + STAGES - 1, i & ~31));
+    if (id < 0) continue;                                  // (a page that is none: nothing to see)
+    const uint8_t *tile = ring + (i % STAGES) * kTile;
     // ---- scores ----
-    float s[NT][4], s2[NT][4];                                           // (two chains of dependent products)
+    float s[NT][4], s2[NT][4];                             // (two chains of dependent products)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = s2[n][e] = 0.f;
 #pragma unroll
-    for (int k = 0; k < kTiles; ++k) {
-      uint32_t a0, a1, a2, a3;
+    for (int j = 0; j < kKeyRegs / 4; ++j) {
+      const uint4 x = *reinterpret_cast<const uint4 *>(tile + g * kRowBytes + ((c + 4 * j) ^ swizzle(g)) * 16), y = *reinterpret_cast<const uint4 *>(tile + (g + 8) * kRowBytes + ((c + 4 * j) ^ swizzle(g)) * 16);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
       if constexpr (EIGHT) {
-        a0 = e4m3x2_to_half2(kr[0][k]);
-        a1 = e4m3x2_to_half2(kr[1][k]);
-        a2 = e4m3x2_to_half2(kr[0][k] >> 16);
-        a3 = e4m3x2_to_half2(kr[1][k] >> 16);
-      } else {
-        a0 = kr[0][2 * k];
-        a1 = kr[1][2 * k];
-        a2 = kr[0][2 * k + 1];
-        a3 = kr[1][2 * k + 1];
-      }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_tile<M>((k & 1) ? s2[n] : s[n], a0, a1, a2, a3, qf[n][k][0], qf[n][k][1]);
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t a0 = e4m3x2_to_half2(xs[w]), a1 = e4m3x2_to_half2(ys[w]), a2 = e4m3x2_to_half2(xs[w] >> 16), a3 = e4m3x2_to_half2(ys[w] >> 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_tile<M>((w & 1) ? s2[n] : s[n], a0, a1, a2, a3, qf[n][4 * j + w][0], qf[n][4 * j + w][1]);
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_tile<M>((w & 1) ? s2[n] : s[n], xs[2 * w], ys[2 * w], xs[2 * w + 1], ys[2 * w + 1], qf[n][2 * j + w][0], qf[n][2 * j + w][1]);
+      }
     }
-    if (more) load_keys(i + 1, id);
-    const float v_log = EIGHT ? __log2f(vs_now) : 0.f, v_inv = EIGHT ? 1.f / vs_now : 1.f;
+    const float v_log = EIGHT ? __log2f(vs) : 0.f, v_inv = EIGHT ? 1.f / vs : 1.f;
     const bool whole = key0 + 16 <= min(hi, first_pos + 1) && key0 >= t.lo && (p.window == 0 || key0 > last_pos - p.window);
     bool grows = false;
 #pragma unroll
@@ -292,7 +268,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = s[n][e] + s2[n][e];
-        float v = EIGHT ? fmaf(x, factor[n][e & 1] * ks_now, v_log) : x * factor[n][e & 1];
+        float v = EIGHT ? fmaf(x, factor[n][e & 1] * ks, v_log) : x * factor[n][e & 1];
         if (!whole) {
           const int key = key0 + g + (e >> 1) * 8, pos = row_pos[n][e & 1];
           if (key >= hi || key > pos || (p.window > 0 && key <= pos - p.window)) v = -INFINITY;
@@ -337,43 +313,60 @@ __global__ void __launch_bounds__(kStepWarps * 32, D == 64 ? (NT == 1 ? 4 : 3) :
           l_run[n][1] = fmaf(rounded.y, v_inv, l_run[n][1]);
         }
       }
-    // value rows that no query row of the tile sees may hold anything
-    if (key0 + 16 > hi || key0 < t.lo) {
+    // ---- O^T += V^T P^T: value rows 2c, 2c + 1, 2c + 8, 2c + 9, dimensions by g ----
+    const bool edge = key0 + 16 > hi || key0 < t.lo;
+    constexpr int kPart = kValRegs < 4 ? kValRegs : 4;   // registers of a row at a time
+#pragma unroll
+    for (int j = 0; j < kValRegs / kPart; ++j) {
+      uint32_t vr[4][kPart];
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        const int key = key0 + 2 * c + (h & 1) + (h >> 1) * 8;
-        if (key >= hi || key < t.lo) {
+        const int row = 2 * c + (h & 1) + (h >> 1) * 8;
+        const uint8_t *y = tile + kHalf + row * kRowBytes + (kPart == 2 ? ((g >> 1) ^ swizzle(row)) * 16 + (g & 1) * 8 : ((8 * j + g) ^ swizzle(row)) * 16);
+        if constexpr (kPart == 2) {
+          const uint2 w = *reinterpret_cast<const uint2 *>(y);
+          vr[h][0] = w.x;
+          vr[h][1] = w.y;
+        } else {
+          const uint4 w = *reinterpret_cast<const uint4 *>(y);
+          vr[h][0] = w.x;
+          vr[h][1] = w.y;
+          vr[h][2] = w.z;
+          vr[h][3] = w.w;
+        }
+        // value rows that no query row of the tile sees may hold anything
+        if (edge && (key0 + row >= hi || key0 + row < t.lo)) {
 #pragma unroll
-          for (int j = 0; j < kValRegs; ++j) vr[h][j] = 0;
+          for (int e = 0; e < kPart; ++e) vr[h][e] = 0;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < (EIGHT ? 2 * kPart : kPart); ++q) {
+        const int k = j * (EIGHT ? 2 * kPart : kPart) + q;
+        uint32_t a0, a1, a2, a3;
+        if constexpr (EIGHT) {
+          // bytes 2 (q % 2) and the next of word q / 2: two dimensions of four keys
+          const uint32_t sel = (q & 1) ? 0x7362 : 0x5140;
+          const uint32_t x = __byte_perm(vr[0][q / 2], vr[1][q / 2], sel), y = __byte_perm(vr[2][q / 2], vr[3][q / 2], sel);
+          a0 = e4m3x2_to_half2(x);
+          a1 = e4m3x2_to_half2(x >> 16);
+          a2 = e4m3x2_to_half2(y);
+          a3 = e4m3x2_to_half2(y >> 16);
+        } else {
+          a0 = __byte_perm(vr[0][q], vr[1][q], 0x5410);
+          a1 = __byte_perm(vr[0][q], vr[1][q], 0x7632);
+          a2 = __byte_perm(vr[2][q], vr[3][q], 0x5410);
+          a3 = __byte_perm(vr[2][q], vr[3][q], 0x7632);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_tile<M>(acc[n][k], a0, a1, a2, a3, pf[n][0], pf[n][1]);
+          if constexpr (kSplitP) mma_tile<M>(acc[n][k], a0, a1, a2, a3, pl[n][0], pl[n][1]);
         }
       }
     }
-    // ---- O^T += V^T P^T ----
-#pragma unroll
-    for (int k = 0; k < kTiles; ++k) {
-      uint32_t a0, a1, a2, a3;
-      if constexpr (EIGHT) {
-        // bytes 2 (k % 2) and the next of word k / 2: two dimensions of four keys
-        const uint32_t sel = (k & 1) ? 0x7362 : 0x5140;
-        const uint32_t x = __byte_perm(vr[0][k / 2], vr[1][k / 2], sel), y = __byte_perm(vr[2][k / 2], vr[3][k / 2], sel);
-        a0 = e4m3x2_to_half2(x);
-        a1 = e4m3x2_to_half2(x >> 16);
-        a2 = e4m3x2_to_half2(y);
-        a3 = e4m3x2_to_half2(y >> 16);
-      } else {
-        a0 = __byte_perm(vr[0][k], vr[1][k], 0x5410);
-        a1 = __byte_perm(vr[0][k], vr[1][k], 0x7632);
-        a2 = __byte_perm(vr[2][k], vr[3][k], 0x5410);
-        a3 = __byte_perm(vr[2][k], vr[3][k], 0x7632);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma_tile<M>(acc[n][k], a0, a1, a2, a3, pf[n][0], pf[n][1]);
-        if constexpr (kSplitP) mma_tile<M>(acc[n][k], a0, a1, a2, a3, pl[n][0], pl[n][1]);
-      }
-    }
-    if (more) load_values(i + 1, id);
   }
+  __syncthreads();                                         // (the rings' memory holds the partial rows from here on)
 
   // ---- the warps' partial rows ----
 #pragma unroll
@@ -511,7 +504,22 @@ template <typename T, int D> __global__ void __launch_bounds__(128) paged_prompt
 }
 
 template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParams &p, cudaStream_t st) {
-  launch_pdl(paged_step_kernel<T, EIGHT, D, NT>, dim3(p.splits, p.kv_heads * p.row_tiles, p.batch.batch), dim3(kStepWarps * 32), 0, st, p);
+  constexpr int kTile = 16 * 2 * (EIGHT ? D : 2 * D), kRed = kStepWarps * 8 * NT * (D + 2) * 4;
+  // (64 sequences of 2048 to 4095 keys in e4m3, heads of 128: 76 us with two tiles, 77 with three, 86 with four, which cost resident CTAs;
+  // 32 of 1500, 16-bit heads of 64: 26, 23 and 23)
+  constexpr int kStages = D == 64 ? 3 : 2, kSmem = kStepWarps * kStages * kTile > kRed ? kStepWarps * kStages * kTile : kRed;
+  auto kern = paged_step_kernel<T, EIGHT, D, NT, kStages>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (kSmem > 48 * 1024 && (dev < 0 || dev >= 64 || !configured[dev])) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(EB_ECUDA, "paged_attention: cannot reserve %d bytes of shared memory", kSmem);
+    }
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  launch_pdl(kern, dim3(p.splits, p.kv_heads * p.row_tiles, p.batch.batch), dim3(kStepWarps * 32), kSmem, st, p);
   if (p.part) launch_pdl(paged_merge_kernel<T, D, NT>, dim3(p.tile_rows, p.kv_heads * p.row_tiles, p.batch.batch), dim3(128), 0, st, p);
   return check_launch("paged_attention");
 }
@@ -521,16 +529,18 @@ constexpr int kMostKeys = 8192, kLeastKeys = 256;
 struct StepPlan {
   int tiles8, row_tiles, chunk, splits;
 };
-StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys) {
+StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, int head_dim, bool eight) {
   StepPlan s;
-  s.tiles8 = rows_per_head > 8 ? 2 : 1;
+  // Tiles of 16 rows read the keys half as often (128 heads on 8, 64 sequences of 2048 to 4095 keys: 108 us, with tiles of 8 125), but not where the
+  // last one would be half empty (20 rows, 24 sequences, window 1024: 25 us, with three tiles of 8 21).
+  s.tiles8 = rows_per_head > 8 && !(rows_per_head > 16 && rows_per_head <= 24) ? 2 : 1;
   s.row_tiles = (rows_per_head + 8 * s.tiles8 - 1) / (8 * s.tiles8);
   const long long units = (long long)batch * kv_heads * s.row_tiles, sms = sm_count();
-  // Two CTAs per multiprocessor and more stream fast enough without splits; fewer are split to four per multiprocessor.  No CTA
-  // gets more than kMostKeys keys (a long sequence among short ones would keep the call waiting) nor fewer than kLeastKeys.  (64 sequences
-  // of 2048 to 4095 keys, 8 key / value heads: 87 us without splits, 96 with two, 86 with four.  A cluster per row that merges in shared
-  // memory was slower than a second launch at every size, 146 us there: clusters wait for room side by side.)
-  const long long want = units >= 2 * sms ? 1 : (4 * sms + units - 1) / units;
+  // CTAs that are resident at a time, as the launch bounds have it.  From half of them on there are no splits, fewer are split to fill
+  // them once.  No CTA gets more than kMostKeys keys (a long sequence among short ones would keep the call waiting) nor fewer
+  // than kLeastKeys.
+  const long long slots = sms * (head_dim == 64 ? (s.tiles8 == 1 ? 4 : 3) : s.tiles8 == 1 ? (eight ? 4 : 3) : 2);
+  const long long want = 2 * units >= slots ? 1 : slots / units;
   keys += 15;                                               // (the first tile may begin in front of the first key)
   long long chunk = (keys + want - 1) / want;
   if (chunk > kMostKeys) chunk = kMostKeys;
@@ -559,13 +569,13 @@ struct PagedPlan {
   PromptPlan tiles;
   size_t step_bytes, prompt_bytes;
 };
-PagedPlan paged_plan(int batch, int kv_heads, int group, int head_dim, int most_new, int most_length, int window) {
+PagedPlan paged_plan(int batch, int kv_heads, int group, int head_dim, bool eight, int most_new, int most_length, int window) {
   PagedPlan s{};
   const long long keys = step_keys(most_length, window, most_new);
   const int rows = most_new * group;
   s.prompt = rows > kFewRows;
   s.step_rows = s.prompt ? kFewRows : rows;
-  s.step = step_plan(batch, kv_heads, s.step_rows, s.prompt ? step_keys(most_length, window, kFewRows) : keys);
+  s.step = step_plan(batch, kv_heads, s.step_rows, s.prompt ? step_keys(most_length, window, kFewRows) : keys, head_dim, eight);
   s.step_bytes = step_scratch(s.step, batch, kv_heads, head_dim);
   if (s.prompt) {
     // a block's keys with a window: its own rows' and the window in front
@@ -584,10 +594,10 @@ template <typename T, int D> void launch_prompt_merge(const PromptParams &p, con
 
 using namespace eb;
 
-extern "C" size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window) {
+extern "C" size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int eight_bit, int most_new, int most_length, int window) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || head_dim <= 0 || most_new <= 0 || most_length <= 0 || window < 0 || heads % kv_heads) return 0;
   if ((long long)most_new * (heads / kv_heads) >= (1 << 30)) return 0;
-  const PagedPlan s = paged_plan(batch, kv_heads, heads / kv_heads, head_dim, most_new, most_length, window);
+  const PagedPlan s = paged_plan(batch, kv_heads, heads / kv_heads, head_dim, eight_bit != 0, most_new, most_length, window);
   return s.step_bytes + s.prompt_bytes;
 }
 
@@ -617,7 +627,7 @@ extern "C" int eb_paged_attention(const eb_paged *cache, const void *q, long lon
   if (most_length > reach) most_length = (int)reach;
   const int group = heads / kv_heads;
   EB_REQUIRE((long long)most_new * group < (1 << 30), "paged_attention: too many rows");
-  const PagedPlan plan = paged_plan(batch, kv_heads, group, head_dim, most_new, most_length, window);
+  const PagedPlan plan = paged_plan(batch, kv_heads, group, head_dim, k_scale != nullptr, most_new, most_length, window);
   const StepPlan &s = plan.step;
   EB_REQUIRE((long long)kv_heads * s.row_tiles <= 65535, "paged_attention: %d heads exceed the grid", kv_heads);
   const size_t need = plan.step_bytes + plan.prompt_bytes;

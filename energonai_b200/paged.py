@@ -175,7 +175,7 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     window = int(window)
     if window >= most_length:
         window = 0                                          # (every key is inside)
-    nbytes = _scratch_bytes(tables.shape[0], heads, kv_heads, head_dim, min(int(most_new), rows), most_length, window)
+    nbytes = _scratch_bytes(tables.shape[0], heads, kv_heads, head_dim, k_scale is not None, min(int(most_new), rows), most_length, window)
     scratch = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None       # (of this call: captured calls share none)
     check(lib().eb_paged_attention(cache, q.data_ptr(), ldq, out.data_ptr(), ldo, rows, heads, window, float(head_dim ** -0.5 if scale is None else scale),
                                    None if scratch is None else scratch.data_ptr(), nbytes, _stream_of(device)), "paged_attention", launches=2 if nbytes else 1)

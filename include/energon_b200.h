@@ -921,7 +921,7 @@ EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, 
  * device need scratch of their own. */
 EB_API int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,
                        void *scratch, size_t scratch_bytes, void *stream);
-EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int most_new, int most_length, int window);
+EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_heads, int head_dim, int eight_bit, int most_new, int most_length, int window);
 
 /* Low-rank adapters of many requests: for the rows starts[b] to starts[b + 1] - 1 (at most most_new) of each sequence, with
  * i = index[b],  delta = scales[i] (x a[i]^T) b[i]^T,  a [adapters][rank][width], b [adapters][columns][rank], rank a multiple

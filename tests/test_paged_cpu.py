@@ -94,14 +94,14 @@ def test_attention_refuses(change, words):
 def test_empty_batches_are_accepted():
     assert append_call(rows=0) == 0 and append_call(batch=0) == 0 and append_call(most_new=0) == 0
     assert attention_call(rows=0) == 0 and attention_call(batch=0) == 0
-    assert _lib.lib().eb_paged_attention_scratch_bytes(0, 8, 4, 64, 1, 100, 0) == 0
+    assert _lib.lib().eb_paged_attention_scratch_bytes(0, 8, 4, 64, 0, 1, 100, 0) == 0
 
 
 def test_scratch_grows_with_the_splits():
     need = _lib.lib().eb_paged_attention_scratch_bytes
-    assert need(1, 8, 8, 128, 1, 64, 0) == 0                              # one CTA per head sees all keys
-    assert need(1, 8, 8, 128, 1, 100000, 0) > 0
-    assert need(1, 8, 8, 128, 1, 100000, 128) == 0                        # a window is short
+    assert need(1, 8, 8, 128, 0, 1, 64, 0) == 0                              # one CTA per head sees all keys
+    assert need(1, 8, 8, 128, 0, 1, 100000, 0) > 0
+    assert need(1, 8, 8, 128, 0, 1, 100000, 128) == 0                        # a window is short
     assert ctypes.sizeof(ctypes.c_size_t) == 8
 
 
