@@ -529,7 +529,7 @@ constexpr int kMostKeys = 8192, kLeastKeys = 256;
 struct StepPlan {
   int tiles8, row_tiles, chunk, splits;
 };
-StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, int head_dim, bool eight) {
+StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, int head_dim, bool eight, bool beside) {
   StepPlan s;
   // Tiles of 16 rows read the keys half as often (128 heads on 8, 64 sequences of 2048 to 4095 keys: 108 us, with tiles of 8 125), but not where the
   // last one would be half empty (20 rows, 24 sequences, window 1024: 25 us, with three tiles of 8 21).
@@ -538,9 +538,9 @@ StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, i
   const long long units = (long long)batch * kv_heads * s.row_tiles, sms = sm_count();
   // CTAs that are resident at a time, as the launch bounds have it.  From half of them on there are no splits, fewer are split to fill
   // them once.  No CTA gets more than kMostKeys keys (a long sequence among short ones would keep the call waiting) nor fewer
-  // than kLeastKeys.
+  // than kLeastKeys.  Beside prompts, which take longer, there are splits only for the former.
   const long long slots = sms * (head_dim == 64 ? (s.tiles8 == 1 ? 4 : 3) : s.tiles8 == 1 ? (eight ? 4 : 3) : 2);
-  const long long want = 2 * units >= slots ? 1 : slots / units;
+  const long long want = beside || 2 * units >= slots ? 1 : slots / units;
   keys += 15;                                               // (the first tile may begin in front of the first key)
   long long chunk = (keys + want - 1) / want;
   if (chunk > kMostKeys) chunk = kMostKeys;
@@ -575,7 +575,7 @@ PagedPlan paged_plan(int batch, int kv_heads, int group, int head_dim, bool eigh
   const int rows = most_new * group;
   s.prompt = rows > kFewRows;
   s.step_rows = s.prompt ? kFewRows : rows;
-  s.step = step_plan(batch, kv_heads, s.step_rows, s.prompt ? step_keys(most_length, window, kFewRows) : keys, head_dim, eight);
+  s.step = step_plan(batch, kv_heads, s.step_rows, s.prompt ? step_keys(most_length, window, kFewRows) : keys, head_dim, eight, s.prompt);
   s.step_bytes = step_scratch(s.step, batch, kv_heads, head_dim);
   if (s.prompt) {
     // a block's keys with a window: its own rows' and the window in front

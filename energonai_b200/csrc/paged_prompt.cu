@@ -64,6 +64,12 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volat
   }
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x),
+               "r"(y), "r"(z), "r"(w), "r"(bar)
+               : "memory");
+}
+
 template <int D, bool EIGHT> struct PromptSmem {
   static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128, kPBytes = 2 * kRows * 128;
   static constexpr int kVStages = D > 64 ? 1 : 2;
@@ -75,11 +81,12 @@ template <int D, bool EIGHT> struct PromptSmem {
 // the value scale and its inverse, and a word of those in no page][Q][K: 2 stages][V][P]
 template <typename T, bool EIGHT, int D>
 __global__ void __launch_bounds__(PromptSmem<D, EIGHT>::kThreads, 1)
-paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
+paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
   using Smem = PromptSmem<D, EIGHT>;
   using M = typename std::conditional<EIGHT, __half, T>::type;
   constexpr int kSub = D / 64, kVStages = Smem::kVStages;
   constexpr uint32_t kQBytes = Smem::kQBytes, kKBytes = Smem::kKBytes, kPBytes = Smem::kPBytes, kTmemCols = 512, kPvCol = 2 * kKeys;
+  constexpr bool kScaled = EIGHT && std::is_same<T, __nv_bfloat16>::value;        // queries become fp16, a power of two per row
   constexpr float kLift = std::is_same<M, __half>::value ? kLiftHalf : 0.f;
   constexpr int kBf16 = std::is_same<M, __nv_bfloat16>::value ? 1 : 0;
   constexpr uint32_t kIdescS = tc_idesc(kKeys, kBf16), kIdescPV = tc_idesc(D, kBf16) | (1u << 16);     // bit 16: B is N-major
@@ -89,7 +96,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bar0 = s32(smem);
   const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56, s_full = bar0 + 72, p_full = bar0 + 88,
-                 pv_full = bar0 + 104, s_free = bar0 + 120;
+                 pv_full = bar0 + 104, s_free = bar0 + 120, q_raw = bar0 + 136;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 256);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 264);
   float *key_scale = reinterpret_cast<float *>(smem + 272), *value_log = key_scale + kScaleRing * 8, *value_inv = value_log + kScaleRing * 8;
@@ -139,7 +146,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_v) : "memory");
     }
-    bar_init(q_full, kRowTiles * 4);
+    bar_init(q_full, p.q_tma && !kScaled ? 1 : kRowTiles * 4);
+    bar_init(q_raw, 1);
     for (int s = 0; s < 2; ++s) {
       bar_init(k_full + 8 * s, EIGHT ? kConvertWarps : 1);
       bar_init(k_empty + 8 * s, kRowTiles);
@@ -152,6 +160,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (p.q_tma) {
+      // queries as soon as there is a barrier to land on: [tokens][heads of the group][D] as rows of a tile; those of bf16 models over codes wait
+      // in the memory of P to become fp16.  (Rows behind the sequence's last are the next one's, or zeros: they store nothing.)
+      const uint32_t bar = kScaled ? q_raw : q_full;
+      bar_expect_tx(bar, kRowTiles * kQBytes);
+#pragma unroll
+      for (int t = 0; t < kRowTiles; ++t)
+#pragma unroll
+        for (int kb = 0; kb < kSub; ++kb)
+          tma_load_4d((kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + kb * kRows * 128, &tm_q, bar, kb * 64, 0, hk, r.row0 + (q0 + t * kRows) / p.group);
+    }
   }
   if (warp == 1) {
     __syncwarp();
@@ -286,25 +305,28 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 8 * t, my_pv_full = pv_full + 8 * t, my_s_free = s_free + 8 * t;
     uint8_t *p_row = p_ptr + t * kPBytes + row * 128;
     float factor = p.scale_log2;                          // exponent of a score
+    bool alive = true;
     {
-      // The warp's 32 rows of Q, swizzled, D / 8 lanes per row, straight to shared memory: with most of it taken, the first-level
-      // cache is too small for as many loads to registers (6 us instead of 2 in front of the first product).
-      constexpr bool kScaled = EIGHT && std::is_same<T, __nv_bfloat16>::value;
-      constexpr int kLanesPer = D / 8, kRowsPer = 32 / kLanesPer;
-      const int sub = lane / kLanesPer, chunk = lane % kLanesPer;
-      const uint32_t dst = (kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + (chunk >> 3) * (kRows * 128);
+      if (p.q_tma) {
+        if (kScaled && !all_wait(q_raw, 0, 6)) alive = false;
+      } else {
+        // groups that do not divide a tile: the warp's 32 rows, swizzled, D / 8 lanes per row, straight to shared memory.  (With most of it
+        // taken, the first-level cache is too small for as many loads to registers: 6 us instead of 2 in front of the first product.)
+        constexpr int kLanesPer = D / 8, kRowsPer = 32 / kLanesPer;
+        const int sub = lane / kLanesPer, chunk = lane % kLanesPer;
+        const uint32_t dst = (kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + (chunk >> 3) * (kRows * 128);
 #pragma unroll 4
-      for (int i = 0; i < 32 / kRowsPer; ++i) {
-        // (token and head of the row, computed by its own lane)
-        const int from = i * kRowsPer + sub, to = quarter * 32 + from, tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from);
-        const bool ok = q0 + t * kRows + to < all;
-        const T *src = reinterpret_cast<const T *>(p.q) + (ok ? (long long)(r.row0 + tk) * p.ldq + (long long)hd * D + chunk * 8 : 0);
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + to * 128 + (((chunk & 7) ^ (to & 7)) << 4)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          // (token and head of the row, computed by its own lane)
+          const int from = i * kRowsPer + sub, to = quarter * 32 + from, tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from);
+          const bool ok = q0 + t * kRows + to < all;
+          const T *src = reinterpret_cast<const T *>(p.q) + (ok ? (long long)(r.row0 + tk) * p.ldq + (long long)hd * D + chunk * 8 : 0);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + to * 128 + (((chunk & 7) ^ (to & 7)) << 4)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      __syncwarp();
       if constexpr (kScaled) {
-        // queries of bf16 models wait in the memory of P to become fp16
         const uint8_t *from = p_row;
         uint8_t *to = q_ptr + t * kQBytes + row * 128;
         float m = 0.f;
@@ -328,14 +350,15 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                                                              pack2<__half>(f2.x * up, f2.y * up), pack2<__half>(f3.x * up, f3.y * up));
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) bar_arrive(q_full);
+      if (kScaled || !p.q_tma) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(q_full);
+      }
     }
     const int pos = r.past + token;
     const int vis_end = there ? min(pos + 1, reach) : 0, vis_begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;       // this row sees [vis_begin, vis_end)
     float m_ref = kNone, l_run = 0.f;
-    bool alive = ntiles > 0;
     for (int j = first_tile; j < ntiles && alive; ++j) {
       const int key0 = j * kKeys, slot = (j - jmin) & (kScaleRing - 1);
       if (!all_wait(my_s_full, (j - first_tile) & 1, 7)) { alive = false; break; }
@@ -613,7 +636,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
   }
 }
 
-template <typename T, bool EIGHT, int D> int launch_prompt(const CUtensorMap &mk, const CUtensorMap &mv, const PromptParams &p, dim3 grid, cudaStream_t st) {
+template <typename T, bool EIGHT, int D> int launch_prompt(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const PromptParams &p, dim3 grid, cudaStream_t st) {
   using Smem = PromptSmem<D, EIGHT>;
   static_assert(Smem::kTotal <= 227 * 1024, "shared memory");
   auto kern = paged_prompt_kernel<T, EIGHT, D>;
@@ -632,7 +655,7 @@ template <typename T, bool EIGHT, int D> int launch_prompt(const CUtensorMap &mk
     }
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  launch_pdl(kern, grid, dim3(Smem::kThreads), Smem::kTotal, st, mk, mv, p);
+  launch_pdl(kern, grid, dim3(Smem::kThreads), Smem::kTotal, st, mq, mk, mv, p);
   return check_launch("paged_attention");
 }
 
@@ -656,7 +679,18 @@ PromptPlan prompt_plan(int batch, int kv_heads, int rows_per_head, long long key
 
 int paged_prompt(PromptParams p, const PromptPlan &s, int head_dim, int dtype, cudaStream_t st) {
   const bool eight = p.k_scale != nullptr;
-  CUtensorMap mk{}, mv{};
+  CUtensorMap mq{}, mk{}, mv{};
+  p.q_tma = kRows % p.group == 0;
+  if (p.q_tma) {
+    EncodeFn fn = tc_encode_fn();
+    if (!fn) return fail(EB_ECUDA, "tensor map: cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[4] = {(cuuint64_t)head_dim, (cuuint64_t)p.group, (cuuint64_t)p.kv_heads, (cuuint64_t)p.batch.rows};
+    const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)p.group * head_dim * 2, (cuuint64_t)p.ldq * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.group, 1, (cuuint32_t)(kRows / p.group)}, ones[4] = {1, 1, 1, 1};
+    const CUresult r = fn(&mq, dtype == EB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(p.q), dims, strides, box, ones,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(EB_ECUDA, "tensor map: cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  }
   if (!eight) {
     const long long blocks = (long long)p.batch.pages * p.kv_heads, page = 1ll << p.batch.page_shift;
     if (blocks >= (1ll << 31)) return fail(EB_EUNSUPPORTED, "paged_attention: %lld blocks exceed the tensor map", blocks);
@@ -666,7 +700,7 @@ int paged_prompt(PromptParams p, const PromptPlan &s, int head_dim, int dtype, c
   p.splits = s.splits;
   p.split_tiles = s.split_tiles;
   const dim3 grid(s.blocks * s.splits, p.kv_heads, p.batch.batch);
-#define EB_PROMPT(T, E) (head_dim == 64 ? launch_prompt<T, E, 64>(mk, mv, p, grid, st) : launch_prompt<T, E, 128>(mk, mv, p, grid, st))
+#define EB_PROMPT(T, E) (head_dim == 64 ? launch_prompt<T, E, 64>(mq, mk, mv, p, grid, st) : launch_prompt<T, E, 128>(mq, mk, mv, p, grid, st))
   if (dtype == EB_F16) return eight ? EB_PROMPT(__half, true) : EB_PROMPT(__half, false);
   return eight ? EB_PROMPT(__nv_bfloat16, true) : EB_PROMPT(__nv_bfloat16, false);
 #undef EB_PROMPT

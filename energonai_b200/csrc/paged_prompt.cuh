@@ -16,6 +16,7 @@ struct PromptParams {
   float scale_log2;
   float *part;                           // [batch][kv_heads][blocks][splits][256][D + 2], or null: one split
   int splits, split_tiles;
+  int q_tma;                             // the heads of a group divide a row tile: queries come by tensor map
 };
 struct PromptPlan {
   int blocks, splits, split_tiles;       // CTAs of 256 rows per key / value head, splits of so many key tiles
