@@ -177,6 +177,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(tmem_slot)), "r"(kTmemCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // the pages of a tile, of lane l of warp 0; those of the first tiles are looked up on the way to the barrier
+  const int per_tile = kKeys >> p.batch.page_shift, page_size = 1 << p.batch.page_shift;
+  auto page_of = [&](int j) {                              // (one outside of the pool reads as zeros)
+    const int key = j * kKeys + (lane << p.batch.page_shift);
+    return lane < per_tile && j < nmax && key < hi && key + page_size > lo ? paged_page(p.batch, b, key >> p.batch.page_shift) : -1;
+  };
+  int now = -1, next = -1;
+  if (!EIGHT && warp == 0) {
+    now = page_of(jmin);
+    next = page_of(jmin + 1);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -193,11 +204,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   if (warp == 0) {
     // ---------------- 16-bit pages: TMA, a lane per page of a tile ----------------
     if (!EIGHT && nmax > jmin) {
-      const int per_tile = kKeys >> p.batch.page_shift, page_size = 1 << p.batch.page_shift;
-      auto page_of = [&](int j) {                          // page of this lane in tile j; one outside of the pool reads as zeros
-        const int key = j * kKeys + (lane << p.batch.page_shift);
-        return lane < per_tile && j < nmax && key < hi && key + page_size > lo ? paged_page(p.batch, b, key >> p.batch.page_shift) : -1;
-      };
       const int outside = p.batch.pages * p.kv_heads;
       auto load = [&](const CUtensorMap *map, uint32_t dst, uint32_t bar, int page) {
         if (lane == 0) bar_expect_tx(bar, kKBytes);
@@ -219,7 +225,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         load(&tm_k, k_addr + st * kKBytes, k_full + 8 * st, page);
         return true;
       };
-      int now = page_of(jmin), next = page_of(jmin + 1);
       bool ok = load_k(jmin, now);
       for (int j = jmin; j < nmax && ok; ++j) {
         const int i = j - jmin, vs = i % kVStages, vu = i / kVStages;
@@ -516,7 +521,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       float *part = p.part ? p.part + ((((long long)b * p.kv_heads + hk) * blocks + qb) * p.splits + split) * kCtaRows * (D + 2) + (long long)(t * kRows + row) * (D + 2) : nullptr;
       if (part && there) *reinterpret_cast<float2 *>(part + D) = make_float2(m_ref, l_run);
       const float inv = part ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
-      T *out = reinterpret_cast<T *>(p.o) + (long long)(r.row0 + token) * p.ldo + (long long)head * D;
+      // 16-bit rows go through the memory of P, which the last value product is done with: written by their threads, 16 bytes of 32 rows
+      // at a time, they took 6100 cycles
+      uint8_t *stage = p_ptr + t * kPBytes;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float x[32];
@@ -526,17 +533,30 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = 0.f;
         }
-        if (!there) continue;
         if (part) {
+          if (there)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2 *>(part + c * 32 + e) = make_float2(x[e], x[e + 1]);
+            for (int e = 0; e < 32; e += 2) *reinterpret_cast<float2 *>(part + c * 32 + e) = make_float2(x[e], x[e + 1]);
         } else {
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             const float *y = x + g * 8;
-            *reinterpret_cast<uint4 *>(out + c * 32 + g * 8) = make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv),
-                                                                          pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
+            *reinterpret_cast<uint4 *>(stage + (c >> 1) * (kRows * 128) + row * 128 + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) =
+                make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv), pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
           }
+        }
+      }
+      if (!part) {
+        __syncwarp();
+        constexpr int kLanesPer = D / 8, kRowsPer = 32 / kLanesPer;
+        const int sub = lane / kLanesPer, chunk = lane % kLanesPer;
+        T *out = reinterpret_cast<T *>(p.o) + chunk * 8;
+#pragma unroll 4
+        for (int i = 0; i < 32 / kRowsPer; ++i) {
+          const int from = i * kRowsPer + sub, of = quarter * 32 + from, tk = __shfl_sync(0xffffffffu, token, from), hd = __shfl_sync(0xffffffffu, head, from);
+          if (q0 + t * kRows + of < all)
+            *reinterpret_cast<uint4 *>(out + (long long)(r.row0 + tk) * p.ldo + (long long)hd * D) =
+                *reinterpret_cast<const uint4 *>(stage + (chunk >> 3) * (kRows * 128) + of * 128 + (((chunk & 7) ^ (of & 7)) << 4));
         }
       }
     }
