@@ -62,11 +62,16 @@ _stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def _one_device(what, *tensors):
     """All tensors (or None) are on the current device; returns its number."""
-    on = {t.get_device() for t in tensors if t is not None}
-    if on != {_device_here()} if -1 not in on else True:
-        require_cuda(*tensors)
-        raise RuntimeError(f"{what}: all tensors must be on the current device (cuda:{_device_here()})")
-    return on.pop()
+    here = None
+    for t in tensors:
+        if t is not None:
+            on = t.get_device()
+            if on != here:
+                if here is not None or on < 0 or on != _device_here():
+                    require_cuda(*tensors)
+                    raise RuntimeError(f"{what}: all tensors must be on the current device (cuda:{_device_here()})")
+                here = on
+    return here
 
 
 def _rows(what, t, width, dtype):
@@ -96,7 +101,9 @@ def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_sc
         held, ks, vs = dtype, 0, 0
     else:
         held = torch.float8_e4m3fn
-        if k_scale is None or v_scale is None or any(s.dtype is not torch.float32 or s.shape != shape[:2] or not s.is_contiguous() for s in (k_scale, v_scale)):
+        per_block = shape[:2]
+        if k_scale is None or v_scale is None or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32 or k_scale.shape != per_block or (
+                v_scale.shape != per_block) or not k_scale.is_contiguous() or not v_scale.is_contiguous():
             raise RuntimeError(f"{what}: scales are contiguous fp32 [pages, kv_heads], for keys and for values")
         ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
     if k_pages.dtype is not held or v_pages.dtype is not held:
@@ -137,7 +144,7 @@ def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, f
         if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * pairs > head_dim:
             raise RuntimeError("paged_append: frequencies are fp32, one for each leading pair of a head")
         if q_out is None:
-            q_out = q.new_empty((rows, columns))
+            q_out = torch.empty_like(q)                     # (contiguous: rows of q are)
     ldo = 0
     if q_out is not None:
         ldo = _rows("paged_append", q_out, columns, dtype)
@@ -167,7 +174,8 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     heads = columns // head_dim
     ldq = _rows("paged_attention", q, columns, dtype)
     if out is None:
-        out, ldo = q.new_empty((rows, columns)), columns
+        out = torch.empty_like(q)                           # (contiguous: rows of q are)
+        ldo = columns
     else:
         ldo = _rows("paged_attention", out, columns, dtype)
         if out.shape[0] != rows:

@@ -1,0 +1,105 @@
+"""An attention layer as a server of many requests runs it: projections with an adapter per request, new tokens into paged caches, attention over
+them, the output projection; prompts, single tokens, and both in one batch.  Every stage is held to its restatement in 64 bits on
+what the stage before left."""
+import pytest
+import torch
+
+from paged_plain import Case
+from test_adapter_gpu import UNIT, Case as Adapters
+from test_paged_gpu import check_append, close, frequencies
+
+pytestmark = pytest.mark.gpu
+
+
+def product(x, c, w):
+    """(x w^T + adapters, tolerance), as in the adapters' own test."""
+    y, size = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    c.x = x
+    delta, tol = c.delta()
+    return y + delta, UNIT[c.dtype] * (y + delta).abs() + tol + (2.0 ** -23 * x.shape[1] / 16 + 2.0 ** -20) * size
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_an_attention_layer_serves_many_requests(bits, dtype):
+    from energonai_b200.adapter import adapter_product
+    from energonai_b200.gemm import device_status
+    from energonai_b200.paged import page_pools, paged_append, paged_attention, paged_batch
+    H, G, D, page, width, pages = 8, 2, 64, 16, 512, 64
+    B, columns = 4, (H + 2 * G) * D
+    into, out_of = Adapters([1], width, columns, 16, 3, dtype, seed=1), Adapters([1], H * D, width, 16, 3, dtype, seed=2)
+    freq = frequencies(D // 2).float()
+    pools = page_pools(pages, page, G, D, torch.float8_e4m3fn if bits == 8 else dtype)
+    k_pages, v_pages, k_scale, v_scale = pools
+    for p in (k_pages, v_pages):
+        p.view(torch.uint8).fill_(0x7f)                                       # NaN, or close to it, wherever nothing was written
+    g = torch.Generator().manual_seed(5)
+    free = torch.randperm(pages, generator=g).tolist()
+    tables, length = [[] for _ in range(B)], [0] * B
+    index = torch.tensor([2, -1, 0, 2], dtype=torch.int32)
+    for new in ([70, 5, 0, 33], [1, 1, 1, 1], [1, 90, 1, 0], [3, 1, 2, 1], [1, 1, 1, 1]):
+        for b in range(B):
+            length[b] += new[b]
+            while len(tables[b]) * page < length[b]:
+                tables[b].append(free.pop())
+        t, starts, lengths, most_new, most_length = paged_batch(new, length, tables, pages, page)
+        rows = sum(new)
+        x = torch.randn(rows, width, generator=g).to(dtype)
+        common = (index.cuda(), starts, most_new)
+        proj = adapter_product(x.cuda(), into.w.cuda(), into.a.cuda(), into.b.cuda(), into.scales.cuda(), *common)
+        for c in (into, out_of):
+            c.new, c.starts, c.rows, c.index = new, starts.tolist(), rows, index
+        close(proj, *product(x, into, into.w), "projection")
+
+        q, k, v = proj[:, :H * D], proj[:, H * D:(H + G) * D], proj[:, (H + G) * D:]
+        c = Case([0], [0], H, G, D, page, dtype, bits)
+        c.new, c.length, c.past, c.tables, c.starts, c.rows, c.pages = new, list(length), [n - m for n, m in zip(length, new)], tables, starts.tolist(), rows, pages
+        c.q, c.k, c.v = (y.cpu() for y in (q, k, v))
+        c.pool, c.scale = [p.cpu() for p in pools[:2]], [s.cpu() if s is not None else None for s in pools[2:]]
+        turned = paged_append(q, k, v, k_pages, v_pages, t, starts, lengths, most_new, freq=freq.cuda(), k_scale=k_scale, v_scale=v_scale)
+        check_append(c, D // 2, turned, pools[:2], pools[2:])
+
+        c.q, c.pool, c.scale = turned.cpu(), [p.cpu() for p in pools[:2]], [s.cpu() if s is not None else None for s in pools[2:]]
+        attended = paged_attention(turned, k_pages, v_pages, t, starts, lengths, most_new, most_length, k_scale=k_scale, v_scale=v_scale)
+        close(attended, *c.attention(prompt=64 * G // H), "attention")
+
+        y = adapter_product(attended, out_of.w.cuda(), out_of.a.cuda(), out_of.b.cuda(), out_of.scales.cuda(), *common)
+        close(y, *product(attended.cpu(), out_of, out_of.w), "output")
+    assert device_status()[0] == 0
+
+
+def test_two_streams_at_once():
+    """Calls on two streams share no scratch."""
+    from energonai_b200.adapter import adapter_product
+    from energonai_b200.paged import paged_attention
+    cases = [Case([1, 1], [9000, 5000], 8, 2, 64, 16, torch.float16, 8, seed=s) for s in (1, 2)]
+    more = [Adapters([40, 3], 512, 256, 16, 2, torch.float16, seed=s) for s in (3, 4)]
+
+    def run(c, a):
+        (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c
+        x, w, rest = a
+        return paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), adapter_product(x, w, *rest)
+
+    inputs = [(c.device(), (a.x.cuda(), a.w.cuda(), a.device())) for c, a in zip(cases, more)]
+    want = [run(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(5):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(run(*inputs[n])[0])
+    torch.cuda.synchronize()
+    for n in (0, 1):
+        assert all(torch.equal(o, want[n][0]) for o in got[n])
+
+
+def test_tables_of_a_wider_table():
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 7], [40, 90], 4, 2, 64, 32, torch.bfloat16, 16, seed=7)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    wide = torch.full((2, 50), 1 << 30, dtype=torch.int32, device="cuda")
+    wide[:, 3:3 + tables.shape[1]] = tables
+    part = wide[:, 3:3 + tables.shape[1]]
+    got = paged_attention(q, *pools, part, starts, lengths, most_new)
+    assert torch.equal(got, paged_attention(q, *pools, tables, starts, lengths, most_new))
+    close(got, *c.attention())
