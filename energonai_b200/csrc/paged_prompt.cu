@@ -28,8 +28,8 @@
 namespace eb {
 namespace {
 
-constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kConvertWarps = 4, kSoftmaxWarp = 4, kConvertWarp = kSoftmaxWarp + 4 * kRowTiles, kScaleRing = 4;
-constexpr float kRaise = 8.f, kMostSum = 256.f;           // the reference of a row is raised when a tile's weights add up to more
+constexpr int kKeys = 128, kRowTiles = 2, kCtaRows = kRowTiles * kRows, kHalf = 64, kConvertWarps = 4, kSoftmaxWarp = 4, kConvertWarp = kSoftmaxWarp + 4 * kRowTiles, kScaleRing = 4;
+constexpr float kRaise = 8.f;               // the reference of a row is raised when a score exceeds it by 2^8
 constexpr float kLiftHalf = 6.f;             // fp16 weights are 2^6 times as large, up to 2^14: fewer fall below the normal range
 constexpr float kNone = -3.402823466e38f;
 
@@ -64,6 +64,16 @@ __device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, volat
   }
 }
 
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                 "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+  tc_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 16; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z, int w) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x),
                "r"(y), "r"(z), "r"(w), "r"(bar)
@@ -71,38 +81,39 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 }
 
 template <int D, bool EIGHT> struct PromptSmem {
-  static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128, kPBytes = 2 * kRows * 128;
-  static constexpr int kVStages = D > 64 ? 1 : 2;
+  static constexpr uint32_t kQBytes = (D / 64) * kRows * 128, kKBytes = (D / 64) * kKeys * 128;
+  static constexpr int kKStages = 3, kVStages = 2;
   static constexpr int kThreads = (kConvertWarp + (EIGHT ? kConvertWarps : 0)) * 32;
-  static constexpr size_t kTotal = 1024 + 1024 + (size_t)kRowTiles * (kQBytes + kPBytes) + (2 + kVStages) * (size_t)kKBytes;
+  static constexpr size_t kTotal = 1024 + 1024 + (size_t)kRowTiles * kQBytes + (kKStages + kVStages) * (size_t)kKBytes;
 };
 
 // Shared memory (1024-aligned): [1 KB: barriers, TMEM slot, abort flag, per 16 keys of the last four tiles: key scale, log2 of
-// the value scale and its inverse, and a word of those in no page][Q][K: 2 stages][V][P]
+// the value scale and its inverse, and a word of those in no page][Q][K: 3 stages][V: 2 stages]
 template <typename T, bool EIGHT, int D>
 __global__ void __launch_bounds__(PromptSmem<D, EIGHT>::kThreads, 1)
 paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PromptParams p) {
   using Smem = PromptSmem<D, EIGHT>;
   using M = typename std::conditional<EIGHT, __half, T>::type;
-  constexpr int kSub = D / 64, kVStages = Smem::kVStages;
-  constexpr uint32_t kQBytes = Smem::kQBytes, kKBytes = Smem::kKBytes, kPBytes = Smem::kPBytes, kTmemCols = 512, kPvCol = 2 * kKeys;
+  constexpr int kSub = D / 64, kKStages = Smem::kKStages, kVStages = Smem::kVStages;
+  constexpr uint32_t kQBytes = Smem::kQBytes, kKBytes = Smem::kKBytes, kTmemCols = 512, kPvCol = 2 * kKeys;
   constexpr bool kScaled = EIGHT && std::is_same<T, __nv_bfloat16>::value;        // queries become fp16, a power of two per row
   constexpr float kLift = std::is_same<M, __half>::value ? kLiftHalf : 0.f;
   constexpr int kBf16 = std::is_same<M, __nv_bfloat16>::value ? 1 : 0;
-  constexpr uint32_t kIdescS = tc_idesc(kKeys, kBf16), kIdescPV = tc_idesc(D, kBf16) | (1u << 16);     // bit 16: B is N-major
+  constexpr uint32_t kIdescS = tc_idesc(kHalf, kBf16), kIdescPV = tc_idesc(D, kBf16) | (1u << 16);     // bit 16: B is N-major
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = s32(smem_raw);
   uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bar0 = s32(smem);
-  const uint32_t q_full = bar0, k_full = bar0 + 8, k_empty = bar0 + 24, v_full = bar0 + 40, v_empty = bar0 + 56, s_full = bar0 + 72, p_full = bar0 + 88,
-                 pv_full = bar0 + 104, s_free = bar0 + 120, q_raw = bar0 + 136;
+  // per stage of K and V; per row tile; per row tile and buffer of P
+  const uint32_t q_full = bar0, q_raw = bar0 + 8, k_full = bar0 + 16, k_empty = bar0 + 40, v_full = bar0 + 64, v_empty = bar0 + 80, s_full = bar0 + 96, s_free = bar0 + 112,
+                 p_full = bar0 + 128, pv_full = bar0 + 160;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 256);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 264);
   float *key_scale = reinterpret_cast<float *>(smem + 272), *value_log = key_scale + kScaleRing * 8, *value_inv = value_log + kScaleRing * 8;
   uint32_t *no_page = reinterpret_cast<uint32_t *>(value_inv + kScaleRing * 8);
-  uint8_t *q_ptr = smem + 1024, *k_ptr = q_ptr + kRowTiles * kQBytes, *v_ptr = k_ptr + 2 * kKBytes, *p_ptr = v_ptr + kVStages * kKBytes;
-  const uint32_t q_addr = s32(q_ptr), k_addr = s32(k_ptr), v_addr = s32(v_ptr), p_addr = s32(p_ptr);
+  uint8_t *q_ptr = smem + 1024, *k_ptr = q_ptr + kRowTiles * kQBytes, *v_ptr = k_ptr + kKStages * kKBytes;
+  const uint32_t q_addr = s32(q_ptr), k_addr = s32(k_ptr), v_addr = s32(v_ptr);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
@@ -110,18 +121,18 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const PagedRows r = paged_rows(p.batch, b);
   const int all = r.count * p.group, q0 = qb * kCtaRows, reach = p.batch.table_cols << p.batch.page_shift;
   if (all <= p.few || q0 >= all) return;
-  // Key tiles that each row tile walks, [ks, nt), none for one that lies behind the sequence's rows; the CTA's own are [jmin, nmax).
-  // Keys outside of [lo, hi) are seen by no row of the CTA.
-  int nt[kRowTiles], ks[kRowTiles], nmax = 0, jmin = 0x7fffffff, lo = 0x7fffffff, hi = 0;
+  // Halves of key tiles (64 keys) that each row tile walks, [hs, he), none for one that lies behind the sequence's rows; the CTA's own tiles
+  // are [jmin, nmax).  Keys outside of [lo, hi) are seen by no row of the CTA.
+  int hs[kRowTiles], he[kRowTiles], nmax = 0, jmin = 0x7fffffff, lo = 0x7fffffff, hi = 0;
 #pragma unroll
   for (int t = 0; t < kRowTiles; ++t) {
     const int a = q0 + t * kRows, z = min(a + kRows, all) - 1;
     const int first = p.window > 0 ? max(0, r.past + a / p.group - p.window + 1) : 0, end = a < all ? min(r.past + z / p.group + 1, reach) : 0;
-    nt[t] = (end + kKeys - 1) / kKeys;
-    ks[t] = first / kKeys;
-    if (nt[t] > ks[t]) {
-      jmin = min(jmin, ks[t]);
-      nmax = max(nmax, nt[t]);
+    he[t] = (end + kHalf - 1) / kHalf;
+    hs[t] = first / kHalf;
+    if (he[t] > hs[t]) {
+      jmin = min(jmin, hs[t] / 2);
+      nmax = max(nmax, (he[t] + 1) / 2);
       lo = min(lo, first);
       hi = max(hi, end);
     }
@@ -133,13 +144,13 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     nmax = min(nmax, split == p.splits - 1 ? nmax : jmin + p.split_tiles);
 #pragma unroll
     for (int t = 0; t < kRowTiles; ++t) {
-      ks[t] = max(ks[t], jmin);
-      nt[t] = min(nt[t], nmax);
+      hs[t] = max(hs[t], 2 * jmin);
+      he[t] = min(he[t], 2 * nmax);
     }
   }
 #pragma unroll
   for (int t = 0; t < kRowTiles; ++t)
-    if (nt[t] <= ks[t]) nt[t] = ks[t] = 0;                // (walks nothing)
+    if (he[t] <= hs[t]) he[t] = hs[t] = 0;                // (walks nothing)
 
   if (threadIdx.x == 0) {
     if (!EIGHT) {
@@ -148,28 +159,34 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
     bar_init(q_full, p.q_tma && !kScaled ? 1 : kRowTiles * 4);
     bar_init(q_raw, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kKStages; ++s) {
       bar_init(k_full + 8 * s, EIGHT ? kConvertWarps : 1);
       bar_init(k_empty + 8 * s, kRowTiles);
+    }
+    for (int s = 0; s < kVStages; ++s) {
       bar_init(v_full + 8 * s, EIGHT ? kConvertWarps : 1);
       bar_init(v_empty + 8 * s, kRowTiles);
-      bar_init(s_full + 8 * s, 1);
+    }
+    for (int t = 0; t < kRowTiles; ++t) {
+      bar_init(s_full + 8 * t, 1);
+      bar_init(s_free + 8 * t, 4);
+    }
+    for (int s = 0; s < 2 * kRowTiles; ++s) {
       bar_init(p_full + 8 * s, 4);
-      bar_init(s_free + 8 * s, 4);
       bar_init(pv_full + 8 * s, 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (p.q_tma) {
-      // queries as soon as there is a barrier to land on: [tokens][heads of the group][D] as rows of a tile; those of bf16 models over codes wait
-      // in the memory of P to become fp16.  (Rows behind the sequence's last are the next one's, or zeros: they store nothing.)
+      // queries as soon as there is a barrier to land on: [tokens][heads of the group][D] as rows of a tile; those of bf16 models over codes then become
+      // fp16 where they lie.  (Rows behind the sequence's last are the next one's, or zeros: they store nothing.)
       const uint32_t bar = kScaled ? q_raw : q_full;
       bar_expect_tx(bar, kRowTiles * kQBytes);
 #pragma unroll
       for (int t = 0; t < kRowTiles; ++t)
 #pragma unroll
         for (int kb = 0; kb < kSub; ++kb)
-          tma_load_4d((kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + kb * kRows * 128, &tm_q, bar, kb * 64, 0, hk, r.row0 + (q0 + t * kRows) / p.group);
+          tma_load_4d(q_addr + t * kQBytes + kb * kRows * 128, &tm_q, bar, kb * 64, 0, hk, r.row0 + (q0 + t * kRows) / p.group);
     }
   }
   if (warp == 1) {
@@ -215,8 +232,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
       };
       auto load_k = [&](int j, int page) -> bool {
-        const int i = j - jmin, st = i & 1;
-        if (i >= 2 && !all_wait(k_empty + 8 * st, ((i >> 1) - 1) & 1, 1)) return false;
+        const int i = j - jmin, st = i % kKStages;
+        if (i >= kKStages && !all_wait(k_empty + 8 * st, (i / kKStages - 1) & 1, 1)) return false;
         // groups of 16 keys without a page, where some row could see them
         const int key = j * kKeys + (lane << p.batch.page_shift), groups = page_size >> 4;
         uint32_t mine = lane < per_tile && page < 0 && key < hi && key + page_size > lo ? ((1u << groups) - 1) << (lane * groups) : 0;
@@ -238,45 +255,46 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else if (warp <= kRowTiles) {
     // ---------------- MMA issuers: a warp per row tile ----------------
-    // S(first), then for every key tile j: S(j + 1), as soon as S(j) has been read, so that the softmax warps find their next scores
-    // ready, and O += P(j) V(j), as soon as P(j) is written.  Both warps hand back every stage, those of tiles that theirs does not
-    // walk too, each when it is full (an earlier arrival would count for the stage's use before).
-    const int t = warp - 1, first = t == 0 ? ks[0] : ks[1], end = t == 0 ? nt[0] : nt[1];
+    // S(first), then for every half n: S(n + 1), as soon as S(n) is in registers, and O += P(n) V(n), as soon as P(n) is written.  Both warps
+    // hand back every stage, those of tiles that theirs does not walk too, each when it is full (an earlier arrival would count for
+    // the stage's use before).
+    const int t = warp - 1, first = t == 0 ? hs[0] : hs[1], end = t == 0 ? he[0] : he[1];
+    const uint32_t t_s = tmem + t * kKeys, t_p = t_s + kHalf, t_pv = t_s + kPvCol;
     auto pass = [&](int j) -> bool {                       // a tile that this row tile does not walk
-      const int i = j - jmin, vs = i % kVStages;
-      if (!all_wait(k_full + 8 * (i & 1), (i >> 1) & 1, 3)) return false;
-      if (lane == 0) bar_arrive(k_empty + 8 * (i & 1));
+      const int i = j - jmin, ks = i % kKStages, vs = i % kVStages;
+      if (!all_wait(k_full + 8 * ks, (i / kKStages) & 1, 3)) return false;
+      if (lane == 0) bar_arrive(k_empty + 8 * ks);
       if (!all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10)) return false;
       if (lane == 0) bar_arrive(v_empty + 8 * vs);
       return true;
     };
-    auto issue_scores = [&](int j) -> bool {
-      const int st = (j - jmin) & 1;
-      if (!all_wait(k_full + 8 * st, ((j - jmin) >> 1) & 1, 3)) return false;
+    auto issue_scores = [&](int n) -> bool {
+      const int i = (n >> 1) - jmin, st = i % kKStages;
+      if (!all_wait(k_full + 8 * st, (i / kKStages) & 1, 3)) return false;
       tc_fence_after();
 #pragma unroll
       for (int kb = 0; kb < kSub; ++kb) {
-        const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128);
+        const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128 + (n & 1) * kHalf * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_warp(tmem + t * kKeys, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) tc_mma_warp(t_s, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
       }
       tc_commit_warp(s_full + 8 * t);
-      tc_commit_warp(k_empty + 8 * st);
+      if ((n & 1) || n + 1 == end) tc_commit_warp(k_empty + 8 * st);
       return true;
     };
     bool ok = true;
     if (end > first) {
-      for (int j = jmin; j < first && ok; ++j) ok = pass(j);
+      for (int j = jmin; j < first / 2 && ok; ++j) ok = pass(j);
       ok = ok && all_wait(q_full, 0, 2) && issue_scores(first);
-      for (int j = first; j < end && ok; ++j) {
-        const int i = j - jmin, vs = i % kVStages;
-        if (j + 1 < end) ok = all_wait(s_free + 8 * t, (j - first) & 1, 4) && issue_scores(j + 1);
-        ok = ok && all_wait(p_full + 8 * t, (j - first) & 1, 5) && all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10);
+      for (int n = first; n < end && ok; ++n) {
+        const int at = n - first, buf = at & 1, j = n >> 1, i = j - jmin, vs = i % kVStages;
+        if (n + 1 < end) ok = all_wait(s_free + 8 * t, at & 1, 4) && issue_scores(n + 1);
+        ok = ok && all_wait(p_full + 8 * (2 * t + buf), (at >> 1) & 1, 5) && all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10);
         if (!ok) break;
-        if (!EIGHT && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
+        if (!EIGHT && ((n & 1) == 0 || n == first) && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
           // value rows that no row sees may hold anything, and a weight of 0 does not make them 0 (both warps may write these zeros)
-          for (int n = lane; n < kKeys * kSub * 8; n += 32) {
-            const int row = n / (kSub * 8), key = j * kKeys + row, c = n % (kSub * 8);
+          for (int e = lane; e < kKeys * kSub * 8; e += 32) {
+            const int row = e / (kSub * 8), key = j * kKeys + row, c = e % (kSub * 8);
             if (key < lo || key >= hi) *reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes + (c >> 3) * (kKeys * 128) + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -284,20 +302,16 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         }
         tc_fence_after();
 #pragma unroll
-        for (int a2 = 0; a2 < 2; ++a2) {
-          const uint64_t a = tc_desc(p_addr + t * kPBytes + a2 * kRows * 128);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile
-            const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + (a2 * 4 + k) * 2048, kKeys * 128);
-            tc_mma_warp(tmem + kPvCol + t * kKeys, a + 2 * k, bd, kIdescPV, (j > first || a2 > 0 || k > 0) ? 1u : 0u);
-          }
+        for (int k = 0; k < 4; ++k) {
+          // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile, eight columns of P
+          const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + ((n & 1) * 4 + k) * 2048, kKeys * 128);
+          tc_mma_ts_warp(t_pv, t_p + buf * (kHalf / 2) + k * 8, bd, kIdescPV, (at > 0 || k > 0) ? 1u : 0u);
         }
-        tc_commit_warp(pv_full + 8 * t);
-        tc_commit_warp(v_empty + 8 * vs);
+        tc_commit_warp(pv_full + 8 * (2 * t + buf));
+        if ((n & 1) || n + 1 == end) tc_commit_warp(v_empty + 8 * vs);
       }
     }
-    for (int j = max(end, jmin); j < nmax && ok; ++j) ok = pass(j);
+    for (int j = max((end + 1) / 2, jmin); j < nmax && ok; ++j) ok = pass(j);
   } else if (warp >= kSoftmaxWarp && warp < kConvertWarp) {
     if (EIGHT) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
@@ -305,21 +319,21 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int t = (warp - kSoftmaxWarp) >> 2, quarter = warp & 3, row = quarter * 32 + lane, at = q0 + t * kRows + row;
     const bool there = at < all;
     const int token = at / p.group, head = hk * p.group + at % p.group;
-    const int ntiles = nt[t], first_tile = ks[t];
-    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_pv = t_s + kPvCol;
-    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 8 * t, my_pv_full = pv_full + 8 * t, my_s_free = s_free + 8 * t;
-    uint8_t *p_row = p_ptr + t * kPBytes + row * 128;
+    const int end_half = t == 0 ? he[0] : he[1], first_half = t == 0 ? hs[0] : hs[1];
+    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_p = t_s + kHalf, t_pv = t_s + kPvCol;
+    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 16 * t, my_pv_full = pv_full + 16 * t, my_s_free = s_free + 8 * t;
     float factor = p.scale_log2;                          // exponent of a score
     bool alive = true;
     {
       if (p.q_tma) {
-        if (kScaled && !all_wait(q_raw, 0, 6)) alive = false;
+        // (waited for by rows that walk nothing too: their memory is used below, and nothing may be on its way when the CTA leaves)
+        if (!all_wait(kScaled ? q_raw : q_full, 0, 6)) alive = false;
       } else {
         // groups that do not divide a tile: the warp's 32 rows, swizzled, D / 8 lanes per row, straight to shared memory.  (With most of it
         // taken, the first-level cache is too small for as many loads to registers: 6 us instead of 2 in front of the first product.)
         constexpr int kLanesPer = D / 8, kRowsPer = 32 / kLanesPer;
         const int sub = lane / kLanesPer, chunk = lane % kLanesPer;
-        const uint32_t dst = (kScaled ? p_addr + t * kPBytes : q_addr + t * kQBytes) + (chunk >> 3) * (kRows * 128);
+        const uint32_t dst = q_addr + t * kQBytes + (chunk >> 3) * (kRows * 128);
 #pragma unroll 4
         for (int i = 0; i < 32 / kRowsPer; ++i) {
           // (token and head of the row, computed by its own lane)
@@ -332,8 +346,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         __syncwarp();
       }
       if constexpr (kScaled) {
-        const uint8_t *from = p_row;
         uint8_t *to = q_ptr + t * kQBytes + row * 128;
+        const uint8_t *from = to;
         float m = 0.f;
 #pragma unroll 4
         for (int i = 0; i < D / 8; ++i) {
@@ -364,50 +378,77 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int pos = r.past + token;
     const int vis_end = there ? min(pos + 1, reach) : 0, vis_begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;       // this row sees [vis_begin, vis_end)
     float m_ref = kNone, l_run = 0.f;
-    for (int j = first_tile; j < ntiles && alive; ++j) {
-      const int key0 = j * kKeys, slot = (j - jmin) & (kScaleRing - 1);
-      if (!all_wait(my_s_full, (j - first_tile) & 1, 7)) { alive = false; break; }
+    for (int n = first_half; n < end_half && alive; ++n) {
+      const int at_half = n - first_half, buf = at_half & 1, key0 = n * kHalf, slot = ((n >> 1) - jmin) & (kScaleRing - 1), c0 = (n & 1) * 2;      // (c0: the half's first chunk of 32 keys in its tile)
+      if (!all_wait(my_s_full, at_half & 1, 7)) { alive = false; break; }
       tc_fence_after();
+      float x0[32], x1[32];
+      tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
+      tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
       // groups of 16 keys without a page
-      const uint32_t gone = EIGHT ? 0 : no_page[slot];
+      const uint32_t gone = EIGHT ? 0 : no_page[slot] >> (2 * c0) & 15;
+      // most halves of a long prompt: every row sees every key
+      const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kHalf <= vis_end)) && !gone;
+      tc_ld_wait_for(x0, x1);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(my_s_free);                // (the scores are in registers: the next ones may come)
       // Which of 32 keys this row sees.  (Rows behind the sequence's last count as seeing all, which leaves it to the others.)
-      auto seen = [&](int c) {
+      auto hide = [&](float (&x)[32], int c) {
         const int end = vis_end - (key0 + c * 32), begin = vis_begin - (key0 + c * 32);
         uint32_t bits = end >= 32 ? 0xffffffffu : end <= 0 ? 0u : (1u << end) - 1u;
         if (begin > 0) bits &= begin >= 32 ? 0u : ~((1u << begin) - 1u);
         if (!EIGHT && gone) bits &= ((gone >> (2 * c)) & 1 ? 0u : 0xffffu) | ((gone >> (2 * c)) & 2 ? 0u : 0xffff0000u);
-        return there ? bits : 0xffffffffu;
-      };
-      // most tiles of a long prompt: every row sees every key
-      const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kKeys <= vis_end)) && !gone;
-      auto hide = [&](float (&x)[32], int c) {
-        const uint32_t bits = seen(c);
+        if (!there) bits = 0xffffffffu;
 #pragma unroll
         for (int e = 0; e < 32; ++e) x[e] = (bits >> e) & 1 ? x[e] : -INFINITY;
       };
+      if (!whole) {
+        hide(x0, 0);
+        hide(x1, 1);
+      }
       // factor and summand of a group's exponents (the factor is never 0, which would make a NaN of a hidden score)
-      auto group_factor = [&](int g) { return EIGHT ? fmaxf(factor * key_scale[slot * 8 + g], 1e-37f) : factor; };
-      auto group_log = [&](int g) { return EIGHT ? value_log[slot * 8 + g] : 0.f; };
-      auto largest = [&](const float (&x)[32], int c) {    // exponent of 32 keys
-        float m = kNone;
+      float factors[4], logs[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float r0 = x[h * 16], r1 = x[h * 16 + 1];
+      for (int g = 0; g < 4; ++g) {
+        factors[g] = EIGHT ? fmaxf(factor * key_scale[slot * 8 + 2 * c0 + g], 1e-37f) : factor;
+        logs[g] = EIGHT ? value_log[slot * 8 + 2 * c0 + g] : 0.f;
+      }
+      auto largest = [&](const float *x, int g) {          // exponent of 16 keys
+        float r0 = x[0], r1 = x[1];
 #pragma unroll
-          for (int e = h * 16 + 2; e < h * 16 + 14; e += 4) {
-            r0 = fmaxf(r0, fmaxf(x[e], x[e + 1]));         // (one instruction for three)
-            r1 = fmaxf(r1, fmaxf(x[e + 2], x[e + 3]));
-          }
-          m = fmaxf(m, fmaf(fmaxf(fmaxf(r0, r1), fmaxf(x[h * 16 + 14], x[h * 16 + 15])), group_factor(2 * c + h), group_log(2 * c + h)));
+        for (int e = 2; e < 14; e += 4) {
+          r0 = fmaxf(r0, fmaxf(x[e], x[e + 1]));           // (one instruction for three)
+          r1 = fmaxf(r1, fmaxf(x[e + 2], x[e + 3]));
         }
-        return m;
+        return fmaf(fmaxf(fmaxf(r0, r1), fmaxf(x[14], x[15])), factors[g], logs[g]);
       };
-      // Weights of 32 keys: exponents, powers, sums, and the 16-bit operand of the second product, two to a register.  sum: of the weights
-      // as they are, l: without the value scale.
-      auto weigh = [&](float (&x)[32], int c, uint32_t (&w)[16], float &sum, float &l) {
+      const float m = fmaxf(fmaxf(largest(x0, 0), largest(x0 + 16, 1)), fmaxf(largest(x1, 2), largest(x1 + 16, 3)));
+      if (__any_sync(0xffffffffu, m > m_ref + kRaise)) {
+        // The reference is raised, for all rows of the warp (tensor memory is read and written warp-wide), behind the last value product.
+        const float m_new = fmaxf(m_ref, m), alpha = ex2(m_ref - m_new);
+        m_ref = m_new;
+        l_run *= alpha;
+        if (at_half > 0) {
+          if (!all_wait(my_pv_full + 8 * (buf ^ 1), ((at_half - 1) >> 1) & 1, 8)) { alive = false; break; }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t y[16];
+            tc_ld16(t_pv + c * 16, y);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * alpha);
+            tc_st16(t_pv + c * 16, y);
+          }
+          tc_st_wait();
+        }
+      }
+      // Weights: exponents, powers, their sum (without the value scale), and the 16-bit operand of the second product, two to a register.
+      uint32_t w0[16], w1[16];
+      auto weigh = [&](float (&x)[32], int c, uint32_t (&w)[16]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float f = group_factor(2 * c + h), a = group_log(2 * c + h) - (m_ref - kLift);
+          const float f = factors[2 * c + h], a = logs[2 * c + h] - (m_ref - kLift);
           float l0 = 0.f, l1 = 0.f;
 #pragma unroll
           for (int e = h * 16; e < h * 16 + 16; e += 2) {
@@ -417,113 +458,32 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             add2(l0, l1, l0, l1, x[e], x[e + 1]);
             w[e / 2] = pack2<M>(x[e], x[e + 1]);
           }
-          sum += l0 + l1;
-          l = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * c + h], l) : sum;
+          l_run = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * (c0 + c) + h], l_run) : l_run + (l0 + l1);
         }
       };
-      auto put = [&](int c, const uint32_t (&w)[16]) {     // swizzled rows of 128 bytes
-        uint8_t *dst = p_row + (c >> 1) * (kRows * 128);
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<uint4 *>(dst + ((((c & 1) * 4 + g) ^ (row & 7)) << 4)) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
-      };
-      // Before P is overwritten the previous tile's value product, which reads it, must be complete.
-      auto before_put = [&]() { return j == first_tile || all_wait(my_pv_full, (j - 1 - first_tile) & 1, 8); };
-      auto release = [&]() {                               // S has been read
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) bar_arrive(my_s_free);
-      };
-      // One pass, with the reference as it is, with or without hidden keys: where the first half's weights add up to no more than 2^8,
-      // none of them is above that, and of the second half the maximum is taken.  Otherwise the tile is done again below.
-      enum { kOut, kDone, kAgain };
-      auto pass = [&](auto plain) -> int {
-        constexpr bool kPlain = decltype(plain)::value;
-        float x0[32], x1[32], sum = 0.f, l = 0.f;
-        uint32_t w0[16], w1[16];
-        tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
-        tc_ld32_issue(t_s + 32, reinterpret_cast<uint32_t *>(x1));
-        tc_ld_wait_for(x0, x1);
-        if (!kPlain) hide(x0, 0);
-        weigh(x0, 0, w0, sum, l);
-        tc_ld32_issue(t_s + 64, reinterpret_cast<uint32_t *>(x0));
-        if (!kPlain) hide(x1, 1);
-        weigh(x1, 1, w1, sum, l);
-        tc_ld32_issue(t_s + 96, reinterpret_cast<uint32_t *>(x1));
-        tc_ld_wait_for(x0, x1);
-        if (!kPlain) hide(x0, 2);
-        if (!kPlain) hide(x1, 3);
-        if (!__all_sync(0xffffffffu, !there || (sum <= kMostSum * (1 << (int)kLift) && fmaxf(largest(x0, 2), largest(x1, 3)) <= m_ref + kRaise))) return kAgain;
-        release();
-        if (!before_put()) return kOut;
-        put(0, w0);
-        put(1, w1);
-        weigh(x0, 2, w0, sum, l);
-        put(2, w0);
-        weigh(x1, 3, w1, sum, l);
-        put(3, w1);
-        l_run += l;
-        return kDone;
-      };
-      int how = kAgain;
-      if (j > first_tile) how = whole ? pass(std::true_type{}) : pass(std::false_type{});
-      if (how == kAgain) {
-        // The first tile, and where the reference has to be raised, for all rows of the warp (tensor memory is read and written warp-wide):
-        // a pass for the maximum, one for the weights.
-        float m_new = m_ref;
-#pragma unroll 1
-        for (int c = 0; c < kKeys / 32; ++c) {
-          float x[32];
-          tc_ld32(t_s + c * 32, x);
-          if (!whole) hide(x, c);
-          m_new = fmaxf(m_new, largest(x, c));
-        }
-        how = before_put() ? kDone : kOut;
-        const float alpha = ex2(m_ref - m_new);
-        m_ref = m_new;
-        l_run *= alpha;
-        if (j > first_tile && how == kDone) {
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float x[32];
-            tc_ld32(t_pv + c * 32, x);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[e] *= alpha;
-            tc_st32(t_pv + c * 32, x);
-          }
-          tc_st_wait();
-        }
-        float sum = 0.f, l = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < kKeys / 32; ++c) {
-          float x[32];
-          uint32_t w[16];
-          tc_ld32(t_s + c * 32, x);
-          if (!whole) hide(x, c);
-          weigh(x, c, w, sum, l);
-          put(c, w);
-        }
-        l_run += l;
-        release();
-      }
-      if (how == kOut) { alive = false; break; }
-      // P is complete for this warp's 32 rows (and these are rescaled): make it visible to the tensor core's reads.
+      weigh(x0, 0, w0);
+      weigh(x1, 1, w1);
+      // this buffer's last weights have been used
+      if (at_half >= 2 && !all_wait(my_pv_full + 8 * buf, ((at_half >> 1) - 1) & 1, 9)) { alive = false; break; }
+      tc_fence_after();
+      tc_st16(t_p + buf * (kHalf / 2), w0);
+      tc_st16(t_p + buf * (kHalf / 2) + 16, w1);
+      tc_st_wait();
       tc_fence_before();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) bar_arrive(my_p_full);
+      if (lane == 0) bar_arrive(my_p_full + 8 * buf);      // P is complete for this warp's 32 rows (and these are rescaled)
     }
-    const bool walked = ntiles > 0;
-    if (walked && alive && !all_wait(my_pv_full, (ntiles - 1 - first_tile) & 1, 11)) alive = false;
+    const bool walked = end_half > first_half;
+    const int last = end_half - 1 - first_half;
+    if (walked && alive && !all_wait(my_pv_full + 8 * (last & 1), (last >> 1) & 1, 11)) alive = false;
     if (alive || !walked) {
       tc_fence_after();
       float *part = p.part ? p.part + ((((long long)b * p.kv_heads + hk) * blocks + qb) * p.splits + split) * kCtaRows * (D + 2) + (long long)(t * kRows + row) * (D + 2) : nullptr;
       if (part && there) *reinterpret_cast<float2 *>(part + D) = make_float2(m_ref, l_run);
       const float inv = part ? 1.f : l_run == 0.f ? 0.f : 1.f / l_run;
-      // 16-bit rows go through the memory of P, which the last value product is done with: written by their threads, 16 bytes of 32 rows
+      // 16-bit rows go through the memory of Q, which the last product is done with: written by their threads, 16 bytes of 32 rows
       // at a time, they took 6100 cycles
-      uint8_t *stage = p_ptr + t * kPBytes;
+      uint8_t *stage = q_ptr + t * kQBytes;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float x[32];
@@ -617,8 +577,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       fetch(p.v_pages, vbuf, jmin, v_pages);
       // K runs a tile ahead of V: its stage is released earlier
       auto put_k = [&](int j) -> bool {
-        const int i = j - jmin, st = i & 1;
-        if (i >= 2 && !all_wait(k_empty + 8 * st, ((i >> 1) - 1) & 1, 1)) return false;
+        const int i = j - jmin, st = i % kKStages;
+        if (i >= kKStages && !all_wait(k_empty + 8 * st, (i / kKStages - 1) & 1, 1)) return false;
         scales(j, k_pages);
         store(k_ptr + st * kKBytes, kbuf);
         if (lane == 0) bar_arrive(k_full + 8 * st);
