@@ -2,19 +2,29 @@
 // rows of a sequence that brings more than a few tokens, behind any cached past, 16-bit pages or e4m3 codes.
 //
 // The rows of a CTA are (token, query head of the group) pairs, so that heads which share a key / value head share its
-// tiles too: 256 rows, two row tiles of 128, walk the visible keys 128 at a time,
-//   S  = Q K^T   (128 x 128)     in tensor memory, columns [128 t, +128) for row tile t
-//   O += P V     (128 x D)       columns [256 + 128 t, +D)
-// with V as an N-major operand.  Warp 0 moves 16-bit pages by TMA (one box per page and 64 dimensions, 128-byte swizzle; boxes
-// of 16 and more rows are whole swizzle atoms and stack up to the tile), warp 1 issues the MMAs, warps 2-5 and 6-9
-// are the softmax of the row tiles, a thread per row; their order and the lazily raised reference of a row are those of
-// the dense prompt kernel.  Codes take four more warps instead of TMA: they load a tile's codes into registers while
-// the tile before is used, and store them as fp16 (exact) in the swizzled layout.  Queries of bf16 models then become
+// tiles too: 256 rows, two row tiles of 128, walk the visible keys in tiles of 128, half a tile (64 keys) at a time,
+//   S  = Q K^T   (128 x 64)      in tensor memory, columns [128 t, +64) for row tile t
+//   O += P V     (128 x D)       columns [256 + 128 t, +D); P, 16-bit, two buffers of 32 columns from 128 t + 64 on
+// with V as an N-major operand.  The softmax warps (4-7 and 8-11, a thread per row) take a half's scores into registers and hand
+// their memory back at once, so that the next scores are there when they are done; their weights return to tensor memory as the
+// A operand of the second product, which spares shared memory a write and a read (it is what bounds products of 128 x 128
+// tiles: 128 bytes per cycle) and leaves it to three stages of K and two of V.  Warps 1 and 2 issue the products of a row tile each.
+// The reference m of a row is raised only when a score exceeds it by 2^8, behind the last value product.
+//
+// Warp 0 moves 16-bit pages by TMA (one box per page and 64 dimensions, 128-byte swizzle; boxes of 16 and more rows are whole
+// swizzle atoms and stack up to the tile).  Codes take four more warps (12-15) instead: they load a tile's codes into registers
+// while the tile before is used, and store them as fp16 (exact) in the swizzled layout.  Queries of bf16 models then become
 // fp16 with a power of two per row, which keeps all their bits.  A page's key scale multiplies its scores, and the value
 // scale z enters the exponent, 2^(s + log2 z - m), and leaves the sum again: fp16 weights keep their precision where pages
 // differ in magnitude.  Both are one fused multiply-add per score, as without scales.
 //
-// Bound by the tensor core and, equally, by the special-function unit (a 256 x 128 tile takes 2048 cycles of either).
+// bf16 weights over 16-bit pages are rounded once (2^-8 of a weight, which averages out over keys): in two pieces, as in the
+// few-token kernel, the second product would take twice as long.
+//
+// Bound by the chain scores -> softmax -> weights of a row tile: 2200 cycles per 64 keys and pair of row tiles, of which the special-function unit
+// is busy 1024 and the tensor core 1280 (1000 to 1500 tokens behind 3700 to 7000 cached ones, e4m3, 32 heads on 8: 289 us, 800 TFLOP/s).
+// Tried and not kept: weights through shared memory and scores handed back at half time, 311 us; a part of the powers of two by
+// multiply-adds (1 to 3 of 8): 290 to 300 us; converting with two warps instead of four: twice as long.
 // Few rows behind a long past do not fill the machine: the key tiles are then split over CTAs, whose rows are merged by
 // a second launch.
 //
