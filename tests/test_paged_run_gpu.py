@@ -103,3 +103,97 @@ def test_tables_of_a_wider_table():
     got = paged_attention(q, *pools, part, starts, lengths, most_new)
     assert torch.equal(got, paged_attention(q, *pools, tables, starts, lengths, most_new))
     close(got, *c.attention())
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.float16, 16), (torch.bfloat16, 8)])
+def test_long_sequences_among_many(bits, dtype):
+    """So many sequences that none is split: hundreds of tiles per warp, and one sequence that is long enough to be split all the same."""
+    from energonai_b200.paged import paged_attention
+    past = [4000, 2047, 2100, 9000, 5] + [40 + b for b in range(43)]
+    c = Case([1] * 48, past, 8, 8, 64, 16, dtype, bits, seed=13)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    for window in (0, 3000):
+        got = paged_attention(q, *pools, tables, starts, lengths, most_new, window=window, k_scale=scales[0], v_scale=scales[1])
+        close(got, *c.attention(window=window))
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_replayed_batches_of_prompts_and_steps(bits):
+    """One captured call serves other batches: who brings a prompt, who a token, how long all are."""
+    from energonai_b200.paged import paged_append, paged_attention
+    H, G, D, page, rows, cols = 8, 2, 128, 32, 200, 40
+    first = Case([100, 1, 99], [0, 30, 5], H, G, D, page, torch.float16, bits, seed=31)
+    (q, k, v), pools, scales, (_, starts, lengths, _) = first.device()
+    pages = 100
+    big = [torch.zeros((pages,) + p.shape[1:], dtype=p.dtype, device="cuda") for p in pools]
+    zs = [torch.ones(pages, G, device="cuda") if s is not None else None for s in scales]
+    tables = torch.full((3, cols), -1, dtype=torch.int32, device="cuda")
+    freq = frequencies(64).float().cuda()
+    out = torch.zeros_like(q)
+
+    def call():
+        turned = paged_append(q, k, v, *big, tables, starts, lengths, 150, freq=freq, k_scale=zs[0], v_scale=zs[1])
+        paged_attention(turned, *big, tables, starts, lengths, 150, 1200, k_scale=zs[0], v_scale=zs[1], out=out)
+        return turned
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for seed, (new, past) in enumerate((([100, 1, 99], [0, 30, 5]), ([1, 150, 1], [700, 0, 1000]), ([1, 1, 1], [5, 6, 900]), ([0, 20, 120], [3, 200, 64]))):
+        c = Case(new, past, H, G, D, page, torch.float16, bits, seed=40 + seed, pad_rows=rows - sum(new))
+        (q1, k1, v1), p1, s1, (t1, st, le, _) = c.device()
+        for to, src in ((q, q1), (k, k1), (v, v1), (starts, st), (lengths, le)):
+            to.copy_(src)
+        for to, src in zip(big, p1):
+            to.view(torch.uint8)[:c.pages].copy_(src.view(torch.uint8))
+        for to, src in zip(zs, s1):
+            if src is not None:
+                to[:c.pages].copy_(src)
+        tables.fill_(-1)
+        tables[:, :t1.shape[1]] = t1
+        keep = [t.clone() for t in (*big, *(z for z in zs if z is not None))]
+        out.fill_(7.0)
+        graph.replay()
+        got = out.clone()
+        after = [t.clone() for t in (*big, *(z for z in zs if z is not None))]
+        for t, old in zip((*big, *(z for z in zs if z is not None)), keep):
+            t.copy_(old)
+        out.fill_(7.0)
+        turned = call()
+        assert torch.equal(got, out) and all(torch.equal(a.view(torch.uint8), t.view(torch.uint8)) for a, t in zip(after, (*big, *(z for z in zs if z is not None))))
+        assert bool((got[sum(new):] == 7.0).all())
+        # against the restatement, over the pages and the turned queries that the call left
+        c.q, c.pool, c.scale = turned.cpu(), [b[:c.pages].cpu() for b in big], [z[:c.pages].cpu() if z is not None else None for z in zs]
+        want, tol = c.attention(prompt=16)
+        close(got[:sum(new)], want[:sum(new)], tol[:sum(new)])
+
+
+def test_pools_beyond_32_bit_offsets():
+    """Pages behind 2^31 elements and 2^32 bytes: the same bits as from the front of the pool."""
+    from energonai_b200.paged import paged_append, paged_attention
+    if torch.cuda.get_device_properties(0).total_memory < 40 << 30:
+        pytest.skip("needs 20 GB")
+    for bits, dtype in ((16, torch.float16), (8, torch.bfloat16)):
+        c = Case([1, 90, 2], [300, 40, 9], 8, 8, 128, 128, dtype, bits, seed=51)
+        (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device()
+        per_page = 8 * 128 * 128
+        pages = (1 << (31 if bits == 16 else 32)) // per_page + 16 + c.pages
+        shift = pages - c.pages
+        far = [torch.empty((pages, 8, 128, 128), dtype=p.dtype, device="cuda") for p in pools]
+        zs = [torch.ones((pages, 8), device="cuda") if s is not None else None for s in scales]
+        for to, src in zip(far, pools):
+            to[shift:].view(torch.uint8).copy_(src.view(torch.uint8))
+        for to, src in zip(zs, scales):
+            if src is not None:
+                to[shift:] = src
+        moved = torch.where(tables >= 0, tables + shift, tables)
+        freq = frequencies(64).float().cuda()
+        results = []
+        for p, z, t in ((pools, scales, tables), (far, zs, moved)):
+            turned = paged_append(q, k, v, *p, t, starts, lengths, most_new, freq=freq, k_scale=z[0], v_scale=z[1])
+            results.append(paged_attention(turned, *p, t, starts, lengths, most_new, k_scale=z[0], v_scale=z[1]))
+        assert torch.isfinite(results[0]).all() and torch.equal(*results)
+        assert all(torch.equal(a[shift:].view(torch.uint8), b.view(torch.uint8)) for a, b in zip(far, pools))
+        del far
+        torch.cuda.empty_cache()
