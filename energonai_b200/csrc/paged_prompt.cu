@@ -3,12 +3,12 @@
 //
 // The rows of a CTA are (token, query head of the group) pairs, so that heads which share a key / value head share its
 // tiles too: 256 rows, two row tiles of 128, walk the visible keys in tiles of 128, half a tile (64 keys) at a time,
-//   S  = Q K^T   (128 x 64)      in tensor memory, columns [128 t, +64) for row tile t
-//   O += P V     (128 x D)       columns [256 + 128 t, +D); P, 16-bit, two buffers of 32 columns from 128 t + 64 on
-// with V as an N-major operand.  The softmax warps (4-7 and 8-11, a thread per row) take a half's scores into registers and hand
-// their memory back at once, so that the next scores are there when they are done; their weights return to tensor memory as the
-// A operand of the second product, which spares shared memory a write and a read (it is what bounds products of 128 x 128
-// tiles: 128 bytes per cycle) and leaves it to three stages of K and two of V.  Warps 1 and 2 issue the products of a row tile each.
+//   S  = Q K^T   (128 x 64)      in tensor memory, two buffers of 64 columns from 128 t on for row tile t
+//   O += P V     (128 x D)       columns [256 + 128 t, +D); P, 16-bit, lies over the first 32 columns of its scores
+// with V as an N-major operand.  The softmax warps (4-7 and 8-11, a thread per row) take a half's scores into registers and put its
+// weights in their place, as the A operand of the second product, which spares shared memory a write and a read (it is what
+// bounds products of 128 x 128 tiles: 128 bytes per cycle) and leaves it to three stages of K and two of V.  Warps 1 and 2 issue the
+// products of a row tile each; the scores of half n + 2 follow the value product of half n, so that the softmax finds its next ones ready.
 // The reference m of a row is raised only when a score exceeds it by 2^8, behind the last value product.
 //
 // Warp 0 moves 16-bit pages by TMA (one box per page and 64 dimensions, 128-byte swizzle; boxes of 16 and more rows are whole
@@ -115,8 +115,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
   const uint32_t raw = s32(smem_raw);
   uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const uint32_t bar0 = s32(smem);
-  // per stage of K and V; per row tile; per row tile and buffer of P
-  const uint32_t q_full = bar0, q_raw = bar0 + 8, k_full = bar0 + 16, k_empty = bar0 + 40, v_full = bar0 + 64, v_empty = bar0 + 80, s_full = bar0 + 96, s_free = bar0 + 112,
+  // per stage of K and V; per row tile and buffer of scores and weights
+  const uint32_t q_full = bar0, q_raw = bar0 + 8, k_full = bar0 + 16, k_empty = bar0 + 40, v_full = bar0 + 64, v_empty = bar0 + 80, s_full = bar0 + 96,
                  p_full = bar0 + 128, pv_full = bar0 + 160;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + 256);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + 264);
@@ -177,11 +177,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       bar_init(v_full + 8 * s, EIGHT ? kConvertWarps : 1);
       bar_init(v_empty + 8 * s, kRowTiles);
     }
-    for (int t = 0; t < kRowTiles; ++t) {
-      bar_init(s_full + 8 * t, 1);
-      bar_init(s_free + 8 * t, 4);
-    }
     for (int s = 0; s < 2 * kRowTiles; ++s) {
+      bar_init(s_full + 8 * s, 1);
       bar_init(p_full + 8 * s, 4);
       bar_init(pv_full + 8 * s, 1);
     }
@@ -265,11 +262,11 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     }
   } else if (warp <= kRowTiles) {
     // ---------------- MMA issuers: a warp per row tile ----------------
-    // S(first), then for every half n: S(n + 1), as soon as S(n) is in registers, and O += P(n) V(n), as soon as P(n) is written.  Both warps
-    // hand back every stage, those of tiles that theirs does not walk too, each when it is full (an earlier arrival would count for
-    // the stage's use before).
+    // The scores of the first two halves, then for every half n, as soon as P(n) is written: O += P(n) V(n), and behind that S(n + 2), which takes
+    // P(n)'s place, so that scores are there a whole half before they are needed.  Both warps hand back every stage, those of tiles that
+    // theirs does not walk too, each when it is full (an earlier arrival would count for the stage's use before).
     const int t = warp - 1, first = t == 0 ? hs[0] : hs[1], end = t == 0 ? he[0] : he[1];
-    const uint32_t t_s = tmem + t * kKeys, t_p = t_s + kHalf, t_pv = t_s + kPvCol;
+    const uint32_t t_s = tmem + t * kKeys, t_pv = t_s + kPvCol;
     auto pass = [&](int j) -> bool {                       // a tile that this row tile does not walk
       const int i = j - jmin, ks = i % kKStages, vs = i % kVStages;
       if (!all_wait(k_full + 8 * ks, (i / kKStages) & 1, 3)) return false;
@@ -279,27 +276,26 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       return true;
     };
     auto issue_scores = [&](int n) -> bool {
-      const int i = (n >> 1) - jmin, st = i % kKStages;
+      const int i = (n >> 1) - jmin, st = i % kKStages, buf = (n - first) & 1;
       if (!all_wait(k_full + 8 * st, (i / kKStages) & 1, 3)) return false;
       tc_fence_after();
 #pragma unroll
       for (int kb = 0; kb < kSub; ++kb) {
         const uint64_t a = tc_desc(q_addr + t * kQBytes + kb * kRows * 128), bd = tc_desc(k_addr + st * kKBytes + kb * kKeys * 128 + (n & 1) * kHalf * 128);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tc_mma_warp(t_s, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
+        for (int k = 0; k < 4; ++k) tc_mma_warp(t_s + buf * kHalf, a + 2 * k, bd + 2 * k, kIdescS, (kb > 0 || k > 0) ? 1u : 0u);
       }
-      tc_commit_warp(s_full + 8 * t);
+      tc_commit_warp(s_full + 8 * (2 * t + buf));
       if ((n & 1) || n + 1 == end) tc_commit_warp(k_empty + 8 * st);
       return true;
     };
     bool ok = true;
     if (end > first) {
       for (int j = jmin; j < first / 2 && ok; ++j) ok = pass(j);
-      ok = ok && all_wait(q_full, 0, 2) && issue_scores(first);
+      ok = ok && all_wait(q_full, 0, 2) && issue_scores(first) && (first + 1 == end || issue_scores(first + 1));
       for (int n = first; n < end && ok; ++n) {
         const int at = n - first, buf = at & 1, j = n >> 1, i = j - jmin, vs = i % kVStages;
-        if (n + 1 < end) ok = all_wait(s_free + 8 * t, at & 1, 4) && issue_scores(n + 1);
-        ok = ok && all_wait(p_full + 8 * (2 * t + buf), (at >> 1) & 1, 5) && all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10);
+        ok = all_wait(p_full + 8 * (2 * t + buf), (at >> 1) & 1, 5) && all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10);
         if (!ok) break;
         if (!EIGHT && ((n & 1) == 0 || n == first) && (j * kKeys < lo || (j + 1) * kKeys > hi)) {
           // value rows that no row sees may hold anything, and a weight of 0 does not make them 0 (both warps may write these zeros)
@@ -315,10 +311,12 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         for (int k = 0; k < 4; ++k) {
           // 16 keys per instruction: two 8-row groups (2048 bytes) down the V tile, eight columns of P
           const uint64_t bd = tc_desc_nmajor(v_addr + vs * kKBytes + ((n & 1) * 4 + k) * 2048, kKeys * 128);
-          tc_mma_ts_warp(t_pv, t_p + buf * (kHalf / 2) + k * 8, bd, kIdescPV, (at > 0 || k > 0) ? 1u : 0u);
+          tc_mma_ts_warp(t_pv, t_s + buf * kHalf + k * 8, bd, kIdescPV, (at > 0 || k > 0) ? 1u : 0u);
         }
         tc_commit_warp(pv_full + 8 * (2 * t + buf));
         if ((n & 1) || n + 1 == end) tc_commit_warp(v_empty + 8 * vs);
+        // (products on different accumulators are ordered by nothing but their completion)
+        if (n + 2 < end) ok = all_wait(pv_full + 8 * (2 * t + buf), (at >> 1) & 1, 4) && issue_scores(n + 2);
       }
     }
     for (int j = max((end + 1) / 2, jmin); j < nmax && ok; ++j) ok = pass(j);
@@ -330,8 +328,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool there = at < all;
     const int token = at / p.group, head = hk * p.group + at % p.group;
     const int end_half = t == 0 ? he[0] : he[1], first_half = t == 0 ? hs[0] : hs[1];
-    const uint32_t t_s = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_p = t_s + kHalf, t_pv = t_s + kPvCol;
-    const uint32_t my_s_full = s_full + 8 * t, my_p_full = p_full + 16 * t, my_pv_full = pv_full + 16 * t, my_s_free = s_free + 8 * t;
+    const uint32_t t_row = tmem + ((uint32_t)(quarter * 32) << 16) + t * kKeys, t_pv = t_row + kPvCol;
+    const uint32_t my_s_full = s_full + 16 * t, my_p_full = p_full + 16 * t, my_pv_full = pv_full + 16 * t;
     float factor = p.scale_log2;                          // exponent of a score
     bool alive = true;
     {
@@ -390,7 +388,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     float m_ref = kNone, l_run = 0.f;
     for (int n = first_half; n < end_half && alive; ++n) {
       const int at_half = n - first_half, buf = at_half & 1, key0 = n * kHalf, slot = ((n >> 1) - jmin) & (kScaleRing - 1), c0 = (n & 1) * 2;      // (c0: the half's first chunk of 32 keys in its tile)
-      if (!all_wait(my_s_full, at_half & 1, 7)) { alive = false; break; }
+      const uint32_t t_s = t_row + buf * kHalf;            // scores of the half, and its weights in the first 32 columns
+      if (!all_wait(my_s_full + 8 * buf, (at_half >> 1) & 1, 7)) { alive = false; break; }
       tc_fence_after();
       float x0[32], x1[32];
       tc_ld32_issue(t_s, reinterpret_cast<uint32_t *>(x0));
@@ -400,9 +399,6 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       // most halves of a long prompt: every row sees every key
       const bool whole = __all_sync(0xffffffffu, !there || (key0 >= vis_begin && key0 + kHalf <= vis_end)) && !gone;
       tc_ld_wait_for(x0, x1);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(my_s_free);                // (the scores are in registers: the next ones may come)
       // Which of 32 keys this row sees.  (Rows behind the sequence's last count as seeing all, which leaves it to the others.)
       auto hide = [&](float (&x)[32], int c) {
         const int end = vis_end - (key0 + c * 32), begin = vis_begin - (key0 + c * 32);
@@ -473,11 +469,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       };
       weigh(x0, 0, w0);
       weigh(x1, 1, w1);
-      // this buffer's last weights have been used
-      if (at_half >= 2 && !all_wait(my_pv_full + 8 * buf, ((at_half >> 1) - 1) & 1, 9)) { alive = false; break; }
-      tc_fence_after();
-      tc_st16(t_p + buf * (kHalf / 2), w0);
-      tc_st16(t_p + buf * (kHalf / 2) + 16, w1);
+      tc_st16(t_s, w0);                                    // (over scores of this warp's own rows, which are in registers)
+      tc_st16(t_s + 16, w1);
       tc_st_wait();
       tc_fence_before();
       __syncwarp();
