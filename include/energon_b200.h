@@ -910,7 +910,8 @@ typedef struct eb_paged {
  * scales: a page's scale is the smallest power of two (2^-100 at least) with which the largest finite magnitude fits
  * 448, or the one that it had if that is larger and the page holds earlier positions of the sequence, whose codes are then
  * rounded to the new scale; infinities and NaN become NaN.  Slots in front of and behind the new rows, other pages and rows
- * of q_out behind the last sequence are left as they were.  A page that this call writes belongs to one sequence. */
+ * of q_out behind the last sequence are left as they were, and so is what a sequence brings beyond most_new rows.  A page
+ * that this call writes belongs to one sequence. */
 EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, const void *k, long long ldk, const void *v, long long ldv, void *q_out,
                     long long ldo, int rows, int heads, const float *freq, int pairs, void *stream);
 

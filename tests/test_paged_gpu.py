@@ -67,6 +67,25 @@ def test_append_takes_columns_of_a_projection_and_leaves_other_rows():
     assert torch.equal(proj[:, 256:], before[:, 256:]) and torch.equal(proj[5:], before[5:])
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("most_new", [1, 3, 16, 17])
+def test_append_leaves_out_rows_behind_the_announced_ones(most_new, bits):
+    """A sequence that brings more rows than announced loses the others, and no memory is touched for them."""
+    from energonai_b200.paged import paged_append
+    c = Case([40, 2], [0, 5], 4, 2, 128, 16, F16, bits, seed=4)
+    (q, k, v), pools, scales, (tables, starts, lengths, _) = c.device()
+    before = [p.clone() for p in pools]
+    freq = frequencies(64).float().cuda()
+    got = paged_append(q, k, v, *pools, tables, starts, lengths, most_new, freq=freq, k_scale=scales[0], v_scale=scales[1], q_out=torch.full_like(q, 7.0))
+    whole, fresh = before, [None if x is None else x.clone() for x in c.device()[2]]
+    want = paged_append(q, k, v, *whole, tables, starts, lengths, 40, freq=freq, k_scale=fresh[0], v_scale=fresh[1])
+    n = min(most_new, 40)
+    assert torch.equal(got[:n], want[:n]) and bool((got[n:40] == 7.0).all()) and torch.equal(got[40:40 + min(n, 2)], want[40:40 + min(n, 2)])
+    last = c.pool[0][c.tables[0][2]].view(torch.uint8 if bits == 8 else torch.int16)                  # (rows 32 .. 39: announced by none of these)
+    have = pools[0][c.tables[0][2]].view(last.dtype).cpu()
+    assert torch.equal(have, last)
+
+
 def test_append_far_positions():
     """The angle is taken in 64 bits: at position 2 million a 32-bit one would be off by 0.1."""
     from energonai_b200.paged import paged_append
