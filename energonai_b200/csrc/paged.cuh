@@ -18,6 +18,9 @@ struct PagedBatch {
 
 namespace {
 
+// Value scales below 2^-100, 0 among them, count as 2^-100: 1 / scale and log2(scale) enter the softmax.
+constexpr float kLeastScale = 7.888609052210118e-31f;
+
 struct PagedRows {
   int row0, count, past, length;       // first row, rows, positions in front of them, positions in all
 };

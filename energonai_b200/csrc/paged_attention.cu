@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
     if (i0 + lane < mine) x.id = paged_page(p.batch, b, (lo + (warp + (i0 + lane) * kStepWarps) * 16) >> p.batch.page_shift);
     if (EIGHT && x.id >= 0) {
       x.ks = p.k_scale[(long long)x.id * p.kv_heads + hk];
-      x.vs = p.v_scale[(long long)x.id * p.kv_heads + hk];
+      x.vs = fmaxf(p.v_scale[(long long)x.id * p.kv_heads + hk], kLeastScale);
     }
     return x;
   };
@@ -302,16 +302,15 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
       for (int h = 0; h < 2; ++h) {
         const float w0 = pow2(s[n][2 * h] - (m_ref[n][0] - kLift)), w1 = pow2(s[n][2 * h + 1] - (m_ref[n][1] - kLift));
         const uint32_t w = pack2<M>(w0, w1);
-        const float2 rounded = unpack2<M>(w);
         pf[n][h] = transposed(w);
         if constexpr (kSplitP) {
+          const float2 rounded = unpack2<M>(w);
           pl[n][h] = transposed(pack2<M>(w0 - rounded.x, w1 - rounded.y));
-          l_run[n][0] += w0;
-          l_run[n][1] += w1;
-        } else {
-          l_run[n][0] = fmaf(rounded.x, v_inv, l_run[n][0]);
-          l_run[n][1] = fmaf(rounded.y, v_inv, l_run[n][1]);
         }
+        // (in fp32: weights of a page whose values are far smaller than another's fall below fp16, where they add nothing to the
+        // values, but they count in the sum)
+        l_run[n][0] = fmaf(w0, v_inv, l_run[n][0]);
+        l_run[n][1] = fmaf(w1, v_inv, l_run[n][1]);
       }
     // ---- O^T += V^T P^T: value rows 2c, 2c + 1, 2c + 8, 2c + 9, dimensions by g ----
     const bool edge = key0 + 16 > hi || key0 < t.lo;

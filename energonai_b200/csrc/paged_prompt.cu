@@ -568,7 +568,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (lane < kGroups) {
         const int at = ((j - jmin) & (kScaleRing - 1)) * 8 + w * kGroups + lane;
         const long long block = (long long)page * p.kv_heads + hk;
-        const float z = page >= 0 ? p.v_scale[block] : 0.f;
+        const float z = page >= 0 ? fmaxf(p.v_scale[block], kLeastScale) : 0.f;
         key_scale[at] = page >= 0 ? p.k_scale[block] : 1.f;
         value_log[at] = page >= 0 ? __log2f(z) : -INFINITY;
         value_inv[at] = page >= 0 ? 1.f / z : 0.f;

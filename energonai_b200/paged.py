@@ -3,7 +3,7 @@
 Many sequences at once, each with a length of its own.  A packed batch: rows starts[b] to starts[b + 1] - 1 of the
 activations are the new tokens of sequence b, lengths[b] counts its positions in the cache with them, and position p lies
 in slot p mod page_size of page tables[b, p // page_size].  Pools are [pages, kv_heads, page_size, head_dim], in the
-activations' type or torch.float8_e4m3fn with fp32 scales [pages, kv_heads] (value = code * scale).  starts, lengths and
+activations' type or torch.float8_e4m3fn with fp32 scales [pages, kv_heads] (value = code * scale, scales not negative).  starts, lengths and
 tables are int32 on the device; a captured call may be replayed with other contents, within most_new new tokens per
 sequence and most_length positions."""
 import functools

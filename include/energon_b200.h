@@ -891,7 +891,7 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
 
 /* Many sequences at once, each with a length of its own, keys and values in pages of page_size (16, 32, 64 or 128)
  * positions: pools [pages][kv_heads][page_size][head_dim], in `dtype` (fp16 or bf16) or, with scales [pages][kv_heads],
- * as e4m3 codes (value = code * scale).  Rows starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the
+ * as e4m3 codes (value = code * scale; scales are not negative, value scales below 2^-100 count as 2^-100).  Rows starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the
  * new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, at most most_length, so that row i
  * of n_b has position lengths[b] - n_b + i.  Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
  * starts, lengths and tables live on the device and may change between replays of a captured call.  Pages that are none

@@ -208,6 +208,22 @@ def test_pages_of_very_different_scales():
     close(got, *c.attention(scale=1.0))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("least", [2.0 ** -100, 2.0 ** -40, 0.0])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (2, 2, 128, 32), (24, 1, 128, 16)])
+def test_pages_of_tiny_values_keep_their_share_of_the_weights(heads, kv_heads, dim, page, least, dtype):
+    """Every fifth page has values far smaller than the others' (or none): its keys take their weights from the others all the same."""
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 70, 5, 2], [31, 0, 200, 9], heads, kv_heads, dim, page, dtype, 8, seed=heads)
+    for page in [p for t in c.tables for p in t[::5]]:
+        c.scale[1][page] = least
+        if least < 2.0 ** -40:
+            codes = c.pool[1][page].view(torch.uint8)
+            codes[codes != 0x7f] = 0
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    close(paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), *c.attention())
+
+
 def test_rows_without_keys_and_rows_behind_the_last_sequence():
     from energonai_b200.paged import paged_attention
     c = Case([1, 2], [40, 5], 4, 4, 64, 16, F16, 16, seed=2, pad_rows=4)
