@@ -46,6 +46,14 @@ template <typename T> __device__ __forceinline__ void two_pieces(float x, float 
   lo = pack2<T>(x - f.x, y - f.y);
 }
 
+// fp16 pieces: the power of two that brings the largest magnitude m of a low-rank row to [2^14, 2^15), so that the row keeps its
+// 22 bits whatever its size (2^-100 to 2^100); the products are divided by it in fp32.  bf16 has fp32's range.
+template <typename T> __device__ __forceinline__ int lift_of(float m) {
+  return std::is_same<T, __half>::value ? min(max(14 - ((__float_as_int(m) >> 23) - 127), -100), 100) : 0;
+}
+__device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ float largest_of(const float4 &v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
+
 // Rows and adapter of sequence b; b = batch: the rows behind the last sequence, without one.
 struct AdapterRows {
   int row0, count, adapter;
@@ -186,6 +194,12 @@ template <typename T, int RT> __global__ void __launch_bounds__(kAdapterWarps * 
   }
 }
 
+// eight columns of row g (from = 0) or g + 8 (2)
+template <typename T> __device__ __forceinline__ uint4 packed_row(const float (&acc)[4][4], int from, float down) {
+  return make_uint4(pack2<T>(acc[0][from] * down, acc[0][from + 1] * down), pack2<T>(acc[1][from] * down, acc[1][from + 1] * down),
+                    pack2<T>(acc[2][from] * down, acc[2][from + 1] * down), pack2<T>(acc[3][from] * down, acc[3][from + 1] * down));
+}
+
 // delta[row][n] = s sum_r low[row][r] B[n][r], 16 rows of a sequence, the warps take turns over the columns.  KR: steps of 16 ranks.
 template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_delta_kernel(const AdapterParams p) {
   griddep_wait();
@@ -222,6 +236,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
     const float s = p.scales[r.adapter];
     // low-rank rows g and g + 8, ranks 16 k + 4 c .. + 3: two pieces each
     uint32_t hi[KR][4], lo[KR][4];
+    float down[2];
     {
       float4 v[KR][2] = {};
 #pragma unroll 4
@@ -235,12 +250,24 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
               v[k][h] = make_float4(v[k][h].x + one.x, v[k][h].y + one.y, v[k][h].z + one.z, v[k][h].w + one.w);
             }
 #pragma unroll
-      for (int k = 0; k < KR; ++k)
+      for (int h = 0; h < 2; ++h) {
+        float m = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          two_pieces<T>(v[k][h].x * s, v[k][h].y * s, hi[k][h], lo[k][h]);
-          two_pieces<T>(v[k][h].z * s, v[k][h].w * s, hi[k][h + 2], lo[k][h + 2]);
+        for (int k = 0; k < KR; ++k) {
+          v[k][h] = make_float4(v[k][h].x * s, v[k][h].y * s, v[k][h].z * s, v[k][h].w * s);
+          m = fmaxf(m, largest_of(v[k][h]));
         }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = lift_of<T>(m);
+        const float up = pow2_of(e);
+        down[h] = pow2_of(-e);
+#pragma unroll
+        for (int k = 0; k < KR; ++k) {
+          two_pieces<T>(v[k][h].x * up, v[k][h].y * up, hi[k][h], lo[k][h]);
+          two_pieces<T>(v[k][h].z * up, v[k][h].w * up, hi[k][h + 2], lo[k][h + 2]);
+        }
+      }
     }
     for (int n0 = first; n0 < end; n0 += step) {
       float acc[4][4];
@@ -256,9 +283,9 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
       fetch(n0 + step);                                    // (the next columns, while these are stored)
       if (n0 + c * 8 < end) {
         if (g < rows)
-          *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(pack2<T>(acc[0][0], acc[0][1]), pack2<T>(acc[1][0], acc[1][1]), pack2<T>(acc[2][0], acc[2][1]), pack2<T>(acc[3][0], acc[3][1]));
+          *reinterpret_cast<uint4 *>(out0 + n0) = packed_row<T>(acc, 0, down[0]);
         if (g + 8 < rows)
-          *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(pack2<T>(acc[0][2], acc[0][3]), pack2<T>(acc[1][2], acc[1][3]), pack2<T>(acc[2][2], acc[2][3]), pack2<T>(acc[3][2], acc[3][3]));
+          *reinterpret_cast<uint4 *>(out1 + n0) = packed_row<T>(acc, 2, down[1]);
       }
     }
   }
@@ -314,6 +341,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
     constexpr int kPieces = kLowRows * kRowBytes;
     const uint32_t at_hi = base + kDeltaStages * kStage, at_lo = at_hi + kPieces;
     uint8_t *pieces = delta_smem + kDeltaStages * kStage;
+    float *downs = reinterpret_cast<float *>(pieces + 2 * kPieces);
     const int all = min(kLowRows, r.count - t0), quads = p.rank / 4;
     for (int e = threadIdx.x; e < kLowRows * KR * 4; e += kAdapterWarps * 32) {
       const int row = e / (KR * 4), quad = e % (KR * 4);
@@ -326,9 +354,16 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
           v = make_float4(v.x + one.x, v.y + one.y, v.z + one.z, v.w + one.w);
         }
       }
+      v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
+      float m = largest_of(v);                             // (a row's quads are in lanes that follow one another)
+#pragma unroll
+      for (int o = 1; o < KR * 4; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const int lift = lift_of<T>(m);
+      const float up = pow2_of(lift);
+      if (quad == 0) downs[row] = pow2_of(-lift);
       uint2 hi2, lo2;
-      two_pieces<T>(v.x * s, v.y * s, hi2.x, lo2.x);
-      two_pieces<T>(v.z * s, v.w * s, hi2.y, lo2.y);
+      two_pieces<T>(v.x * up, v.y * up, hi2.x, lo2.x);
+      two_pieces<T>(v.z * up, v.w * up, hi2.y, lo2.y);
       const int to = row * kRowBytes + swizzled(row & 7, quad >> 1) * 16 + (quad & 1) * 8;
       *reinterpret_cast<uint2 *>(pieces + to) = hi2;
       *reinterpret_cast<uint2 *>(pieces + kPieces + to) = lo2;
@@ -341,6 +376,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
       ldmatrix_x4(hi[k], at_hi + to);
       ldmatrix_x4(lo[k], at_lo + to);
     }
+    const float down[2] = {downs[warp * kRowTile + g], downs[warp * kRowTile + g + 8]};
     for (int i = 0; i < steps; ++i) {
       cp_async_wait<kDeltaStages - 2>();
       __syncthreads();
@@ -373,9 +409,9 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
         const int n = begin + i * kDeltaCols + n0;
         if (n + c * 8 < end) {
           if (g < rows)
-            *reinterpret_cast<uint4 *>(out0 + n) = make_uint4(pack2<T>(acc[0][0], acc[0][1]), pack2<T>(acc[1][0], acc[1][1]), pack2<T>(acc[2][0], acc[2][1]), pack2<T>(acc[3][0], acc[3][1]));
+            *reinterpret_cast<uint4 *>(out0 + n) = packed_row<T>(acc, 0, down[0]);
           if (g + 8 < rows)
-            *reinterpret_cast<uint4 *>(out1 + n) = make_uint4(pack2<T>(acc[0][2], acc[0][3]), pack2<T>(acc[1][2], acc[1][3]), pack2<T>(acc[2][2], acc[2][3]), pack2<T>(acc[3][2], acc[3][3]));
+            *reinterpret_cast<uint4 *>(out1 + n) = packed_row<T>(acc, 2, down[1]);
         }
       }
     }
@@ -429,7 +465,7 @@ template <typename T, int KR> int launch_delta(AdapterParams p, const AdapterPla
     launch_pdl(adapter_delta_kernel<T, KR>, grid, block, 0, st, p);
     return EB_OK;
   }
-  constexpr int kSmem = (kDeltaStages * kDeltaCols + 2 * kLowRows) * 32 * KR;
+  constexpr int kSmem = (kDeltaStages * kDeltaCols + 2 * kLowRows) * 32 * KR + kLowRows * (int)sizeof(float);
   auto kern = adapter_delta_many_kernel<T, KR>;
   if (kSmem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) {
     cudaGetLastError();

@@ -64,6 +64,17 @@ def test_delta_and_product(new, width, columns, rank, adapters, dtype):
     close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * width / 16 + 2.0 ** -20) * size)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("x,a,b", [(2.0 ** 9, 2.0 ** 6, 2.0 ** -6), (2.0 ** -8, 2.0 ** -6, 2.0 ** 6)])
+@pytest.mark.parametrize("new,rank", [([1, 3, 16], 8), ([5, 9], 40), ([70, 1], 16), ([33], 24), ([40, 100], 64), ([64], 120)])
+def test_low_rank_rows_beyond_half_precision(new, rank, x, a, b, dtype):
+    """The low-rank row itself may be larger or smaller than fp16 can say; the result is not."""
+    from energonai_b200.adapter import adapter_delta
+    c = Case(new, 512, 264, rank, 2, dtype, seed=rank, pad_rows=2)
+    c.x, c.a, c.b = c.x * x, c.a * a, c.b * b
+    close(adapter_delta(c.x.cuda(), *c.device()), *c.delta())
+
+
 def test_many_rows_behind_the_last_sequence():
     from energonai_b200.adapter import adapter_delta
     c = Case([1, 2], 64, 96, 8, 2, F16, seed=3, pad_rows=500)
