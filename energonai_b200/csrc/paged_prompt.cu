@@ -128,7 +128,9 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   griddep_wait();
-  const int blocks = gridDim.x / p.splits, split = blockIdx.x % p.splits, qb = blocks - 1 - blockIdx.x / p.splits, hk = blockIdx.y, b = blockIdx.z;    // the latest rows, which see most, first
+  // of a sequence the latest rows, which see most, of all heads first: its earliest, with few keys, fill up the end
+  const int blocks = gridDim.x / p.splits, id = blockIdx.y * gridDim.x + blockIdx.x, hk = id % p.kv_heads, of_head = id / p.kv_heads,
+            split = of_head % p.splits, qb = blocks - 1 - of_head / p.splits, b = blockIdx.z;
   const PagedRows r = paged_rows(p.batch, b);
   const int all = r.count * p.group, q0 = qb * kCtaRows, reach = p.batch.table_cols << p.batch.page_shift;
   if (all <= p.few || q0 >= all) return;
