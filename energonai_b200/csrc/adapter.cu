@@ -212,7 +212,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
   for (int t0 = blockIdx.x * kRowTile; t0 < r.count; t0 += gridDim.x * kRowTile) {
     const int rows = min(kRowTile, r.count - t0), row0 = r.row0 + t0;
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
-    if (r.adapter < 0) {
+    if (r.adapter < 0 || t0 >= (int)gridDim.x * kRowTile) {       // (rows that were not announced have no low-rank row)
       for (int n0 = first; n0 < end; n0 += step)
         if (n0 + c * 8 < end) {
           if (g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
@@ -311,7 +311,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
   for (int t0 = blockIdx.x * kLowRows; t0 < r.count; t0 += gridDim.x * kLowRows) {
     const int rows = min(kRowTile, r.count - t0 - warp * kRowTile), row0 = r.row0 + t0 + warp * kRowTile;      // (of this warp; none: <= 0)
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
-    if (r.adapter < 0) {
+    if (r.adapter < 0 || t0 >= (int)gridDim.x * kLowRows) {       // (rows that were not announced have no low-rank row)
       for (int n0 = begin; n0 < end; n0 += 32)
         if (n0 + c * 8 < end) {
           if (g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);

@@ -83,6 +83,19 @@ def test_many_rows_behind_the_last_sequence():
     assert not delta[3:].any()
 
 
+@pytest.mark.parametrize("most_new", [16, 64])
+def test_rows_that_were_not_announced_get_nothing(most_new):
+    from energonai_b200.adapter import adapter_delta
+    c = Case([200, 3], 64, 96, 8, 2, BF16, seed=6)
+    c.index[:] = 1
+    want, tol = c.delta()
+    c.most_new = most_new
+    got = adapter_delta(c.x.cuda(), *c.device())
+    assert not got[most_new:200].any()
+    want[most_new:200] = 0
+    close(got, want, tol)
+
+
 def test_other_indices_are_none():
     from energonai_b200.adapter import adapter_delta
     c = Case([2, 3, 1], 64, 96, 8, 2, BF16, seed=4)
