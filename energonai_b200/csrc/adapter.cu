@@ -336,37 +336,47 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
     __syncthreads();                                       // (the stages of the rows before are done with)
     for (int i = 0; i < kDeltaStages - 1; ++i) fetch(i);
     const float s = p.scales[r.adapter];
-    // The low-rank rows, summed over the splits in order by whoever comes across 4 ranks of a row, then as two pieces each through shared
-    // memory to the fragments.  (Each lane gathering its own fragments took 10 us.)
+    // The low-rank rows, summed over the splits in order, 4 ranks of a row at a time, then as two pieces each through shared memory to the
+    // fragments.  A split's loads go together, kPer of a thread, so that the CTA waits for splits and not for rows of splits.
     constexpr int kPieces = kLowRows * kRowBytes;
     const uint32_t at_hi = base + kDeltaStages * kStage, at_lo = at_hi + kPieces;
     uint8_t *pieces = delta_smem + kDeltaStages * kStage;
     float *downs = reinterpret_cast<float *>(pieces + 2 * kPieces);
     const int all = min(kLowRows, r.count - t0), quads = p.rank / 4;
-    for (int e = threadIdx.x; e < kLowRows * KR * 4; e += kAdapterWarps * 32) {
-      const int row = e / (KR * 4), quad = e % (KR * 4);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row < all && quad < quads) {
-        const float4 *from = reinterpret_cast<const float4 *>(p.low + ((long long)r.row0 + t0 + row) * p.rank) + quad;
-#pragma unroll 4
-        for (int q = 0; q < p.splits; ++q) {
-          const float4 one = from[(long long)q * p.rows * quads];
-          v = make_float4(v.x + one.x, v.y + one.y, v.z + one.z, v.w + one.w);
+    constexpr int kPer = 8 < 2 * KR ? 8 : 2 * KR;
+    for (int e0 = threadIdx.x; e0 < kLowRows * KR * 4; e0 += kPer * kAdapterWarps * 32) {
+      float4 v[kPer];
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+      for (int q = 0; q < p.splits; ++q) {
+        const float4 *from = reinterpret_cast<const float4 *>(p.low + ((long long)q * p.rows + r.row0 + t0) * p.rank);
+#pragma unroll
+        for (int u = 0; u < kPer; ++u) {
+          const int e = e0 + u * kAdapterWarps * 32, row = e / (KR * 4), quad = e % (KR * 4);
+          if (row < all && quad < quads) {
+            const float4 one = from[row * quads + quad];
+            v[u] = make_float4(v[u].x + one.x, v[u].y + one.y, v[u].z + one.z, v[u].w + one.w);
+          }
         }
       }
-      v = make_float4(v.x * s, v.y * s, v.z * s, v.w * s);
-      float m = largest_of(v);                             // (a row's quads are in lanes that follow one another)
 #pragma unroll
-      for (int o = 1; o < KR * 4; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const int lift = lift_of<T>(m);
-      const float up = pow2_of(lift);
-      if (quad == 0) downs[row] = pow2_of(-lift);
-      uint2 hi2, lo2;
-      two_pieces<T>(v.x * up, v.y * up, hi2.x, lo2.x);
-      two_pieces<T>(v.z * up, v.w * up, hi2.y, lo2.y);
-      const int to = row * kRowBytes + swizzled(row & 7, quad >> 1) * 16 + (quad & 1) * 8;
-      *reinterpret_cast<uint2 *>(pieces + to) = hi2;
-      *reinterpret_cast<uint2 *>(pieces + kPieces + to) = lo2;
+      for (int u = 0; u < kPer; ++u) {
+        const int e = e0 + u * kAdapterWarps * 32, row = e / (KR * 4), quad = e % (KR * 4);
+        v[u] = make_float4(v[u].x * s, v[u].y * s, v[u].z * s, v[u].w * s);
+        float m = largest_of(v[u]);                        // (a row's quads are in lanes that follow one another)
+#pragma unroll
+        for (int o = 1; o < KR * 4; o *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int lift = lift_of<T>(m);
+        const float up = pow2_of(lift);
+        if (quad == 0) downs[row] = pow2_of(-lift);
+        uint2 hi2, lo2;
+        two_pieces<T>(v[u].x * up, v[u].y * up, hi2.x, lo2.x);
+        two_pieces<T>(v[u].z * up, v[u].w * up, hi2.y, lo2.y);
+        const int to = row * kRowBytes + swizzled(row & 7, quad >> 1) * 16 + (quad & 1) * 8;
+        *reinterpret_cast<uint2 *>(pieces + to) = hi2;
+        *reinterpret_cast<uint2 *>(pieces + kPieces + to) = lo2;
+      }
     }
     __syncthreads();
     uint32_t hi[KR][4], lo[KR][4];
@@ -429,7 +439,7 @@ AdapterPlan adapter_plan(int batch, int most_new, int width) {
   s.tiles = (most_new + rows - 1) / rows;
   const long long ctas = (long long)s.tiles * batch;
   const int turns = (width + turn - 1) / turn, least = s.many ? 8 : 4;                  // turns of the CTA over its columns, at least
-  int want = (int)(((s.many ? 3ll : 4ll) * sm_count() + ctas - 1) / ctas);
+  int want = (int)((4ll * sm_count() + ctas - 1) / ctas);
   if (want > turns / least) want = turns / least > 0 ? turns / least : 1;
   const int per = (turns + want - 1) / want;
   s.splits = (turns + per - 1) / per;
