@@ -292,7 +292,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
 }
 
 // The same for 64 rows of a sequence, 16 per warp; B comes through shared memory, 128 columns at a time, two steps ahead.  (Loaded to
-// registers by every warp, 8 bytes of eight rows at a time, it kept the first-level cache busy for 48 us where this takes 19:
+// registers by every warp, 8 bytes of eight rows at a time, it kept the first-level cache busy for 48 us where this takes 20:
 // 6144 columns, rank 64, 4000 rows.)  The rows of 32 columns lie in the order in which the tiles use them, so that a tile's
 // eight rows follow one another; their chunks of 16 bytes are XOR-swizzled.
 constexpr int kDeltaCols = 128, kDeltaStages = 3;

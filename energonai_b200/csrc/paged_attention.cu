@@ -18,7 +18,7 @@
 // The reference m of a row is raised only when a score exceeds it by 2^8 (one vote per tile instead of a reduction); fp16
 // weights are 2^6 times as large, up to 2^14, which leaves fewer of them below fp16's normal range.
 // Weights of bf16 caches are split into two bf16 pieces, which costs tensor time that is there and keeps
-// the result within its own rounding; fp16 weights are rounded once and the sum adds up the rounded ones.
+// the result within its own rounding; fp16 weights are rounded once.
 //
 // Keys are split over CTAs by a fixed number of keys per CTA (short sequences then take fewer CTAs), the warps of a
 // CTA take every fourth tile; partial rows are merged in order, across CTAs by a second launch.
@@ -302,15 +302,14 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
       for (int h = 0; h < 2; ++h) {
         const float w0 = pow2(s[n][2 * h] - (m_ref[n][0] - kLift)), w1 = pow2(s[n][2 * h + 1] - (m_ref[n][1] - kLift));
         const uint32_t w = pack2<M>(w0, w1);
+        const float2 rounded = unpack2<M>(w);
         pf[n][h] = transposed(w);
-        if constexpr (kSplitP) {
-          const float2 rounded = unpack2<M>(w);
-          pl[n][h] = transposed(pack2<M>(w0 - rounded.x, w1 - rounded.y));
-        }
-        // (in fp32: weights of a page whose values are far smaller than another's fall below fp16, where they add nothing to the
-        // values, but they count in the sum)
-        l_run[n][0] = fmaf(w0, v_inv, l_run[n][0]);
-        l_run[n][1] = fmaf(w1, v_inv, l_run[n][1]);
+        if constexpr (kSplitP) pl[n][h] = transposed(pack2<M>(w0 - rounded.x, w1 - rounded.y));
+        // fp16 weights of 16-bit pages are summed as they are rounded, which takes a tenth off the error.  Not those of codes: weights of a page
+        // whose values are far smaller than another's fall below fp16, where they add nothing to the values, but they count in the sum.
+        constexpr bool kAsRounded = !EIGHT && !kSplitP;
+        l_run[n][0] = fmaf(kAsRounded ? rounded.x : w0, v_inv, l_run[n][0]);
+        l_run[n][1] = fmaf(kAsRounded ? rounded.y : w1, v_inv, l_run[n][1]);
       }
     // ---- O^T += V^T P^T: value rows 2c, 2c + 1, 2c + 8, 2c + 9, dimensions by g ----
     const bool edge = key0 + 16 > hi || key0 < t.lo;

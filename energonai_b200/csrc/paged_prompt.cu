@@ -22,7 +22,7 @@
 // few-token kernel, the second product would take twice as long.
 //
 // Bound by the chain scores -> softmax -> weights of a row tile: 2100 cycles per 64 keys and pair of row tiles, of which the special-function unit
-// is busy 1024 and the tensor core 1280 (1000 to 1500 tokens behind 3700 to 7000 cached ones, e4m3, 32 heads on 8: 279 us, 830 TFLOP/s).
+// is busy 1024 and the tensor core 1280 (1000 to 1500 tokens behind 3700 to 7000 cached ones, e4m3, 32 heads on 8: 277 us, 830 TFLOP/s).
 // Tried and not kept: weights through shared memory, 311 us; weights in columns of their own, scores handed back before the softmax, 289 us; a part of
 // the powers of two by multiply-adds (1 to 3 of 8), 290 to 300 us; halves that the mask hides skipped one by one, 296 us; two sets of softmax warps that take halves in turn, 415 us; converting with two warps instead
 // of four, twice as long.  Over 16-bit pages of 64 positions the same takes 330 us: twice the bytes through the second-level cache.
