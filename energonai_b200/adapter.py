@@ -19,7 +19,7 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
     """What each row's adapter adds to a projection of x [rows, width]: scales[i] (x a[i].T) b[i].T, [rows, columns], with
     i = index[s] for the rows starts[s] to starts[s + 1] - 1 of sequence s (at most most_new).  a [adapters, rank, width], b
     [adapters, columns, rank], scales fp32 [adapters]; index int32 [batch], negative for none; starts int32 [batch + 1].  rank is
-    a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows behind the last sequence get zeros."""
+    a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows of no sequence get zeros."""
     device = _one_device("adapter_delta", x, a, b, scales, index, starts)
     dtype, shape, of, to = x.dtype, x.shape, a.shape, b.shape
     if len(of) != 3 or len(to) != 3 or len(shape) != 2 or of[0] != to[0] or of[1] != to[2] or of[2] != shape[1]:
@@ -33,7 +33,7 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
     if index.dtype is not torch.int32 or starts.dtype is not torch.int32 or index.dim() != 1 or starts.shape != (batch + 1,) or batch == 0 or not (
             index.is_contiguous() and starts.is_contiguous()):
         raise RuntimeError("adapter_delta: int32 index [batch] and starts [batch + 1] required")
-    rows, columns, most_new = shape[0], to[1], int(most_new)
+    rows, columns, most_new = shape[0], to[1], int(most_new) or 1        # (0: zeros are all that is asked for)
     ldx = _rows("adapter_delta", x, width, dtype)
     delta = x.new_empty((rows, columns))
     nbytes = _scratch_bytes(rows, width, rank, batch, most_new)
@@ -46,7 +46,7 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
 
 def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=None, static_weight=False):
     """x @ w.T + bias for all rows, and beside it each sequence's adapter (adapter_delta), added to the fp32 sums: [rows, columns].
-    Rows behind the last sequence get the shared projection alone."""
+    Rows of no sequence get the shared projection alone."""
     _one_device("adapter_product", w, bias, out)
     if w.dim() != 2 or w.shape != (b.shape[1], x.shape[1]) or w.dtype != x.dtype:
         raise RuntimeError("adapter_product: the shared weight is [columns, width] of the type of x")

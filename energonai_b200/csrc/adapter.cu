@@ -54,14 +54,14 @@ template <typename T> __device__ __forceinline__ int lift_of(float m) {
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float largest_of(const float4 &v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
-// Rows and adapter of sequence b; b = batch: the rows behind the last sequence, without one.
+// Rows and adapter of sequence b; b = batch and batch + 1: the rows behind the last sequence and in front of the first, without one.
 struct AdapterRows {
   int row0, count, adapter;
 };
 __device__ __forceinline__ AdapterRows adapter_rows(const AdapterParams &p, int b) {
   AdapterRows r;
-  r.row0 = min(max(p.starts[b], 0), p.rows);
-  r.count = (b < p.batch ? min(p.starts[b + 1], p.rows) : p.rows) - r.row0;
+  r.row0 = b > p.batch ? 0 : min(max(p.starts[b], 0), p.rows);
+  r.count = (b == p.batch ? p.rows : min(p.starts[b > p.batch ? 0 : b + 1], p.rows)) - r.row0;
   r.adapter = b < p.batch ? p.index[b] : -1;
   if (r.adapter >= p.count) r.adapter = -1;
   return r;
@@ -470,7 +470,7 @@ template <typename T, int KR> int launch_delta(AdapterParams p, const AdapterPla
   const int parts = (int)(want < turns ? want : turns);
   p.chunk = (turns + parts - 1) / parts * kDeltaCols;
   static_assert(kDeltaCols == kAdapterWarps * 32, "a turn of either form");
-  const dim3 grid(s.tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch + 1), block(kAdapterWarps * 32);
+  const dim3 grid(s.tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch + 2), block(kAdapterWarps * 32);
   if (!s.many) {
     launch_pdl(adapter_delta_kernel<T, KR>, grid, block, 0, st, p);
     return EB_OK;
@@ -509,7 +509,7 @@ extern "C" int eb_adapter_delta(const void *x, long long ldx, const void *a, con
   if (rows == 0 || columns == 0) return EB_OK;
   EB_REQUIRE(dtype == EB_F16 || dtype == EB_BF16, "adapter_delta: fp16 or bf16 only (dtype %d)", dtype);
   EB_REQUIRE(x && a && b && scales && index && starts && delta, "adapter_delta: null pointer");
-  EB_REQUIRE(rows > 0 && width > 0 && columns > 0 && adapters > 0 && batch > 0 && batch < 65535 && most_new > 0, "adapter_delta: bad sizes");
+  EB_REQUIRE(rows > 0 && width > 0 && columns > 0 && adapters > 0 && batch > 0 && batch < 65534 && most_new > 0, "adapter_delta: bad sizes");
   EB_REQUIRE(rank >= 8 && rank <= 128 && rank % 8 == 0, "adapter_delta: rank %d not supported (multiples of 8 up to 128; fill up with zeros)", rank);
   EB_REQUIRE(width % 8 == 0 && columns % 8 == 0 && ldx % 8 == 0 && ldd % 8 == 0 && ldx >= width && ldd >= columns,
              "adapter_delta: widths and strides must be multiples of 8 elements that hold a row");

@@ -121,7 +121,7 @@ def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_sc
     reach = cols * page_size
     most_length = reach if most_length is None else min(int(most_length), reach)
     return kv_heads, head_dim, most_length, _paged.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), ld, pages,
-                                                        page_size, kv_heads, head_dim, cols, batch, int(most_new), most_length, dtype_code(dtype), 0)
+                                                        page_size, kv_heads, head_dim, cols, batch, min(int(most_new), (1 << 31) - 1), most_length, dtype_code(dtype), 0)
 
 
 def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, freq=None, k_scale=None, v_scale=None, q_out=None):
@@ -164,7 +164,7 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     """Causal attention of the new tokens q [rows, heads*head_dim] over their sequences' pages, which hold the new keys and values
     already: single tokens, a few per sequence, prompts and chunks of prompts, or all of them in one batch.  window > 0:
     the row at position p sees the positions above p - window only.  most_length: no sequence is longer (None: what the
-    tables address).  Returns out [rows, heads*head_dim]; rows behind the last sequence are left as they are."""
+    tables address).  Returns out [rows, heads*head_dim]; rows of no sequence are left as they are."""
     device = _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)
     dtype, shape = q.dtype, q.shape
     kv_heads, head_dim, most_length, cache = _cache("paged_attention", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length)

@@ -891,8 +891,8 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
 
 /* Many sequences at once, each with a length of its own, keys and values in pages of page_size (16, 32, 64 or 128)
  * positions: pools [pages][kv_heads][page_size][head_dim], in `dtype` (fp16 or bf16) or, with scales [pages][kv_heads],
- * as e4m3 codes (value = code * scale; scales are not negative, value scales below 2^-100 count as 2^-100).  Rows starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the
- * new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, at most most_length, so that row i
+ * as e4m3 codes (value = code * scale; no scale is negative, value scales below 2^-100 count as 2^-100).  Rows
+ * starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, at most most_length, so that row i
  * of n_b has position lengths[b] - n_b + i.  Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
  * starts, lengths and tables live on the device and may change between replays of a captured call.  Pages that are none
  * (outside of the pool or behind the table's columns) hold nothing: nothing is written to them and nothing read.
@@ -910,13 +910,13 @@ typedef struct eb_paged {
  * scales: a page's scale is the smallest power of two (2^-100 at least) with which the largest finite magnitude fits
  * 448, or the one that it had if that is larger and the page holds earlier positions of the sequence, whose codes are then
  * rounded to the new scale; infinities and NaN become NaN.  Slots in front of and behind the new rows, other pages and rows
- * of q_out behind the last sequence are left as they were, and so is what a sequence brings beyond most_new rows.  A page
+ * of q_out of no sequence are left as they were, and so is what a sequence brings beyond most_new rows.  A page
  * that this call writes belongs to one sequence. */
 EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, const void *k, long long ldk, const void *v, long long ldv, void *q_out,
                     long long ldo, int rows, int heads, const float *freq, int pairs, void *stream);
 
 /* Causal attention of the new tokens over the cache (which holds them already): the row at position p sees the positions
- * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros; rows of `out` behind the last
+ * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros; rows of `out` of no
  * sequence are left as they were.  Slots that no row sees may hold anything.
  * scratch: eb_paged_attention_scratch_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the
  * device need scratch of their own. */
@@ -926,7 +926,7 @@ EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_head
 
 /* Low-rank adapters of many requests: for the rows starts[b] to starts[b + 1] - 1 (at most most_new) of each sequence, with
  * i = index[b],  delta = scales[i] (x a[i]^T) b[i]^T,  a [adapters][rank][width], b [adapters][columns][rank], rank a multiple
- * of 8 up to 128.  An index outside of 0 .. adapters - 1, and rows behind the last sequence: zeros.  delta is what the
+ * of 8 up to 128.  An index outside of 0 .. adapters - 1, and rows of no sequence: zeros.  delta is what the
  * projection beside it adds as its residual.  scratch: eb_adapter_scratch_bytes(...) bytes, 16-byte aligned, of any content.
  * No counterpart in the reference. */
 EB_API int eb_adapter_delta(const void *x, long long ldx, const void *a, const void *b, const float *scales, const int32_t *index,

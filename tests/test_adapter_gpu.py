@@ -96,6 +96,22 @@ def test_rows_that_were_not_announced_get_nothing(most_new):
     close(got, want, tol)
 
 
+@pytest.mark.parametrize("most_new", [6, 40])
+def test_rows_in_front_of_the_first_sequence(most_new):
+    """A part of a batch: the later sequences' starts and adapters alone."""
+    from energonai_b200.adapter import adapter_delta
+    c = Case([30, 5, 6], 64, 96, 8, 2, BF16, seed=7, pad_rows=2)
+    c.index[:] = 1
+    a, b, scales, index, starts, _ = c.device()
+    torch.full((43, 96), 5.0, dtype=BF16, device="cuda")                     # (what an output that is not written would hold)
+    got = adapter_delta(c.x.cuda(), a, b, scales, index[1:], starts[1:], most_new)
+    want, tol = c.delta()
+    want[:30] = 0
+    close(got, want, tol)
+    assert not got[:30].any()
+    assert not adapter_delta(c.x.cuda(), a, b, scales, index[:1], starts[:1].expand(2).contiguous(), 0).any()
+
+
 def test_other_indices_are_none():
     from energonai_b200.adapter import adapter_delta
     c = Case([2, 3, 1], 64, 96, 8, 2, BF16, seed=4)
