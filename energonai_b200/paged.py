@@ -164,7 +164,7 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     """Causal attention of the new tokens q [rows, heads*head_dim] over their sequences' pages, which hold the new keys and values
     already: single tokens, a few per sequence, prompts and chunks of prompts, or all of them in one batch.  window > 0:
     the row at position p sees the positions above p - window only.  most_length: no sequence is longer (None: what the
-    tables address).  Returns out [rows, heads*head_dim]; rows of no sequence are left as they are."""
+    tables address).  Returns out [rows, heads*head_dim], which may be q; rows of no sequence are left as they are."""
     device = _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)
     dtype, shape = q.dtype, q.shape
     kv_heads, head_dim, most_length, cache = _cache("paged_attention", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length)

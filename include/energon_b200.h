@@ -892,8 +892,9 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
 /* Many sequences at once, each with a length of its own, keys and values in pages of page_size (16, 32, 64 or 128)
  * positions: pools [pages][kv_heads][page_size][head_dim], in `dtype` (fp16 or bf16) or, with scales [pages][kv_heads],
  * as e4m3 codes (value = code * scale; no scale is negative, value scales below 2^-100 count as 2^-100).  Rows
- * starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the new tokens of sequence b, at most most_new; lengths[b] counts its positions with them, at most most_length, so that row i
- * of n_b has position lengths[b] - n_b + i.  Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
+ * starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the new tokens of sequence b, at most most_new;
+ * lengths[b] counts its positions with them, at most most_length, so that row i of n_b has position lengths[b] - n_b + i.
+ * Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
  * starts, lengths and tables live on the device and may change between replays of a captured call.  Pages that are none
  * (outside of the pool or behind the table's columns) hold nothing: nothing is written to them and nothing read.
  * head_dim is 64 or 128; heads / kv_heads query heads share a key / value head.  No counterpart in the reference. */
@@ -917,7 +918,7 @@ EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, 
 
 /* Causal attention of the new tokens over the cache (which holds them already): the row at position p sees the positions
  * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros; rows of `out` of no
- * sequence are left as they were.  Slots that no row sees may hold anything.
+ * sequence are left as they were.  `out` may be q.  Slots that no row sees may hold anything.
  * scratch: eb_paged_attention_scratch_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the
  * device need scratch of their own. */
 EB_API int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,

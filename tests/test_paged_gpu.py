@@ -248,6 +248,51 @@ def test_strided_queries_and_output():
     assert not out[:, :512].any() and not out[:, 1024:].any()
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("new,past", [([3, 1, 40, 2], [0, 300, 30, 5]), ([200, 1, 150, 90], [10, 3, 900, 0])])
+def test_a_part_of_a_batch(new, past, bits):
+    """The later sequences alone, out of tensors that hold them all: the rows in front of theirs stay as they are."""
+    from energonai_b200.paged import paged_append, paged_attention
+    c = Case(new, past, 6, 2, 128, 32, BF16, bits, seed=9, pad_rows=2)
+    (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    freq = frequencies(64).float()
+    some = (tables[1:], starts[1:], lengths[1:])
+    want = c.append(freq)
+    turned = paged_append(q, k, v, *pools, *some, most_new, freq=freq.cuda(), k_scale=scales[0], v_scale=scales[1], q_out=torch.full_like(q, 2.0))
+    n, end = c.starts[1], c.starts[-1]
+    close(turned[n:end], want[0][0][n:end], want[0][1][n:end])
+    assert bool((turned[:n] == 2.0).all()) and bool((turned[end:] == 2.0).all())
+    for i in (0, 1):                                                         # (the first sequence's pages: as before)
+        first = torch.tensor(c.tables[0], dtype=torch.long)
+        assert torch.equal(pools[i].cpu()[first].view(torch.uint8), c.pool[i][first].view(torch.uint8))
+    out = paged_attention(q, *pools, *some, most_new, k_scale=scales[0], v_scale=scales[1], out=torch.full_like(q, 3.0))
+    c.pool, c.scale = [p.cpu() for p in pools], [None if s is None else s.cpu() for s in scales]
+    value, tol = c.attention(prompt=64 // 3)
+    close(out[n:end], value[n:end], tol[n:end])
+    assert bool((out[:n] == 3.0).all()) and bool((out[end:] == 3.0).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("new,past,heads,kv_heads", [([1, 5, 2], [700, 30, 9], 8, 2), ([300, 1, 129], [0, 900, 60], 6, 2), ([80], [20000], 8, 8), ([130, 70], [5, 0], 10, 2)])
+def test_in_place_over_the_queries(new, past, heads, kv_heads, bits, dtype):
+    from energonai_b200.paged import paged_attention
+    c = Case(new, past, heads, kv_heads, 64, 64, dtype, bits, seed=11)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    want = paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1])
+    assert torch.equal(paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1], out=q), want)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_sequences_that_share_their_first_pages(bits):
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 70, 3], [100, 40, 60], 4, 2, 64, 16, F16, bits, seed=12)
+    for t in c.tables[1:]:
+        t[:2] = c.tables[0][:2]
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    close(paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), *c.attention())
+
+
 def test_results_do_not_depend_on_the_other_sequences():
     """A sequence gets the same bits alone and in a batch that is cut alike, and the same bits every time."""
     from energonai_b200.paged import paged_attention
