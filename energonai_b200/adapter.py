@@ -46,7 +46,7 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
 
 def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=None, static_weight=False):
     """x @ w.T + bias for all rows, and beside it each sequence's adapter (adapter_delta), added to the fp32 sums: [rows, columns].
-    Rows of no sequence get the shared projection alone."""
+    Rows of no sequence get the shared projection alone.  Calls on several streams and replayed graphs may overlap."""
     _one_device("adapter_product", w, bias, out)
     if w.dim() != 2 or w.shape != (b.shape[1], x.shape[1]) or w.dtype != x.dtype:
         raise RuntimeError("adapter_product: the shared weight is [columns, width] of the type of x")
@@ -58,4 +58,4 @@ def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=
             raise RuntimeError("adapter_product: one row of out per row of x")
     if x.shape[0] == 0:
         return torch.empty((0, w.shape[0]), dtype=x.dtype, device=x.device) if out is None else out
-    return gemm(x, w, bias=bias, residual=adapter_delta(x, a, b, scales, index, starts, most_new), out=out, static_weight=static_weight)
+    return gemm(x, w, bias=bias, residual=adapter_delta(x, a, b, scales, index, starts, most_new), out=out, static_weight=static_weight, overlap=True)

@@ -1410,6 +1410,14 @@ extern "C" size_t eb_gemm_workspace_bytes(int M, int N, int K) {
   return kCounterBytes + (size_t)sm_count() * 2 * swap_bn(M) * kLanes * sizeof(float);
 }
 
+extern "C" size_t eb_gemm_counter_bytes(int M, int N, int K, long long ldc) {
+  if (M > kLanes || M <= 0 || N <= 0 || K <= 0) return 0;
+  // the forms of gemm_impl that count nothing: tiles of 128 rows, and the generation step's
+  if (M > 32 && N % 8 == 0 && ldc % 8 == 0) return 0;
+  if (step_form_pays(M, N, K, step_geometry(M, K).smem)) return 0;
+  return (size_t)((N + kLanes - 1) / kLanes) * 4 * sizeof(int);
+}
+
 namespace eb {
 int attention_tc_status(int *out4, bool clear);   // attention_tc.cu
 int latent_status(int *out4, bool clear);         // latent_attention.cu

@@ -5,7 +5,7 @@ from ._lib import lib, check, dtype_code, ptr, stream_ptr, require_cuda, ACT_NON
 
 ACT_CODES = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "gelu_tanh": ACT_GELU_TANH, "gelu": ACT_GELU_ERF}
 
-_workspaces, _outgrown = {}, []
+_workspaces, _stream_workspaces, _outgrown = {}, {}, []
 
 
 def workspace(device, nbytes):
@@ -21,9 +21,31 @@ def workspace(device, nbytes):
     return ws
 
 
+def stream_workspace(device, M, N, K, ldc):
+    """Scratch of a small-M GEMM that may overlap others on its device: one buffer per stream, where calls follow one another, and
+    within a captured graph, which may be replayed on any stream, one of the call's own whose arrival counters the graph clears.  Sizes that
+    leave the scratch as it is take the device's."""
+    nbytes = lib().eb_gemm_workspace_bytes(M, N, K)
+    if not nbytes:
+        return None
+    counters = lib().eb_gemm_counter_bytes(M, N, K, ldc)
+    if not counters:
+        return workspace(device, nbytes)
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws[:counters].zero_()
+        return ws
+    key = torch.device(device).index, stream_ptr()
+    ws = _stream_workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        # (an outgrown one goes back to its stream's memory: no graph holds its address)
+        ws = _stream_workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    return ws
+
+
 def gemm(a, w, bias=None, act=None, residual=None, out=None, out_dtype=None, out_rows_per_batch=0,
          out_batch_stride=0, out_ld=None, out_row_offset_device=None, out_row_limit=0, static_weight=False, peer=None,
-         ln_fold=None):
+         ln_fold=None, overlap=False):
     """a [M,K] (row stride allowed), w [N,K]; returns out [M,N].
 
     `out`, if given, receives the result; with out_rows_per_batch > 0 row m is written at
@@ -35,6 +57,8 @@ def gemm(a, w, bias=None, act=None, residual=None, out=None, out_dtype=None, out
     on the stream (model weights), which lets the kernel prefetch it early.
     ln_fold=(colsum, bias32, eps), from fold_layernorm(): `a` is the un-normalised input of a
     LayerNorm and `w` the weight with the LayerNorm scale folded in (M <= 32 only).
+    overlap=True: the call may run beside others on the device (other streams, replayed graphs), so its scratch is not the
+    device's common one.
     (Asking a launch to pull the NEXT launch's weights into L2 was tried and removed: measured on
     B200 it slowed the generation step at every size, 6.50 -> 6.70 / 7.28 ms for 16 / 64 MB on one
     GPU and 2.50 -> 2.57 / 2.63 ms on an 8-way shard.)"""
@@ -57,8 +81,11 @@ def gemm(a, w, bias=None, act=None, residual=None, out=None, out_dtype=None, out
     if residual is not None and (residual.stride(-1) != 1 or residual.dtype != a.dtype):
         raise RuntimeError("gemm: residual must be row-major and of the operand dtype")
     code = ACT_CODES[act] if not isinstance(act, int) else act
-    nbytes = lib().eb_gemm_workspace_bytes(M, N, K)
-    ws = workspace(a.device, nbytes) if nbytes else None
+    if overlap:
+        ws = stream_workspace(a.device, M, N, K, out_ld)
+    else:
+        nbytes = lib().eb_gemm_workspace_bytes(M, N, K)
+        ws = workspace(a.device, nbytes) if nbytes else None
     if ln_fold is not None:
         colsum, bias32, eps = ln_fold
         if bias is not None or peer is not None:

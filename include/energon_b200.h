@@ -261,6 +261,11 @@ EB_API int eb_gemm(const void *A, long long lda, const void *W, long long ldw, v
             int c_row_offset_limit, int flags, void *workspace, size_t workspace_bytes, void *stream);
 EB_API size_t eb_gemm_workspace_bytes(int M, int N, int K);
 
+/* Bytes at the head of `workspace` that eb_gemm of these sizes keeps arrival counters in, zero before and after the call, with
+ * partial sums behind them; 0: the call leaves `workspace` alone, and calls that share it may overlap.  (Rows of C and of a residual
+ * ldc elements apart, c_rows_per_batch 0.) */
+EB_API size_t eb_gemm_counter_bytes(int M, int N, int K, long long ldc);
+
 /* eb_gemm (no residual, plain rows) for several things at once that read the same A, their weights
  * stacked in W.  act_params (or NULL): xIELU on the columns below act_cols, a multiple of 8; device floats
  * (softplus(p), 1/2 + softplus(q)) of

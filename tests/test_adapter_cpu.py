@@ -35,3 +35,35 @@ def test_cpu_tensors_are_rejected():
         adapter_delta(x, a, b, torch.ones(1), i32([0]), i32([0, 2]), 2)
     with pytest.raises(RuntimeError, match="CUDA"):
         adapter_product(x, torch.zeros(16, 64), a, b, torch.ones(1), i32([0]), i32([0, 2]), 2)
+
+
+def test_products_that_may_overlap_share_no_scratch(monkeypatch):
+    """A generation-step product keeps arrival counters and partial sums in its scratch: calls on two streams, and captured calls, have their own."""
+    from energonai_b200 import adapter, gemm
+    L = _lib.lib()
+    # few rows of a large weight count, the step form of a small one and tiles of 128 rows do not
+    assert L.eb_gemm_counter_bytes(16, 5120, 5120, 5120) == 40 * 16 and L.eb_gemm_counter_bytes(40, 520, 512, 516) == 5 * 16
+    assert L.eb_gemm_counter_bytes(16, 1024, 1024, 1024) == 0 and L.eb_gemm_counter_bytes(48, 5120, 5120, 5120) == 0 and L.eb_gemm_counter_bytes(200, 5120, 5120, 5120) == 0
+    stream, capturing = [7], [False]
+    monkeypatch.setattr(gemm, "stream_ptr", lambda: stream[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(gemm, "_stream_workspaces", {})
+    large = lambda: gemm.stream_workspace("cpu", 16, 5120, 5120, 5120)
+    first, again = large(), large()
+    assert first is again and first.numel() >= L.eb_gemm_workspace_bytes(16, 5120, 5120) and not first.any()
+    assert gemm.stream_workspace("cpu", 32, 5120, 5120, 5120).numel() > first.numel()
+    stream[0] = 9
+    other = large()
+    assert other.data_ptr() != first.data_ptr()
+    capturing[0] = True
+    captured = [large() for _ in range(2)]
+    assert len({t.data_ptr() for t in (first, other, *captured)}) == 4 and all(not t[:640].any() for t in captured)
+    assert gemm.stream_workspace("cpu", 200, 5120, 5120, 5120) is None
+
+    # ... and adapter_product asks for it
+    asked = []
+    monkeypatch.setattr(adapter, "_one_device", lambda *a: 0)
+    monkeypatch.setattr(adapter, "adapter_delta", lambda *a: None)
+    monkeypatch.setattr(adapter, "gemm", lambda *a, **kw: asked.append(kw))
+    adapter.adapter_product(torch.zeros(2, 64), torch.zeros(16, 64), torch.zeros(1, 8, 64), torch.zeros(1, 16, 8), None, None, None, 2)
+    assert asked[0]["overlap"] is True

@@ -93,6 +93,45 @@ def test_two_streams_at_once():
         assert all(torch.equal(o, want[n][0]) for o in got[n])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("new,width,columns", [([1] * 16, 5120, 5120), ([5, 27], 2048, 8192), ([2], 4096, 12288), ([40, 3], 512, 256), ([1] * 9, 512, 256)])
+def test_adapters_on_two_streams(new, width, columns, dtype):
+    """Products of few rows of a large weight are split over K and meet in scratch: eager calls on two streams, and two captured graphs that are
+    replayed on two streams, get the bits that they get alone."""
+    from energonai_b200.adapter import adapter_product
+    from energonai_b200.gemm import device_status
+    cases = [Adapters(new, width, columns, 16, 2, dtype, seed=s) for s in (3, 4)]
+    inputs = [(c.x.cuda(), c.w.cuda(), *c.device()) for c in cases]
+    want = [adapter_product(*i) for i in inputs]
+    close(want[0], *product(cases[0].x, cases[0], cases[0].w))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for n in (0, 1):
+        with torch.cuda.graph(graphs[n]):
+            outs.append([adapter_product(*inputs[n]) for _ in range(8)])
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(adapter_product(*inputs[n]))
+    torch.cuda.synchronize()
+    for n in (0, 1):
+        assert all(torch.equal(y, want[n]) for y in got[n])
+    for _ in range(5):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                graphs[n].replay()
+        torch.cuda.synchronize()
+        for n in (0, 1):
+            assert all(torch.equal(y, want[n]) for y in outs[n])
+            for y in outs[n]:
+                y.fill_(5.0)
+        torch.cuda.synchronize()
+    assert device_status()[0] == 0
+
+
 def test_tables_of_a_wider_table():
     from energonai_b200.paged import paged_attention
     c = Case([1, 7], [40, 90], 4, 2, 64, 32, torch.bfloat16, 16, seed=7)
