@@ -433,7 +433,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         return fmaf(fmaxf(fmaxf(r0, r1), fmaxf(x[14], x[15])), factors[g], logs[g]);
       };
       const float m = fmaxf(fmaxf(largest(x0, 0), largest(x0 + 16, 1)), fmaxf(largest(x1, 2), largest(x1 + 16, 3)));
-      if (__any_sync(0xffffffffu, m > m_ref + kRaise)) {
+      // (Rows behind the sequence's last have no vote: they hold another sequence's queries, or anything, which must not change these rows' bits.)
+      if (__any_sync(0xffffffffu, there && m > m_ref + kRaise)) {
         // The reference is raised, for all rows of the warp (tensor memory is read and written warp-wide), behind the last value product.
         const float m_new = fmaxf(m_ref, m), alpha = ex2(m_ref - m_new);
         m_ref = m_new;

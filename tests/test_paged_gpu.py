@@ -304,6 +304,33 @@ def test_results_do_not_depend_on_the_other_sequences():
         assert torch.equal(a, paged_attention(q, *pools, tables, starts, lengths, 1, **kw))
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("new,watched", [([1, 2, 1, 3, 1], (0, 3)), ([90, 1, 200, 5, 1], (0, 1, 2, 3))])
+def test_a_sequence_does_not_depend_on_the_others(new, watched, bits):
+    """The same bits whatever the other sequences bring, hold and are long, in a batch that is cut alike."""
+    from energonai_b200.paged import paged_attention
+    past = [9000, 8300, 30, 700, 5]
+    c = Case(new, past, 8, 2, 128, 16, BF16, bits, seed=1)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    kw = dict(k_scale=scales[0], v_scale=scales[1])
+    want = paged_attention(q, *pools, tables, starts, lengths, most_new, **kw)
+    close(want, *c.attention(prompt=16))
+    for b in watched:
+        rows, mine = slice(c.starts[b], c.starts[b + 1]), torch.zeros(c.pages, dtype=torch.bool, device="cuda")
+        mine[torch.tensor(c.tables[b], device="cuda")] = True
+        other = [p.clone() for p in pools]
+        for p in other:
+            p.view(torch.uint8)[~mine] = 0x35
+        zs = [None if s is None else torch.where(mine[:, None], s, 2.0 * s) for s in scales]
+        q2, lengths2, tables2 = -q, torch.clamp(lengths - 3, min=1), tables.flip(1).contiguous()
+        q2[rows], lengths2[b], tables2[b] = q[rows], lengths[b], tables[b]
+        lengths2 = torch.maximum(lengths2, starts[1:] - starts[:-1])
+        assert torch.equal(paged_attention(q2, *other, tables2, starts, lengths2, most_new, k_scale=zs[0], v_scale=zs[1])[rows], want[rows]), b
+        # the others bring nothing: its rows alone, in the same places
+        starts3 = torch.tensor([c.starts[b] if i <= b else c.starts[b + 1] for i in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+        assert torch.equal(paged_attention(q2, *other, tables2, starts3, lengths2, most_new, k_scale=zs[0], v_scale=zs[1])[rows], want[rows]), b
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
