@@ -39,17 +39,19 @@ template <typename T> __device__ __forceinline__ void mma_low(float (&c)[4], uin
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// two numbers as two 16-bit pieces each
+// two numbers as two 16-bit pieces each (an infinity is its first piece, and nothing is left of it)
 template <typename T> __device__ __forceinline__ void two_pieces(float x, float y, uint32_t &hi, uint32_t &lo) {
   hi = pack2<T>(x, y);
   const float2 f = unpack2<T>(hi);
-  lo = pack2<T>(x - f.x, y - f.y);
+  lo = pack2<T>(x == f.x ? 0.f : x - f.x, y == f.y ? 0.f : y - f.y);
 }
 
 // fp16 pieces: the power of two that brings the largest magnitude m of a low-rank row to [2^14, 2^15), so that the row keeps its
-// 22 bits whatever its size (2^-100 to 2^100); the products are divided by it in fp32.  bf16 has fp32's range.
+// 22 bits whatever its size (from 2^-100 on); the products are divided by it in fp32.  bf16 has fp32's range, but for what rounds up
+// beyond its largest number.
 template <typename T> __device__ __forceinline__ int lift_of(float m) {
-  return std::is_same<T, __half>::value ? min(max(14 - ((__float_as_int(m) >> 23) - 127), -100), 100) : 0;
+  const int e = (__float_as_int(m) >> 23) - 127;
+  return std::is_same<T, __half>::value ? min(max(14 - e, -113), 100) : e > 126 ? -1 : 0;
 }
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float largest_of(const float4 &v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }

@@ -159,3 +159,49 @@ def test_refusals():
         adapter_product(x, w[:8], a, b, scales, index, starts, most_new)
     with pytest.raises(RuntimeError, match="bias"):
         adapter_product(x, w, a, b, scales, index, starts, most_new, bias=torch.zeros(96, device="cuda"))
+
+
+def same_kind(got, want, tol):
+    """Infinities with their sign and NaN where they belong, the rest within the tolerance."""
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    there = want.isfinite()
+    assert bool(((got - want).abs()[there] <= tol[there]).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,rank", [([1, 3, 16], 8), ([5, 9], 40), ([70, 1], 16), ([40, 100], 64), ([64], 120)])
+def test_infinities_of_low_rank_rows(new, rank, dtype):
+    """An infinity keeps its sign, NaN stays NaN."""
+    from energonai_b200.adapter import adapter_delta
+    c = Case(new, 264, 136, rank, 2, dtype, seed=rank + len(new), pad_rows=2)
+    c.index[:] = 1
+    c.x[:, 7] = 0.0
+    c.x[0, 7], c.x[c.rows - 3, 7] = 1.0, -2.0                                # (the rows that meet them; for the others 0 * infinity is NaN)
+    rows = [0, c.rows - 3]
+    for value in (float("inf"), float("-inf"), float("nan")):
+        c.a[1, rank - 3, 7] = value
+        want, tol = c.delta()
+        same_kind(adapter_delta(c.x.cuda(), *c.device())[rows], want[rows], tol[rows])
+
+
+def test_low_rank_values_at_the_end_of_the_range():
+    """A low-rank value between bf16's and fp32's largest; and fp16's scaled far beyond its own range."""
+    from energonai_b200.adapter import adapter_delta
+    for dtype, x, a, b, scale in ((BF16, (1.0, 1.0), (torch.finfo(BF16).max, 1.5 * 2.0 ** 119), 2.0 ** -30, 1.0), (F16, (2.0 ** 14, 2.0 ** 14), (2.0 ** 13, 2.0 ** 12), 2.0 ** -20, 2.0 ** 97)):
+        for new in (3, 70):
+            c = Case([new], 64, 64, 16, 1, dtype, seed=2)
+            c.x.zero_()
+            c.a.zero_()
+            c.x[:, 0], c.x[:, 1] = x
+            c.a[0, 3, 0], c.a[0, 3, 1] = a
+            c.b[:] = b
+            c.scales[:] = scale
+            want, tol = c.delta()
+            if dtype == F16:                                                 # (beyond fp16 in the end: infinite, not NaN)
+                assert bool((adapter_delta(c.x.cuda(), *c.device()) == float("inf")).all())
+                c.b *= -1.0
+                assert bool((adapter_delta(c.x.cuda(), *c.device()) == float("-inf")).all())
+            else:
+                close(adapter_delta(c.x.cuda(), *c.device()), want, tol)
