@@ -19,7 +19,8 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
     """What each row's adapter adds to a projection of x [rows, width]: scales[i] (x a[i].T) b[i].T, [rows, columns], with
     i = index[s] for the rows starts[s] to starts[s + 1] - 1 of sequence s (at most most_new).  a [adapters, rank, width], b
     [adapters, columns, rank], scales fp32 [adapters]; index int32 [batch], negative for none; starts int32 [batch + 1].  rank is
-    a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows of no sequence get zeros."""
+    a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows of no sequence, and
+    those behind a sequence's first most_new, get zeros."""
     device = _one_device("adapter_delta", x, a, b, scales, index, starts)
     dtype, shape, of, to = x.dtype, x.shape, a.shape, b.shape
     if len(of) != 3 or len(to) != 3 or len(shape) != 2 or of[0] != to[0] or of[1] != to[2] or of[2] != shape[1]:
@@ -46,7 +47,7 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
 
 def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=None, static_weight=False):
     """x @ w.T + bias for all rows, and beside it each sequence's adapter (adapter_delta), added to the fp32 sums: [rows, columns].
-    Rows of no sequence get the shared projection alone.  Calls on several streams and replayed graphs may overlap."""
+    Rows of no sequence, and those behind a sequence's first most_new, get the shared projection alone.  Calls on several streams and replayed graphs may overlap."""
     _one_device("adapter_product", w, bias, out)
     if w.dim() != 2 or w.shape != (b.shape[1], x.shape[1]) or w.dtype != x.dtype:
         raise RuntimeError("adapter_product: the shared weight is [columns, width] of the type of x")

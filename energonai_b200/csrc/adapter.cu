@@ -25,7 +25,7 @@ struct AdapterParams {
   void *delta;
   float *low;                            // [splits][rows][rank]
   long long ldx, ldd;
-  int rows, width, columns, rank, count, batch, splits, per_split, chunk;   // per_split: columns of x per CTA; chunk: columns of delta per CTA
+  int rows, width, columns, rank, count, batch, most_new, splits, per_split, chunk;   // per_split: columns of x per CTA; chunk: columns of delta per CTA
 };
 
 template <typename T> __device__ __forceinline__ void mma_low(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -56,9 +56,10 @@ template <typename T> __device__ __forceinline__ int lift_of(float m) {
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float largest_of(const float4 &v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
-// Rows and adapter of sequence b; b = batch and batch + 1: the rows behind the last sequence and in front of the first, without one.
+// Rows and adapter of sequence b, which serves `live` of them, the announced ones; b = batch and batch + 1: the rows behind the last
+// sequence and in front of the first, without one.
 struct AdapterRows {
-  int row0, count, adapter;
+  int row0, count, live, adapter;
 };
 __device__ __forceinline__ AdapterRows adapter_rows(const AdapterParams &p, int b) {
   AdapterRows r;
@@ -66,6 +67,7 @@ __device__ __forceinline__ AdapterRows adapter_rows(const AdapterParams &p, int 
   r.count = (b == p.batch ? p.rows : min(p.starts[b > p.batch ? 0 : b + 1], p.rows)) - r.row0;
   r.adapter = b < p.batch ? p.index[b] : -1;
   if (r.adapter >= p.count) r.adapter = -1;
+  r.live = r.adapter < 0 ? 0 : min(r.count, p.most_new);
   return r;
 }
 
@@ -77,8 +79,8 @@ template <typename T, int NR> __global__ void __launch_bounds__(kAdapterWarps * 
   const int split = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const AdapterRows r = adapter_rows(p, b);
   const int t0 = blockIdx.x * kRowTile;
-  if (r.adapter < 0 || t0 >= r.count) return;
-  const int rows = min(kRowTile, r.count - t0), row0 = r.row0 + t0;
+  if (t0 >= r.live) return;
+  const int rows = min(kRowTile, r.live - t0), row0 = r.row0 + t0;
   const T *x = reinterpret_cast<const T *>(p.x), *a = reinterpret_cast<const T *>(p.a) + (long long)r.adapter * p.rank * p.width;
   const T *x0 = x + (long long)(row0 + min(g, rows - 1)) * p.ldx, *x1 = x + (long long)(row0 + min(g + 8, rows - 1)) * p.ldx;
   const bool in0 = g < rows, in1 = g + 8 < rows;
@@ -137,8 +139,8 @@ template <typename T, int RT> __global__ void __launch_bounds__(kAdapterWarps * 
   const int split = blockIdx.y, b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const AdapterRows r = adapter_rows(p, b);
   const int t0 = blockIdx.x * kLowRows;
-  if (r.adapter < 0 || t0 >= r.count) return;
-  const int rows = min(kLowRows, r.count - t0), row0 = r.row0 + t0;
+  if (t0 >= r.live) return;
+  const int rows = min(kLowRows, r.live - t0), row0 = r.row0 + t0;
   const T *x = reinterpret_cast<const T *>(p.x) + (long long)row0 * p.ldx, *a = reinterpret_cast<const T *>(p.a) + (long long)r.adapter * p.rank * p.width;
   const int begin = split * p.per_split, end = min(p.width, begin + p.per_split), steps = (end - begin + kLowStep - 1) / kLowStep;
   const uint32_t base = smem_u32(low_smem);
@@ -212,15 +214,15 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
   T *delta = reinterpret_cast<T *>(p.delta);
   // (the rows behind the last sequence may be more than the grid has tiles for)
   for (int t0 = blockIdx.x * kRowTile; t0 < r.count; t0 += gridDim.x * kRowTile) {
-    const int rows = min(kRowTile, r.count - t0), row0 = r.row0 + t0;
+    const int rows = min(kRowTile, r.count - t0), live = min(rows, r.live - t0), row0 = r.row0 + t0;
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
-    if (r.adapter < 0 || t0 >= (int)gridDim.x * kRowTile) {       // (rows that were not announced have no low-rank row)
+    if (live < rows) {                                     // (rows that were not announced have no low-rank row)
       for (int n0 = first; n0 < end; n0 += step)
         if (n0 + c * 8 < end) {
-          if (g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
-          if (g + 8 < rows) *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(0, 0, 0, 0);
+          if (g >= live && g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
+          if (g + 8 >= live && g + 8 < rows) *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(0, 0, 0, 0);
         }
-      continue;
+      if (live <= 0) continue;
     }
     const T *bm = reinterpret_cast<const T *>(p.b) + (long long)r.adapter * p.columns * p.rank + c * 4;
     // column i of tile t is n0 + 8 (i / 2) + 2 t + i % 2: lane c ends up with 8 columns that follow one another
@@ -247,7 +249,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
         for (int k = 0; k < KR; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (k * 16 + c * 4 < p.rank && g + 8 * h < rows) {
+            if (k * 16 + c * 4 < p.rank && g + 8 * h < live) {
               const float4 one = *reinterpret_cast<const float4 *>(p.low + ((long long)q * p.rows + row0 + g + 8 * h) * p.rank + k * 16 + c * 4);
               v[k][h] = make_float4(v[k][h].x + one.x, v[k][h].y + one.y, v[k][h].z + one.z, v[k][h].w + one.w);
             }
@@ -284,9 +286,9 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
       }
       fetch(n0 + step);                                    // (the next columns, while these are stored)
       if (n0 + c * 8 < end) {
-        if (g < rows)
+        if (g < live)
           *reinterpret_cast<uint4 *>(out0 + n0) = packed_row<T>(acc, 0, down[0]);
-        if (g + 8 < rows)
+        if (g + 8 < live)
           *reinterpret_cast<uint4 *>(out1 + n0) = packed_row<T>(acc, 2, down[1]);
       }
     }
@@ -311,16 +313,16 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
   // chunk of row i of a tile's eight
   auto swizzled = [](int i, int chunk) { return KR == 1 ? chunk ^ (i >> 2) : KR == 2 ? chunk ^ (i >> 1) : chunk ^ i; };
   for (int t0 = blockIdx.x * kLowRows; t0 < r.count; t0 += gridDim.x * kLowRows) {
-    const int rows = min(kRowTile, r.count - t0 - warp * kRowTile), row0 = r.row0 + t0 + warp * kRowTile;      // (of this warp; none: <= 0)
+    const int row0 = r.row0 + t0 + warp * kRowTile;          // (of this warp, which may have none: <= 0)
+    const int rows = min(kRowTile, r.count - t0 - warp * kRowTile), live = min(rows, r.live - t0 - warp * kRowTile);
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
-    if (r.adapter < 0 || t0 >= (int)gridDim.x * kLowRows) {       // (rows that were not announced have no low-rank row)
+    if (live < rows)                                       // (rows that were not announced have no low-rank row)
       for (int n0 = begin; n0 < end; n0 += 32)
         if (n0 + c * 8 < end) {
-          if (g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
-          if (g + 8 < rows) *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(0, 0, 0, 0);
+          if (g >= live && g < rows) *reinterpret_cast<uint4 *>(out0 + n0) = make_uint4(0, 0, 0, 0);
+          if (g + 8 >= live && g + 8 < rows) *reinterpret_cast<uint4 *>(out1 + n0) = make_uint4(0, 0, 0, 0);
         }
-      continue;
-    }
+    if (t0 >= r.live) continue;
     const T *bm = reinterpret_cast<const T *>(p.b) + (long long)r.adapter * p.columns * p.rank;
     auto fetch = [&](int i) {
       if (i < steps) {
@@ -344,7 +346,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
     const uint32_t at_hi = base + kDeltaStages * kStage, at_lo = at_hi + kPieces;
     uint8_t *pieces = delta_smem + kDeltaStages * kStage;
     float *downs = reinterpret_cast<float *>(pieces + 2 * kPieces);
-    const int all = min(kLowRows, r.count - t0), quads = p.rank / 4;
+    const int all = min(kLowRows, r.live - t0), quads = p.rank / 4;
     constexpr int kPer = 8 < 2 * KR ? 8 : 2 * KR;
     for (int e0 = threadIdx.x; e0 < kLowRows * KR * 4; e0 += kPer * kAdapterWarps * 32) {
       float4 v[kPer];
@@ -420,9 +422,9 @@ template <typename T, int KR> __global__ void __launch_bounds__(kAdapterWarps * 
         }
         const int n = begin + i * kDeltaCols + n0;
         if (n + c * 8 < end) {
-          if (g < rows)
+          if (g < live)
             *reinterpret_cast<uint4 *>(out0 + n) = packed_row<T>(acc, 0, down[0]);
-          if (g + 8 < rows)
+          if (g + 8 < live)
             *reinterpret_cast<uint4 *>(out1 + n) = packed_row<T>(acc, 2, down[1]);
         }
       }
@@ -522,7 +524,7 @@ extern "C" int eb_adapter_delta(const void *x, long long ldx, const void *a, con
   const AdapterPlan s = adapter_plan(batch, most_new, width);
   AdapterParams p{};
   p.x = x; p.a = a; p.b = b; p.scales = scales; p.index = index; p.starts = starts; p.delta = delta; p.low = reinterpret_cast<float *>(scratch);
-  p.ldx = ldx; p.ldd = ldd; p.rows = rows; p.width = width; p.columns = columns; p.rank = rank; p.count = adapters; p.batch = batch;
+  p.ldx = ldx; p.ldd = ldd; p.rows = rows; p.width = width; p.columns = columns; p.rank = rank; p.count = adapters; p.batch = batch; p.most_new = most_new;
   p.splits = s.splits; p.per_split = s.per_split;
   return dtype == EB_F16 ? launch_adapter<__half>(p, s, as_stream(stream)) : launch_adapter<__nv_bfloat16>(p, s, as_stream(stream));
 }

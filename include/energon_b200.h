@@ -932,7 +932,7 @@ EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_head
 
 /* Low-rank adapters of many requests: for the rows starts[b] to starts[b + 1] - 1 (at most most_new) of each sequence, with
  * i = index[b],  delta = scales[i] (x a[i]^T) b[i]^T,  a [adapters][rank][width], b [adapters][columns][rank], rank a multiple
- * of 8 up to 128.  An index outside of 0 .. adapters - 1, and rows of no sequence: zeros.  delta is what the
+ * of 8 up to 128.  An index outside of 0 .. adapters - 1, rows of no sequence, and what a sequence brings beyond most_new rows: zeros.  delta is what the
  * projection beside it adds as its residual.  scratch: eb_adapter_scratch_bytes(...) bytes, 16-byte aligned, of any content.
  * No counterpart in the reference. */
 EB_API int eb_adapter_delta(const void *x, long long ldx, const void *a, const void *b, const float *scales, const int32_t *index,

@@ -205,3 +205,19 @@ def test_low_rank_values_at_the_end_of_the_range():
                 assert bool((adapter_delta(c.x.cuda(), *c.device()) == float("-inf")).all())
             else:
                 close(adapter_delta(c.x.cuda(), *c.device()), want, tol)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("most_new", [1, 10, 15, 17, 63, 65, 70])
+def test_the_adapter_ends_at_the_announced_rows(most_new, dtype):
+    from energonai_b200.adapter import adapter_delta, adapter_product
+    c = Case([100, 12, 30], 136, 264, 24, 2, dtype, seed=most_new, pad_rows=1)
+    c.index[:] = torch.tensor([1, -1, 0], dtype=torch.int32)
+    want, tol = c.delta()
+    c.most_new = most_new
+    for first, n in ((0, 100), (112, 30)):
+        want[first + most_new:first + n], tol[first + most_new:first + n] = 0, 0
+    close(adapter_delta(c.x.cuda(), *c.device()), want, tol)
+    y = c.x.double() @ c.w.double().T
+    size = c.x.double().abs() @ c.w.double().abs().T
+    close(adapter_product(c.x.cuda(), c.w.cuda(), *c.device()), y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 136 / 16 + 2.0 ** -20) * size)
