@@ -21,28 +21,39 @@ def adapter_delta(x, a, b, scales, index, starts, most_new):
     [adapters, columns, rank], scales fp32 [adapters]; index int32 [batch], negative for none; starts int32 [batch + 1].  rank is
     a multiple of 8 up to MAX_RANK (smaller adapters are filled up with zeros).  Rows of no sequence, and
     those behind a sequence's first most_new, get zeros."""
-    device = _one_device("adapter_delta", x, a, b, scales, index, starts)
+    return _adapters("adapter_delta", x, a, b, scales, index, starts, most_new)
+
+
+def _adapters(what, x, a, b, scales, index, starts, most_new, base=None, out=None):
+    """adapter_delta, or what base() returns (fp32) and adapter_delta, added up and rounded once (to out, of the type of x)."""
+    device = _one_device(what, x, a, b, scales, index, starts)
     dtype, shape, of, to = x.dtype, x.shape, a.shape, b.shape
     if len(of) != 3 or len(to) != 3 or len(shape) != 2 or of[0] != to[0] or of[1] != to[2] or of[2] != shape[1]:
-        raise RuntimeError("adapter_delta: x [rows, width], a [adapters, rank, width] and b [adapters, columns, rank] required")
+        raise RuntimeError(f"{what}: x [rows, width], a [adapters, rank, width] and b [adapters, columns, rank] required")
     if a.dtype is not dtype or b.dtype is not dtype or not a.is_contiguous() or not b.is_contiguous():
-        raise RuntimeError("adapter_delta: adapters are contiguous and of the type of x")
+        raise RuntimeError(f"{what}: adapters are contiguous and of the type of x")
     adapters, rank, width = of
     if scales.dtype is not torch.float32 or scales.shape != (adapters,) or not scales.is_contiguous():
-        raise RuntimeError("adapter_delta: one fp32 scale per adapter")
+        raise RuntimeError(f"{what}: one fp32 scale per adapter")
     batch = index.numel()
     if index.dtype is not torch.int32 or starts.dtype is not torch.int32 or index.dim() != 1 or starts.shape != (batch + 1,) or batch == 0 or not (
             index.is_contiguous() and starts.is_contiguous()):
-        raise RuntimeError("adapter_delta: int32 index [batch] and starts [batch + 1] required")
+        raise RuntimeError(f"{what}: int32 index [batch] and starts [batch + 1] required")
     rows, columns, most_new = shape[0], to[1], int(most_new) or 1        # (0: zeros are all that is asked for)
-    ldx = _rows("adapter_delta", x, width, dtype)
-    delta = x.new_empty((rows, columns))
+    ldx = _rows(what, x, width, dtype)
+    given, out = out, out if out is not None and out.stride(0) % 8 == 0 else x.new_empty((rows, columns))
     nbytes = _scratch_bytes(rows, width, rank, batch, most_new)
     scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None       # (of this call: captured calls share none)
-    check(lib().eb_adapter_delta(x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), scales.data_ptr(), index.data_ptr(), starts.data_ptr(), delta.data_ptr(), columns,
-                                 rows, width, columns, rank, adapters, batch, most_new, dtype_code(dtype), None if scratch is None else scratch.data_ptr(),
-                                 nbytes, _stream_of(device)), "adapter_delta", launches=2)
-    return delta
+    of, sequences = (x.data_ptr(), ldx, a.data_ptr()), (index.data_ptr(), starts.data_ptr())
+    sizes = (rank, adapters, batch, most_new, dtype_code(dtype), None if scratch is None else scratch.data_ptr(), nbytes, _stream_of(device))
+    to = (out.data_ptr(), _rows(what, out, columns, dtype), rows, width, columns)
+    if base is None:
+        check(lib().eb_adapter_delta(*of, b.data_ptr(), scales.data_ptr(), *sequences, *to, *sizes), what, launches=2)
+        return out
+    check(lib().eb_adapter_low(*of, *sequences, rows, width, *sizes), what)
+    sums = base()
+    check(lib().eb_adapter_add(b.data_ptr(), scales.data_ptr(), *sequences, sums.data_ptr(), columns, *to, *sizes), what)
+    return out if given is None or given is out else given.copy_(out)      # (rows that do not begin on 16 bytes)
 
 
 def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=None, static_weight=False):
@@ -59,4 +70,7 @@ def adapter_product(x, w, a, b, scales, index, starts, most_new, bias=None, out=
             raise RuntimeError("adapter_product: one row of out per row of x")
     if x.shape[0] == 0:
         return torch.empty((0, w.shape[0]), dtype=x.dtype, device=x.device) if out is None else out
+    if x.dtype is torch.float16:                            # (the adapter's part alone may be beyond fp16)
+        return _adapters("adapter_product", x, a, b, scales, index, starts, most_new,
+                         lambda: gemm(x, w, bias=bias, out_dtype=torch.float32, static_weight=static_weight, overlap=True), out)
     return gemm(x, w, bias=bias, residual=adapter_delta(x, a, b, scales, index, starts, most_new), out=out, static_weight=static_weight, overlap=True)

@@ -1,4 +1,6 @@
 """Python entry to the tcgen05 GEMM (eb_gemm): C = act(A @ W.T + bias) + residual."""
+import functools
+
 import torch
 
 from ._lib import lib, check, dtype_code, ptr, stream_ptr, require_cuda, ACT_NONE, ACT_RELU, ACT_GELU_TANH, ACT_GELU_ERF
@@ -21,16 +23,18 @@ def workspace(device, nbytes):
     return ws
 
 
+@functools.lru_cache(maxsize=4096)
+def _stream_workspace_bytes(M, N, K, ldc):
+    return lib().eb_gemm_workspace_bytes(M, N, K), lib().eb_gemm_counter_bytes(M, N, K, ldc)
+
+
 def stream_workspace(device, M, N, K, ldc):
     """Scratch of a small-M GEMM that may overlap others on its device: one buffer per stream, where calls follow one another, and
     within a captured graph, which may be replayed on any stream, one of the call's own whose arrival counters the graph clears.  Sizes that
     leave the scratch as it is take the device's."""
-    nbytes = lib().eb_gemm_workspace_bytes(M, N, K)
-    if not nbytes:
-        return None
-    counters = lib().eb_gemm_counter_bytes(M, N, K, ldc)
+    nbytes, counters = _stream_workspace_bytes(M, N, K, ldc)
     if not counters:
-        return workspace(device, nbytes)
+        return workspace(device, nbytes) if nbytes else None
     if torch.cuda.is_current_stream_capturing():
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
         ws[:counters].zero_()

@@ -938,6 +938,14 @@ EB_API size_t eb_paged_attention_scratch_bytes(int batch, int heads, int kv_head
 EB_API int eb_adapter_delta(const void *x, long long ldx, const void *a, const void *b, const float *scales, const int32_t *index,
                      const int32_t *starts, void *delta, long long ldd, int rows, int width, int columns, int rank, int adapters, int batch,
                      int most_new, int dtype, void *scratch, size_t scratch_bytes, void *stream);
+/* The same for fp16, whose range delta may leave where its sum with the projection does not: eb_adapter_low leaves x a[i]^T in scratch, and eb_adapter_add,
+ * with the same sizes and scratch, adds delta to the projection's fp32 sums base [rows][columns] and rounds once: out = base + delta, for rows
+ * without an adapter base alone. */
+EB_API int eb_adapter_low(const void *x, long long ldx, const void *a, const int32_t *index, const int32_t *starts, int rows, int width, int rank,
+                   int adapters, int batch, int most_new, int dtype, void *scratch, size_t scratch_bytes, void *stream);
+EB_API int eb_adapter_add(const void *b, const float *scales, const int32_t *index, const int32_t *starts, const float *base, long long ldbase, void *out,
+                   long long ldo, int rows, int width, int columns, int rank, int adapters, int batch, int most_new, int dtype,
+                   void *scratch, size_t scratch_bytes, void *stream);
 EB_API size_t eb_adapter_scratch_bytes(int rows, int width, int rank, int batch, int most_new);
 
 /* Device-side waits are bounded; when one expires the kernel records it and returns.  This

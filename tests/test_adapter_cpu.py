@@ -67,3 +67,20 @@ def test_products_that_may_overlap_share_no_scratch(monkeypatch):
     monkeypatch.setattr(adapter, "gemm", lambda *a, **kw: asked.append(kw))
     adapter.adapter_product(torch.zeros(2, 64), torch.zeros(16, 64), torch.zeros(1, 8, 64), torch.zeros(1, 16, 8), None, None, None, 2)
     assert asked[0]["overlap"] is True
+
+
+def test_the_two_launches_refuse():
+    of = dict(x=FAKE, ldx=64, a=FAKE)
+    sequences = dict(index=FAKE, starts=FAKE)
+    sizes = dict(rank=16, adapters=3, batch=2, most_new=4, dtype=_lib.F16, scratch=FAKE, scratch_bytes=1 << 20, stream=None)
+    low = {**of, **sequences, "rows": 4, "width": 64, **sizes}
+    add = {"b": FAKE, "scales": FAKE, **sequences, "base": FAKE, "ldbase": 128, "out": FAKE, "ldo": 128, "rows": 4, "width": 64, "columns": 128, **sizes}
+    L = _lib.lib()
+    both = [(dict(index=None), "null"), (dict(dtype=_lib.BF16), "fp16 only"), (dict(dtype=_lib.F32), "fp16 or bf16"), (dict(rank=12), "rank 12"), (dict(scratch_bytes=8), "scratch"),
+            (dict(most_new=0), "bad sizes"), (dict(batch=0), "bad sizes")]
+    for change, words in both + [(dict(x=None), "null"), (dict(a=FAKE + 8), "16-byte"), (dict(ldx=56), "hold a row"), (dict(width=60), "multiples of 8")]:
+        assert L.eb_adapter_low(*{**low, **change}.values()) == -1 and words in _lib.last_error(), change
+    for change, words in both + [(dict(base=None), "null"), (dict(out=None), "null"), (dict(ldbase=124), "hold a row"), (dict(ldbase=120), "hold a row"), (dict(ldo=132), "hold a row"),
+                                 (dict(base=FAKE + 4), "16-byte"), (dict(columns=124), "multiples of 8")]:
+        assert L.eb_adapter_add(*{**add, **change}.values()) == -1 and words in _lib.last_error(), change
+    assert L.eb_adapter_low(*{**low, "rows": 0}.values()) == 0 and L.eb_adapter_add(*{**add, "rows": 0}.values()) == 0

@@ -221,3 +221,41 @@ def test_the_adapter_ends_at_the_announced_rows(most_new, dtype):
     y = c.x.double() @ c.w.double().T
     size = c.x.double().abs() @ c.w.double().abs().T
     close(adapter_product(c.x.cuda(), c.w.cuda(), *c.device()), y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 136 / 16 + 2.0 ** -20) * size)
+
+
+@pytest.mark.parametrize("new", [[3, 1], [40], [70, 30, 1]])
+def test_an_adapters_part_beyond_half_precision(new):
+    """The adapter's part alone is more than fp16 holds, its sum with the shared projection is not."""
+    from energonai_b200.adapter import adapter_product
+    c = Case(new, 256, 136, 16, 2, F16, seed=len(new), pad_rows=2)
+    c.index[:] = 0
+    c.index[-1] = 1
+    # x W^T near -100,000, the adapters' part near 100,000: one column of ones carries both
+    c.x[:, 0] = 256.0
+    c.w[:, 0] = -390.0
+    c.a[:, :, 0] = 0.0
+    c.a[:, 0, 0] = 4.0
+    c.b[:, :, 0] = 97.5
+    c.scales[:] = 1.0
+    want, tol = c.delta()
+    y = c.x.double() @ c.w.double().T
+    size = c.x.double().abs() @ c.w.double().abs().T
+    n = sum(new)
+    assert float(want[:n].abs().min()) > 65504 and float((y + want)[:n].abs().max()) < 30000
+    got = adapter_product(c.x.cuda(), c.w.cuda(), *c.device())
+    tol = tol - UNIT[F16] * want.abs() + UNIT[F16] * (y + want).abs() + (2.0 ** -23 * 256 / 16 + 2.0 ** -20) * size
+    close(got[:n], (y + want)[:n], tol[:n])
+    assert bool((got[n:].double().cpu() == float("-inf")).all())             # (rows of no sequence: the shared projection alone, beyond fp16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new", [[4, 30], [1]])
+def test_output_rows_of_any_stride(new, dtype):
+    from energonai_b200.adapter import adapter_product
+    c = Case(new, 256, 128, 16, 2, dtype, seed=5)
+    wide = torch.zeros(c.rows, 132, dtype=dtype, device="cuda")
+    got = adapter_product(c.x.cuda(), c.w.cuda(), *c.device(), out=wide[:, :128])
+    assert got.data_ptr() == wide.data_ptr() and not wide[:, 128:].any()
+    want, tol = c.delta()
+    y, size = c.x.double() @ c.w.double().T, c.x.double().abs() @ c.w.double().abs().T
+    close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 256 / 16 + 2.0 ** -20) * size)
