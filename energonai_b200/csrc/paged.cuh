@@ -14,6 +14,7 @@ struct PagedBatch {
   const int *tables, *starts, *lengths;
   long long table_ld;
   int batch, rows, table_cols, pages, page_shift;
+  int most_new, clear;                 // rows of a sequence that are served at most; whether rows that none serves get zeros
 };
 
 namespace {
@@ -22,16 +23,32 @@ namespace {
 constexpr float kLeastScale = 7.888609052210118e-31f;
 
 struct PagedRows {
-  int row0, count, past, length;       // first row, rows, positions in front of them, positions in all
+  int row0, count, past, length, end;  // first row, rows (the announced ones), positions in front of them, positions in all, end of the sequence's rows
 };
 __device__ __forceinline__ PagedRows paged_rows(const PagedBatch &p, int b) {
   PagedRows r;
   r.row0 = max(p.starts[b], 0);
-  r.count = min(p.starts[b + 1], p.rows) - r.row0;
+  r.end = min(p.starts[b + 1], p.rows);
+  r.count = min(r.end - r.row0, p.most_new);
   r.length = p.lengths[b];
   r.past = r.length - (p.starts[b + 1] - p.starts[b]);
   if (r.past < 0 || r.count < 0) r.count = 0;          // (no such sequence)
   return r;
+}
+// Zeros to the rows of `out` (columns `col` to `col + cols`, a multiple of 8) that no sequence serves: those behind the announced ones of
+// sequence b (all of one that is none), in front of the first sequence and behind the last.  By `threads` threads, this one number `thread`.
+template <typename T> __device__ __forceinline__ void paged_clear(const PagedBatch &p, const PagedRows &r, int b, T *out, long long ld, int col, int cols, int thread, int threads) {
+  const bool front = b == 0 && r.row0 > 0, behind = b == p.batch - 1 && r.end < p.rows;
+  if (__builtin_expect(!(front || behind || r.row0 + r.count < r.end), 1)) return;
+  const int per = cols / 8;
+  auto clear = [&](int from, int to) {
+#pragma unroll 1
+    for (long long i = thread; i < (long long)(to - from) * per; i += threads)
+      *reinterpret_cast<uint4 *>(out + (from + i / per) * ld + col + i % per * 8) = make_uint4(0, 0, 0, 0);
+  };
+  clear(r.row0 + r.count, r.end);
+  if (front) clear(0, min(r.row0, p.rows));
+  if (behind) clear(max(r.end, 0), p.rows);
 }
 __device__ __forceinline__ int paged_page(const PagedBatch &p, int b, int at) {   // page of table entry `at`, or -1
   if (at < 0 || at >= p.table_cols) return -1;
@@ -61,8 +78,9 @@ inline int paged_check(const char *what, PagedBatch &p, const eb_paged &c, int r
   EB_REQUIRE(page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128, "%s: pages of %d positions not supported (16, 32, 64 or 128)", what,
              page_size);
   EB_REQUIRE((long long)table_cols * page_size < (1ll << 30), "%s: a table addresses at most 2^30 positions", what);
+  EB_REQUIRE((c.flags & ~EB_PAGED_CLEAR) == 0, "%s: unknown flag bits 0x%x", what, c.flags);
   p.tables = tables; p.table_ld = table_ld; p.starts = starts; p.lengths = lengths; p.batch = batch; p.rows = rows; p.table_cols = table_cols;
-  p.pages = pages;
+  p.pages = pages; p.most_new = c.most_new < rows ? c.most_new : rows; p.clear = c.flags & EB_PAGED_CLEAR;
   p.page_shift = page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : 7;
   return EB_OK;
 }

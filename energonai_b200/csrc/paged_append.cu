@@ -29,7 +29,7 @@ struct AppendParams {
   void *k_pages, *v_pages;             // [pages][kv_heads][page_size][D]
   float *k_scale, *v_scale;            // [pages][kv_heads] (8 bits)
   const float *freq;                   // [pairs]
-  int heads, kv_heads, pairs, parts, most_new;   // parts: CTAs that share the heads
+  int heads, kv_heads, pairs, parts;   // parts: CTAs that share the heads
 };
 
 // Sine and cosine of an angle of any size: less its quarter turns in 64 bits (two parts of pi / 2: the rest is good to 2^-40 for
@@ -61,7 +61,9 @@ template <typename T, bool EIGHT, int D> __global__ void __launch_bounds__(kAppe
   const int b = blockIdx.z, part = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int page_size = 1 << p.batch.page_shift;
   const PagedRows r = paged_rows(p.batch, b);
-  const int at = (r.past >> p.batch.page_shift) + blockIdx.x, begin = max(at << p.batch.page_shift, r.past), end = min((at + 1) << p.batch.page_shift, r.past + min(r.count, p.most_new));
+  if (p.batch.clear && p.q_out && blockIdx.x == 0)
+    paged_clear(p.batch, r, b, reinterpret_cast<T *>(p.q_out), p.ldo, 0, p.heads * D, part * kAppendThreads + threadIdx.x, p.parts * kAppendThreads);
+  const int at = (r.past >> p.batch.page_shift) + blockIdx.x, begin = max(at << p.batch.page_shift, r.past), end = min((at + 1) << p.batch.page_shift, r.past + r.count);
   if (begin >= end) return;
   const int n = end - begin, slot0 = begin & (page_size - 1), row0 = r.row0 + begin - r.past;
   const int page = paged_page(p.batch, b, at);
@@ -254,7 +256,6 @@ extern "C" int eb_paged_append(const eb_paged *cache, const void *q, long long l
   p.k_pages = k_pages; p.v_pages = v_pages; p.k_scale = k_scale; p.v_scale = v_scale; p.freq = freq;
   p.heads = heads; p.kv_heads = kv_heads; p.pairs = pairs;
   if (most_new > rows) most_new = rows;
-  p.most_new = most_new;
   const int touched = (most_new - 1 + page_size - 1) / page_size + 1, held = most_new < page_size ? most_new : page_size;
   // up to eight CTAs for every multiprocessor, as the sequences may bring much less than they are announced with (75 us with two,
   // 61 with eight: nine prompts of up to 1500 tokens); each computes the angles of its rows

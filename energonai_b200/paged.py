@@ -87,11 +87,16 @@ def _rows(what, t, width, dtype):
     raise RuntimeError(f"{what}: rows of {width} contiguous columns of {dtype} required, not {tuple(shape)} of {t.dtype}")
 
 
+def _new_like(q, most_new):
+    """Rows for the results of q, contiguous as rows of q are; the kernel clears those of no sequence, unless nothing is announced."""
+    return torch.empty_like(q) if most_new else torch.zeros_like(q)
+
+
 # struct eb_paged of the header
 _paged = struct.Struct("@7Pq10i")
 
 
-def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length):
+def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length, clear):
     """Checks pools and batch; returns (kv_heads, head_dim, positions that the tables address, struct eb_paged)."""
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
@@ -121,18 +126,19 @@ def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_sc
     reach = cols * page_size
     most_length = reach if most_length is None else min(int(most_length), reach)
     return kv_heads, head_dim, most_length, _paged.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), ld, pages,
-                                                        page_size, kv_heads, head_dim, cols, batch, min(int(most_new), (1 << 31) - 1), most_length, dtype_code(dtype), 0)
+                                                        page_size, kv_heads, head_dim, cols, batch, min(int(most_new), (1 << 31) - 1), most_length, dtype_code(dtype), 1 if clear else 0)
 
 
 def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, freq=None, k_scale=None, v_scale=None, q_out=None):
     """New keys and values k, v [rows, kv_heads*head_dim] to their pages; freq (fp32: angle per position of each leading pair of
     neighbouring dimensions): queries q [rows, heads*head_dim] and keys are turned on the way.  q, k and v may be column
     ranges of one projection.  Returns the turned queries (in q_out, which may be q, or a new tensor; without freq: q itself
-    unless q_out is given).  k_scale / v_scale belong to 8-bit pools and are updated: a page's scale grows to what its largest
+    unless q_out is given).  Rows of no sequence, and those behind a sequence's first most_new, are zeros in a new tensor and left as they are in
+    q_out.  k_scale / v_scale belong to 8-bit pools and are updated: a page's scale grows to what its largest
     value needs, and the codes that it holds already are rounded to the new one."""
     device = _one_device("paged_append", q, k, v, k_pages, v_pages, tables, starts, lengths, freq, k_scale, v_scale, q_out)
     dtype = q.dtype
-    kv_heads, head_dim, _, cache = _cache("paged_append", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, None)
+    kv_heads, head_dim, _, cache = _cache("paged_append", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, None, q_out is None)
     shape, width = q.shape, kv_heads * head_dim
     if len(shape) != 2 or shape[1] % width or k.shape[0] != shape[0] or v.shape[0] != shape[0]:
         raise RuntimeError("paged_append: one row of q, k and v per token, query heads in equal groups")
@@ -144,7 +150,7 @@ def paged_append(q, k, v, k_pages, v_pages, tables, starts, lengths, most_new, f
         if freq.dtype is not torch.float32 or freq.dim() != 1 or not freq.is_contiguous() or 2 * pairs > head_dim:
             raise RuntimeError("paged_append: frequencies are fp32, one for each leading pair of a head")
         if q_out is None:
-            q_out = torch.empty_like(q)                     # (contiguous: rows of q are)
+            q_out = _new_like(q, most_new)
     ldo = 0
     if q_out is not None:
         ldo = _rows("paged_append", q_out, columns, dtype)
@@ -164,17 +170,18 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
     """Causal attention of the new tokens q [rows, heads*head_dim] over their sequences' pages, which hold the new keys and values
     already: single tokens, a few per sequence, prompts and chunks of prompts, or all of them in one batch.  window > 0:
     the row at position p sees the positions above p - window only.  most_length: no sequence is longer (None: what the
-    tables address).  Returns out [rows, heads*head_dim], which may be q; rows of no sequence are left as they are."""
+    tables address).  Returns out [rows, heads*head_dim], which may be q.  Rows of no sequence, and those behind a sequence's first most_new,
+    are left as they are in an out that is given, and zeros in a new tensor."""
     device = _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)
     dtype, shape = q.dtype, q.shape
-    kv_heads, head_dim, most_length, cache = _cache("paged_attention", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length)
+    kv_heads, head_dim, most_length, cache = _cache("paged_attention", dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, most_new, most_length, out is None)
     if len(shape) != 2 or shape[1] % (kv_heads * head_dim):
         raise RuntimeError("paged_attention: q is [rows, heads*head_dim], query heads in equal groups")
     rows, columns = shape
     heads = columns // head_dim
     ldq = _rows("paged_attention", q, columns, dtype)
     if out is None:
-        out = torch.empty_like(q)                           # (contiguous: rows of q are)
+        out = _new_like(q, most_new)
         ldo = columns
     else:
         ldo = _rows("paged_attention", out, columns, dtype)

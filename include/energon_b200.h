@@ -900,30 +900,33 @@ EB_API int eb_attention_decode_noalloc(const void *q, const void *k, const void 
  * starts[b] to starts[b + 1] - 1 (starts: batch + 1 entries, rising) are the new tokens of sequence b, at most most_new;
  * lengths[b] counts its positions with them, at most most_length, so that row i of n_b has position lengths[b] - n_b + i.
  * Position p lies in slot p mod page_size of page tables[b * table_ld + p / page_size].
+ * What a sequence brings beyond most_new rows, and a sequence of fewer positions than rows, is not served.
+ * flags: EB_PAGED_CLEAR sets the rows of q_out and out that no sequence serves to zeros, without it they are left as they were (most_new 0: nothing is
+ * touched either way).
  * starts, lengths and tables live on the device and may change between replays of a captured call.  Pages that are none
  * (outside of the pool or behind the table's columns) hold nothing: nothing is written to them and nothing read.
  * head_dim is 64 or 128; heads / kv_heads query heads share a key / value head.  No counterpart in the reference. */
+#define EB_PAGED_CLEAR 1
 typedef struct eb_paged {
   void *k_pages, *v_pages;
   float *k_scale, *v_scale;       /* both or neither */
   const int32_t *tables, *starts, *lengths;
   int64_t table_ld;
-  int32_t pages, page_size, kv_heads, head_dim, table_cols, batch, most_new, most_length, dtype, reserved;
+  int32_t pages, page_size, kv_heads, head_dim, table_cols, batch, most_new, most_length, dtype;
+  union { int32_t flags, reserved; };      /* (`reserved`: its earlier name, 0 then) */
 } eb_paged;
 
 /* New tokens into the cache: for i < pairs (z_2i, z_2i+1) of every query and key head turned by the angle
  * position * freq[i] (taken in 64 bits), queries to q_out (NULL: left alone; may be q), keys and values to their pages.  With
  * scales: a page's scale is the smallest power of two (2^-100 at least) with which the largest finite magnitude fits
  * 448, or the one that it had if that is larger and the page holds earlier positions of the sequence, whose codes are then
- * rounded to the new scale; infinities and NaN become NaN.  Slots in front of and behind the new rows, other pages and rows
- * of q_out of no sequence are left as they were, and so is what a sequence brings beyond most_new rows.  A page
- * that this call writes belongs to one sequence. */
+ * rounded to the new scale; infinities and NaN become NaN.  Slots in front of and behind the new rows and other pages are
+ * left as they were.  A page that this call writes belongs to one sequence. */
 EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, const void *k, long long ldk, const void *v, long long ldv, void *q_out,
                     long long ldo, int rows, int heads, const float *freq, int pairs, void *stream);
 
 /* Causal attention of the new tokens over the cache (which holds them already): the row at position p sees the positions
- * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros; rows of `out` of no
- * sequence are left as they were.  `out` may be q.  Slots that no row sees may hold anything.
+ * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros.  `out` may be q.  Slots that no row sees may hold anything.
  * scratch: eb_paged_attention_scratch_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the
  * device need scratch of their own. */
 EB_API int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,

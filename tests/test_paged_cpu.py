@@ -123,3 +123,8 @@ def test_the_cache_struct_matches_the_header(tmp_path):
     assert [getattr(Paged, n).offset for n in names] == offsets
     packed = Paged.from_buffer_copy(paged._paged.pack(*range(1, len(names) + 1)))
     assert [getattr(packed, n) for n in names] == list(range(1, len(names) + 1))
+
+
+def test_unknown_flags_are_refused():
+    for call in (append_call, attention_call):
+        assert call(reserved=2) == -1 and "flag bits" in _lib.last_error()

@@ -331,6 +331,57 @@ def test_a_sequence_does_not_depend_on_the_others(new, watched, bits):
         assert torch.equal(paged_attention(q2, *other, tables2, starts3, lengths2, most_new, k_scale=zs[0], v_scale=zs[1])[rows], want[rows]), b
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("new,past", [([1, 1], [40, 9]), ([3, 1, 40, 2], [0, 300, 30, 5]), ([200, 1, 150, 90], [10, 3, 900, 0]), ([1, 0, 1], [20000, 5, 7])])
+def test_rows_of_no_sequence_of_new_tensors_are_zeros(new, past, bits):
+    """In front of the first sequence and behind the last one, behind the announced rows, and of a sequence that is none: zeros where the call makes the
+    tensor, nothing where the caller gives it."""
+    from energonai_b200.paged import paged_append, paged_attention
+    c = Case(new, past, 6, 2, 128, 32, BF16, bits, seed=9, pad_rows=5)
+    (q, k, v), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    freq = frequencies(64).float().cuda()
+    kw = dict(k_scale=scales[0], v_scale=scales[1])
+    dirty = lambda: torch.full_like(q, float("nan"))                         # (what an output that is not written would hold)
+
+    def both(tables, starts, lengths, most_new):
+        dirty()
+        turned = paged_append(q, k, v, *[p.clone() for p in pools], tables, starts, lengths, most_new, freq=freq, k_scale=None if bits == 16 else scales[0].clone(),
+                              v_scale=None if bits == 16 else scales[1].clone())
+        dirty()
+        out = paged_attention(q, *pools, tables, starts, lengths, most_new, **kw)
+        given = paged_attention(q, *pools, tables, starts, lengths, most_new, out=torch.full_like(q, 3.0), **kw)
+        turned_given = paged_append(q, k, v, *[p.clone() for p in pools], tables, starts, lengths, most_new, freq=freq, k_scale=None if bits == 16 else scales[0].clone(),
+                                    v_scale=None if bits == 16 else scales[1].clone(), q_out=torch.full_like(q, 3.0))
+        return (turned, turned_given), (out, given)
+
+    def check(pairs, none):
+        for made, given in pairs:
+            assert not made[none].any() and bool((given[none] == 3.0).all())
+            assert torch.equal(made[~none], given[~none]) and bool(made[~none].isfinite().all())
+
+    none = torch.zeros(c.rows, dtype=torch.bool, device="cuda")
+    none[c.starts[-1]:] = True
+    check(both(tables, starts, lengths, most_new), none)
+    # the later sequences alone
+    none[:c.starts[1]] = True
+    check(both(tables[1:], starts[1:], lengths[1:], most_new), none)
+    # a sequence with fewer positions than new tokens is none
+    none[:c.starts[1]] = True
+    wrong = lengths.clone()
+    wrong[0] = new[0] - 1
+    check(both(tables, starts, wrong, most_new), none)
+    # fewer rows are announced than come
+    if most_new > 2:
+        few = most_new // 3
+        none = torch.zeros(c.rows, dtype=torch.bool, device="cuda")
+        none[c.starts[-1]:] = True
+        for first, n in zip(c.starts, new):
+            none[first + few:first + max(n, few)] = True
+        check(both(tables, starts, lengths, few), none)
+    # nothing is announced
+    check(both(tables, starts, lengths, 0), torch.ones_like(none))
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
