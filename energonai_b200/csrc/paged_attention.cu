@@ -525,6 +525,11 @@ template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParam
 }
 
 constexpr int kMostKeys = 8192, kLeastKeys = 256;
+// What the partial rows of a call may take: as many sequences as a call brings may be long, and the tables may address more than any of them is.
+// Fewer splits cost a long sequence among many more than the memory is worth (tables of 131072 positions, 32 heads on 8, 62 short sequences, one of
+// 100,000 keys and a prompt chunk: 276 MB unbounded and with 256 MB 362 us, with 128 MB 462, with 64 MB 706, without splits 1262; 40 heads of 128
+// sequences beside a chunk: 2762 MB 1411 us, with 256 MB, which leaves no splits, 1690).
+constexpr size_t kMostPartial = (size_t)256 << 20;
 // How the step form cuts a call: query rows per tile, tiles, keys per CTA, splits.
 struct StepPlan {
   int tiles8, row_tiles, chunk, splits;
@@ -538,7 +543,8 @@ StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, i
   const long long units = (long long)batch * kv_heads * s.row_tiles, sms = sm_count();
   // CTAs that are resident at a time, as the launch bounds have it.  From half of them on there are no splits, fewer are split to fill
   // them once.  No CTA gets more than kMostKeys keys (a long sequence among short ones would keep the call waiting) nor fewer
-  // than kLeastKeys.  Beside prompts, which take longer, there are splits only for the former.
+  // than kLeastKeys.  Beside prompts, whose launch follows this one, there are splits only for the former: the plan does not know how many of
+  // the sequences bring few rows.
   const long long slots = sms * (head_dim == 64 ? (s.tiles8 == 1 ? 4 : 3) : s.tiles8 == 1 ? (eight ? 4 : 3) : 2);
   const long long want = beside || 2 * units >= slots ? 1 : slots / units;
   keys += 15;                                               // (the first tile may begin in front of the first key)
@@ -546,6 +552,8 @@ StepPlan step_plan(int batch, int kv_heads, int rows_per_head, long long keys, i
   if (chunk > kMostKeys) chunk = kMostKeys;
   if (chunk < kLeastKeys) chunk = kLeastKeys;
   if (chunk < (keys + 511) / 512) chunk = (keys + 511) / 512;
+  const long long most = (long long)(kMostPartial / ((size_t)batch * kv_heads * s.row_tiles * 8 * s.tiles8 * (head_dim + 2) * sizeof(float)));
+  if (chunk * most < keys) chunk = most > 0 ? (keys + most - 1) / most : keys;
   chunk = (chunk + 63) / 64 * 64;
   s.splits = (int)((keys + chunk - 1) / chunk);
   s.chunk = (int)chunk;

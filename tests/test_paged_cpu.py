@@ -128,3 +128,14 @@ def test_the_cache_struct_matches_the_header(tmp_path):
 def test_unknown_flags_are_refused():
     for call in (append_call, attention_call):
         assert call(reserved=2) == -1 and "flag bits" in _lib.last_error()
+
+
+def test_scratch_is_bounded():
+    """However many sequences a call brings and whatever the tables address: prompts beside many sequences, and steps of very long tables."""
+    need = _lib.lib().eb_paged_attention_scratch_bytes
+    for batch, heads, kv_heads, most_new, reach in ((64, 32, 8, 1024, 131072), (128, 40, 40, 1024, 131072), (128, 40, 40, 1, 131072), (64, 40, 40, 1, 1 << 20), (1024, 8, 8, 3, 131072),
+                                                    (60000, 64, 8, 100, 1 << 24), (1, 128, 1, 1, (1 << 30) - 128)):
+        for dim in (64, 128):
+            # (the prompt form splits only what does not fill one wave)
+            assert need(batch, heads, kv_heads, dim, 1, most_new, reach, 0) <= (256 + 20) << 20, (batch, heads, kv_heads, most_new, reach)
+    assert need(1, 32, 8, 128, 1, 1, 131072, 0) > 0 and need(16, 32, 8, 128, 1, 100, 131072, 0) > 0
