@@ -21,6 +21,19 @@ namespace {
 
 // Value scales below 2^-100, 0 among them, count as 2^-100: 1 / scale and log2(scale) enter the softmax.
 constexpr float kLeastScale = 7.888609052210118e-31f;
+// The weights of a page are summed without its value scale z, 2^(s + log2 z - m) / z.  Where log2 z is so far below the reference m that
+// the power may fall out of fp32's range (pages of next to nothing beside huge ones), those that do are summed as 2^(s - m).  For the
+// same reason a sum is taken over to another reference in two halves of its exponent.
+constexpr float kFarBelow = 90.f, kLeastPower = -126.f;
+__device__ __forceinline__ float pow2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sum_at(float l, float by) {         // l 2^by
+  const float half = pow2(0.5f * by);
+  return l * half * half;
+}
 
 struct PagedRows {
   int row0, count, past, length, end;  // first row, rows (the announced ones), positions in front of them, positions in all, end of the sequence's rows

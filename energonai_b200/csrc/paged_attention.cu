@@ -53,11 +53,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ float pow2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 template <typename T> __device__ __forceinline__ void mma_tile(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if (std::is_same<T, __half>::value)
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -214,7 +209,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
     for (int e = 0; e < 2; ++e) row_pos[n][e] = t.past + (rt * kRowsT + n * 8 + 2 * c + e) / p.group;
   const int first_pos = t.past + rt * kRowsT / p.group, last_pos = t.past + (rt * kRowsT + t.rows - 1) / p.group;
 
-  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2];
+  float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2], far_below = -3.402823466e38f;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     m_ref[n][0] = m_ref[n][1] = -3.402823466e38f;
@@ -288,13 +283,23 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
           const float alpha = pow2(m_ref[n][e] - m);
+          l_run[n][e] = EIGHT ? sum_at(l_run[n][e], m_ref[n][e] - m) : l_run[n][e] * alpha;
           m_ref[n][e] = m;
-          l_run[n][e] *= alpha;
+          if (EIGHT) far_below = fmaxf(far_below, m - kFarBelow);
 #pragma unroll
           for (int k = 0; k < kTiles; ++k) {
             acc[n][k][e] *= alpha;
             acc[n][k][e + 2] *= alpha;
           }
+        }
+    }
+    if (EIGHT && __builtin_expect(v_log < far_below, 0)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = s[n][e] - (m_ref[n][e & 1] - kLift);
+          if (x < kLeastPower) l_run[n][e & 1] += pow2(x - v_log);
         }
     }
     uint32_t pf[NT][2], pl[NT][2];
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
 #pragma unroll
     for (int w = 0; w < kStepWarps; ++w) {
       const float a = pow2(red[w][row][D] - r.m);
-      r.l = fmaf(red[w][row][D + 1], a, r.l);
+      r.l = EIGHT ? r.l + sum_at(red[w][row][D + 1], red[w][row][D] - r.m) : fmaf(red[w][row][D + 1], a, r.l);
       r.x = fmaf(red[w][row][d], a, r.x);
       r.y = fmaf(red[w][row][d + 1], a, r.y);
     }
@@ -445,7 +450,7 @@ template <typename T, int D> __device__ __forceinline__ void merge_row(const flo
     const float *one = in + (long long)s * stride;
     const float2 ml = *reinterpret_cast<const float2 *>(one + D);
     const float a = pow2(ml.x - m);
-    l = fmaf(ml.y, a, l);
+    l += sum_at(ml.y, ml.x - m);
 #pragma unroll
     for (int e = 0; e < kPer; e += 2) {
       const float2 v = *reinterpret_cast<const float2 *>(one + lane * kPer + e);

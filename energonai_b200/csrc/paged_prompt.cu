@@ -437,8 +437,8 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (__any_sync(0xffffffffu, there && m > m_ref + kRaise)) {
         // The reference is raised, for all rows of the warp (tensor memory is read and written warp-wide), behind the last value product.
         const float m_new = fmaxf(m_ref, m), alpha = ex2(m_ref - m_new);
+        l_run = EIGHT ? sum_at(l_run, m_ref - m_new) : l_run * alpha;
         m_ref = m_new;
-        l_run *= alpha;
         if (at_half > 0) {
           if (!all_wait(my_pv_full + 8 * (buf ^ 1), ((at_half - 1) >> 1) & 1, 8)) { alive = false; break; }
           tc_fence_after();
@@ -471,6 +471,17 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           l_run = EIGHT ? fmaf(l0 + l1, value_inv[slot * 8 + 2 * (c0 + c) + h], l_run) : l_run + (l0 + l1);
         }
       };
+      if (EIGHT && __builtin_expect(fminf(fminf(logs[0], logs[1]), fminf(logs[2], logs[3])) < m_ref - kFarBelow, 0)) {
+        auto far = [&](const float (&x)[32], int c) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int g = 2 * c + e / 16;
+            if (logs[g] > kNone && fmaf(x[e], factors[g], logs[g] - (m_ref - kLift)) < kLeastPower) l_run += ex2(fmaf(x[e], factors[g], kLift - m_ref));
+          }
+        };
+        far(x0, 0);
+        far(x1, 1);
+      }
       weigh(x0, 0, w0);
       weigh(x1, 1, w1);
       tc_st16(t_s, w0);                                    // (over scores of this warp's own rows, which are in registers)

@@ -382,6 +382,22 @@ def test_rows_of_no_sequence_of_new_tensors_are_zeros(new, past, bits):
     check(both(tables, starts, lengths, 0), torch.ones_like(none))
 
 
+@pytest.mark.parametrize("least", [0.0, 2.0 ** -60, 2.0 ** -20])
+@pytest.mark.parametrize("most", [2.0 ** 20, 2.0 ** 50, 2.0 ** 90])
+def test_pages_of_tiny_values_beside_huge_ones(most, least):
+    """Every fifth page holds next to nothing, the others numbers far beyond fp16: the former keep their share of the weights."""
+    from energonai_b200.paged import paged_attention
+    c = Case([1, 70, 5, 2], [31, 0, 200, 9], 4, 2, 64, 16, BF16, 8, seed=3)
+    c.scale[1] *= most
+    for page in [p for t in c.tables for p in t[::5]]:
+        c.scale[1][page] = least
+        if not least:
+            codes = c.pool[1][page].view(torch.uint8)
+            codes[codes != 0x7f] = 0
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    close(paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), *c.attention(prompt=32))
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
