@@ -2,6 +2,8 @@
 // fp16 / fp32, and the limits that every page number passes before it becomes an address.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace eb {
@@ -79,6 +81,20 @@ __device__ __forceinline__ uint32_t floats_to_e4m3x2(float lo, float hi) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+// Whether one of the values in 16 bytes is not finite (T: the 16-bit type, or uint8_t for e4m3 codes).
+template <typename T> __device__ __forceinline__ bool any_not_finite(const uint4 &x) {
+  // (the exponent's ones, or a NaN code's, and one more carry into the sign's place)
+  constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x7c007c00u : std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7f7f7f7fu;
+  constexpr uint32_t kOne = kOnes & ~(kOnes << 1), kSigns = std::is_same<T, uint8_t>::value ? 0x80808080u : 0x80008000u;
+  return ((((x.x & kOnes) + kOne) | ((x.y & kOnes) + kOne) | ((x.z & kOnes) + kOne) | ((x.w & kOnes) + kOne)) & kSigns) != 0;
+}
+// The same bytes with zeros in the place of such values.
+template <typename T> __device__ __forceinline__ uint4 finite_only(const uint4 &x) {
+  constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x7c007c00u : std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7f7f7f7fu;
+  auto kept = [](uint32_t w) { return w & ~(std::is_same<T, uint8_t>::value ? __vcmpeq4(w & kOnes, kOnes) : __vcmpeq2(w & kOnes, kOnes)); };
+  return make_uint4(kept(x.x), kept(x.y), kept(x.z), kept(x.w));
 }
 
 // Host side of the checks that all entry points make of a packed batch.

@@ -78,12 +78,39 @@ __device__ __forceinline__ StepTile step_tile(const StepParams &p, const PagedRo
   t.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
   return t;
 }
+// whether one of the 16 keys from key0 on is seen by some only of the rows at the positions from `first` to `last`
+__device__ __forceinline__ bool step_hides(int first, int last, int key0, int window) { return key0 + 15 > first || (window > 0 && key0 <= last - window); }
 
-// T: type of queries and output; EIGHT: e4m3 pages; NT: tiles of 8 query rows
+// The values that are not finite of a warp's tiles (from key0 on, every kStepWarps-th), each added to the partial rows that see it; V: the values' type, or
+// uint8_t for codes.
+template <typename V> __device__ __noinline__ void add_not_finite(const PagedBatch batch, const uint8_t *values, long long page_bytes, int b, int key0, int hi, const StepTile t, int row0,
+                                                                  int group, int window, int dim, float *rows) {
+  constexpr bool kCodes = std::is_same<V, uint8_t>::value;
+  __syncwarp();
+  for (; key0 < hi; key0 += kStepWarps * 16) {
+    const int id = paged_page(batch, b, key0 >> batch.page_shift);
+    if (id < 0 || !step_hides(t.past + row0 / group, t.past + (row0 + t.rows - 1) / group, key0, window)) continue;
+    for (int key = max(key0, t.lo); key < min(key0 + 16, hi); ++key) {
+      const V *y = reinterpret_cast<const V *>(values + id * page_bytes) + (key & ((1 << batch.page_shift) - 1)) * dim;
+      for (int d = threadIdx.x & 31; d < dim; d += 32) {
+        float v;
+        if constexpr (kCodes) v = unpack2<__half>(e4m3x2_to_half2(y[d])).x;
+        else v = to_f32<V>(y[d]);
+        if (isfinite(v)) continue;
+        for (int row = 0; row < t.rows; ++row) {
+          const int pos = t.past + (row0 + row) / group;
+          if (key <= pos && (window == 0 || key > pos - window)) rows[row * (dim + 2) + d] += v;
+        }
+      }
+    }
+  }
+}
+
+// T: type of queries and output; EIGHT: e4m3 pages; NT: tiles of 8 query rows; SPREAD: a tile's rows may be at several positions
 template <bool EIGHT, int D, int NT> struct StepShape {
   static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : 3) : NT == 1 ? (EIGHT ? 4 : 3) : 2;      // resident per multiprocessor
 };
-template <typename T, bool EIGHT, int D, int NT, int STAGES>
+template <typename T, bool EIGHT, int D, int NT, int STAGES, bool SPREAD>
 __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCtas) paged_step_kernel(const StepParams p) {
   using M = typename std::conditional<EIGHT, __half, T>::type;           // operand type of the products
   constexpr bool kSplitP = std::is_same<M, __nv_bfloat16>::value;
@@ -208,6 +235,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
 #pragma unroll
     for (int e = 0; e < 2; ++e) row_pos[n][e] = t.past + (rt * kRowsT + n * 8 + 2 * c + e) / p.group;
   const int first_pos = t.past + rt * kRowsT / p.group, last_pos = t.past + (rt * kRowsT + t.rows - 1) / p.group;
+  using V = typename std::conditional<EIGHT, uint8_t, T>::type;
+  bool taken = false;                                                    // values that are not finite were taken out of a tile
 
   float acc[NT][kTiles][4], m_ref[NT][2], l_run[NT][2], far_below = -3.402823466e38f;
 #pragma unroll
@@ -233,6 +262,26 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
     request(i + STAGES - 1, id_of(i + STAGES - 1, i & ~31));
     if (id < 0) continue;                                  // (a page that is none: nothing to see)
     const uint8_t *tile = ring + (i % STAGES) * kTile;
+    // A weight of 0 does not hide a value that is not finite: tokens further on in the call, or keys that a window left behind, may hold such for rows
+    // that do not see them.  They leave the tile here, and are added behind the loop to the rows that do.  (In front of the scores, so that the
+    // values' loads need not wait for what is stored here.)
+    if (SPREAD && step_hides(first_pos, last_pos, key0, p.window)) {
+      bool found = false;
+#pragma unroll 1
+      for (int n = 0; n < kHalf / 512; ++n) {
+        const int key = key0 + (n * 32 + lane) / kChunks;
+        if (key < hi && key >= t.lo) found |= any_not_finite<V>(*reinterpret_cast<const uint4 *>(tile + kHalf + (n * 32 + lane) * 16));
+      }
+      if (__builtin_expect(__any_sync(0xffffffffu, found), 0)) {
+        taken = true;
+#pragma unroll 1
+        for (int n = 0; n < kHalf / 512; ++n) {
+          uint4 *x = reinterpret_cast<uint4 *>(ring + (i % STAGES) * kTile + kHalf + (n * 32 + lane) * 16);
+          *x = finite_only<V>(*x);
+        }
+        __syncwarp();
+      }
+    }
     // ---- scores ----
     float s[NT][4], s2[NT][4];                             // (two chains of dependent products)
 #pragma unroll
@@ -396,6 +445,8 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
         row[D + 1] = l;
       }
     }
+  if (SPREAD && __builtin_expect(taken, 0))
+    add_not_finite<V>(p.batch, vp + hk * block_bytes, p.kv_heads * block_bytes, b, lo + warp * 16, hi, t, rt * kRowsT, p.group, p.window, D, &red[warp][0][0]);
   __syncthreads();
   // two columns of a row, of this CTA's warps
   struct Sum {
@@ -508,12 +559,12 @@ template <typename T, int D> __global__ void __launch_bounds__(128) paged_prompt
                   reinterpret_cast<T *>(p.o) + (long long)(r.row0 + all / p.group) * p.ldo + (long long)(hk * p.group + all % p.group) * D);
 }
 
-template <typename T, bool EIGHT, int D, int NT> int launch_step(const StepParams &p, cudaStream_t st) {
+template <typename T, bool EIGHT, int D, int NT, bool SPREAD> int launch_step(const StepParams &p, cudaStream_t st) {
   constexpr int kTile = 16 * 2 * (EIGHT ? D : 2 * D), kRed = kStepWarps * 8 * NT * (D + 2) * 4;
   // (64 sequences of 2048 to 4095 keys in e4m3, heads of 128: 76 us with two tiles, 77 with three, 86 with four, which cost resident CTAs;
   // 32 of 1500, 16-bit heads of 64: 26, 23 and 23)
   constexpr int kStages = D == 64 ? 3 : 2, kSmem = kStepWarps * kStages * kTile > kRed ? kStepWarps * kStages * kTile : kRed;
-  auto kern = paged_step_kernel<T, EIGHT, D, NT, kStages>;
+  auto kern = paged_step_kernel<T, EIGHT, D, NT, kStages, SPREAD>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -650,7 +701,10 @@ extern "C" int eb_paged_attention(const eb_paged *cache, const void *q, long lon
   p.scale_log2 = scale * kLog2eStep; p.part = plan.step_bytes ? reinterpret_cast<float *>(scratch) : nullptr;
   cudaStream_t st = as_stream(stream);
   int rc;
-#define EB_STEP(T, E, D) (s.tiles8 == 1 ? launch_step<T, E, D, 1>(p, st) : launch_step<T, E, D, 2>(p, st))
+  // Single tokens take a kernel of their own: what rows at several positions need costs it 9 % (64 sequences of 2048 to 4095 keys in e4m3)
+#define EB_STEP(T, E, D)                                                                                      \
+  (most_new == 1 ? (s.tiles8 == 1 ? launch_step<T, E, D, 1, false>(p, st) : launch_step<T, E, D, 2, false>(p, st)) \
+                 : (s.tiles8 == 1 ? launch_step<T, E, D, 1, true>(p, st) : launch_step<T, E, D, 2, true>(p, st)))
 #define EB_STEP_D(T, E) (head_dim == 64 ? EB_STEP(T, E, 64) : EB_STEP(T, E, 128))
   if (dtype == EB_F16) rc = k_scale ? EB_STEP_D(__half, true) : EB_STEP_D(__half, false);
   else rc = k_scale ? EB_STEP_D(__nv_bfloat16, true) : EB_STEP_D(__nv_bfloat16, false);

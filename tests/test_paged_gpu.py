@@ -398,6 +398,55 @@ def test_pages_of_tiny_values_beside_huge_ones(most, least):
     close(paged_attention(q, *pools, tables, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), *c.attention(prompt=32))
 
 
+def check_values_that_are_not_finite(new, past, heads, kv_heads, dim, bits, dtype):
+    """Infinities and NaN among the values: not finite is what sees them, everything else is as without them; rows whose window has left them
+    behind too."""
+    from energonai_b200.paged import paged_attention
+    page = (16, 32, 64, 128)[(heads + len(new)) % 4]
+    c = Case(new, past, heads, kv_heads, dim, page, dtype, bits, seed=heads + sum(past))
+    r = torch.Generator().manual_seed(heads)
+    kinds = [float("inf"), float("-inf"), float("nan")]
+    bad = []                                                                # (sequence, position, key / value head, dimension, value)
+    for b, (n, p) in enumerate(zip(new, past)):
+        for at in {n + p - 1, p + n // 2, p + n // 3 + 1, max(0, p - 20)}:
+            if at < n + p:
+                bad.append((b, at, int(torch.randint(kv_heads, (1,), generator=r)), int(torch.randint(dim, (1,), generator=r)), kinds[len(bad) % 3]))
+    for b, at, h, d, value in bad:
+        place = (c.tables[b][at // page], h, at % page, d)
+        if bits == 8:
+            c.pool[1].view(torch.uint8)[place] = 0
+        else:
+            c.pool[1][place] = 0.0
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    for b, at, h, d, value in bad:
+        place = (c.tables[b][at // page], h, at % page, d)
+        if bits == 8:
+            pools[1].view(torch.uint8)[place] = 0x7f if value > 0 else 0xff
+        else:
+            pools[1][place] = value
+    group = heads // kv_heads
+    for window in (0, 25, 130):
+        want, tol = c.attention(window=window, prompt=64 * kv_heads // heads)
+        sees = torch.zeros(c.rows, heads, dim, dtype=torch.bool)
+        for b, at, h, d, _ in bad:
+            for i in range(new[b]):
+                pos = past[b] + i
+                if at <= pos and (not window or at > pos - window):
+                    sees[c.starts[b] + i, h * group:(h + 1) * group, d] = True
+        sees = sees.flatten(1)
+        got = paged_attention(q, *pools, tables, starts, lengths, most_new, max(c.length), window=window, k_scale=scales[0], v_scale=scales[1]).double().cpu()
+        assert torch.equal(got.isfinite(), ~sees), f"window {window}: {int((got.isfinite() == sees).sum())} of {got.numel()}"
+        assert bool(((got - want).abs()[~sees] <= tol[~sees]).all()), f"window {window}"
+
+
+@pytest.mark.parametrize("dtype,bits", [(F16, 16), (BF16, 16), (F16, 8), (BF16, 8)])
+@pytest.mark.parametrize("new,past", [([5, 3], [40, 0]), ([9, 1, 2], [250, 30, 100]), ([7], [700]), ([3, 8], [5000, 0])])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (8, 2, 128), (6, 2, 128), (7, 1, 64)])
+def test_values_that_are_not_finite_reach_no_token_in_front_of_them(new, past, heads, kv_heads, dim, bits, dtype):
+    check_values_that_are_not_finite(new, past, heads, kv_heads, dim, bits, dtype)
+
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
