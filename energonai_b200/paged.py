@@ -169,7 +169,8 @@ def _scratch_bytes(*sizes):
 def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most_length=None, scale=None, window=0, k_scale=None, v_scale=None, out=None):
     """Causal attention of the new tokens q [rows, heads*head_dim] over their sequences' pages, which hold the new keys and values
     already: single tokens, a few per sequence, prompts and chunks of prompts, or all of them in one batch.  window > 0:
-    the row at position p sees the positions above p - window only.  most_length: no sequence is longer (None: what the
+    the row at position p sees the positions above p - window only.  What a row does not see may hold anything, a value that is not finite makes
+    what sees it infinite or NaN.  most_length: no sequence is longer (None: what the
     tables address).  Returns out [rows, heads*head_dim], which may be q.  Rows of no sequence, and those behind a sequence's first most_new,
     are left as they are in an out that is given, and zeros in a new tensor."""
     device = _one_device("paged_attention", q, k_pages, v_pages, tables, starts, lengths, k_scale, v_scale, out)

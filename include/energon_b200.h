@@ -926,7 +926,8 @@ EB_API int eb_paged_append(const eb_paged *cache, const void *q, long long ldq, 
                     long long ldo, int rows, int heads, const float *freq, int pairs, void *stream);
 
 /* Causal attention of the new tokens over the cache (which holds them already): the row at position p sees the positions
- * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros.  `out` may be q.  Slots that no row sees may hold anything.
+ * up to p, with a window > 0 those above p - window.  A row that sees nothing gives zeros.  `out` may be q.  Slots that a row does not see
+ * may hold anything; a value that is not finite makes what sees it infinite or NaN.
  * scratch: eb_paged_attention_scratch_bytes(...) bytes, 16-byte aligned, of any content; calls that may overlap on the
  * device need scratch of their own. */
 EB_API int eb_paged_attention(const eb_paged *cache, const void *q, long long ldq, void *out, long long ldo, int rows, int heads, int window, float scale,

@@ -447,6 +447,16 @@ def test_values_that_are_not_finite_reach_no_token_in_front_of_them(new, past, h
 
 
 
+@pytest.mark.parametrize("dtype,bits", [(F16, 16), (BF16, 16), (F16, 8), (BF16, 8)])
+@pytest.mark.parametrize("new,past", [([100], [0]), ([300, 70, 129], [77, 512, 0]), ([257, 1, 90], [3000, 200, 1]), ([600], [130])])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(2, 2, 64), (8, 2, 128), (6, 2, 128), (7, 1, 64)])
+def test_values_that_are_not_finite_reach_no_row_of_a_prompt_in_front_of_them(new, past, heads, kv_heads, dim, bits, dtype):
+    from energonai_b200.gemm import device_status
+    check_values_that_are_not_finite(new, past, heads, kv_heads, dim, bits, dtype)
+    assert device_status()[0] == 0
+
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
