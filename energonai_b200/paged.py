@@ -102,6 +102,8 @@ def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_sc
     if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
         raise RuntimeError(f"{what}: pools are contiguous [pages, kv_heads, page_size, head_dim], alike for keys and values")
     pages, kv_heads, page_size, head_dim = shape
+    if not 0 < pages < 1 << 31 or not 0 < kv_heads < 1 << 31 or page_size not in PAGE_SIZES or head_dim not in HEAD_DIMS:
+        raise RuntimeError(f"{what}: pools of pages of {PAGE_SIZES} positions and heads of {HEAD_DIMS} required, not {tuple(shape)}")
     if k_scale is None and v_scale is None:
         held, ks, vs = dtype, 0, 0
     else:
@@ -124,6 +126,10 @@ def _cache(what, dtype, k_pages, v_pages, tables, starts, lengths, k_scale, v_sc
     if batch == 0 or cols == 0 or (one != 1 and cols > 1) or ld < cols:
         raise RuntimeError(f"{what}: int32 tables of one or more rows of contiguous columns required")
     reach = cols * page_size
+    if reach >= 1 << 30 or batch >= 1 << 16:
+        raise RuntimeError(f"{what}: a batch of {batch} sequences whose tables address {reach} positions exceeds 65535, or 2^30")
+    if not 0 <= int(most_new) or (most_length is not None and not 0 <= int(most_length)):
+        raise RuntimeError(f"{what}: negative limits (most_new {most_new}, most_length {most_length})")
     most_length = reach if most_length is None else min(int(most_length), reach)
     return kv_heads, head_dim, most_length, _paged.pack(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, tables.data_ptr(), starts.data_ptr(), lengths.data_ptr(), ld, pages,
                                                         page_size, kv_heads, head_dim, cols, batch, min(int(most_new), (1 << 31) - 1), most_length, dtype_code(dtype), 1 if clear else 0)
@@ -189,6 +195,8 @@ def paged_attention(q, k_pages, v_pages, tables, starts, lengths, most_new, most
         if out.shape[0] != rows:
             raise RuntimeError("paged_attention: one row of out per row of q")
     window = int(window)
+    if window < 0:
+        raise RuntimeError(f"paged_attention: a window of {window} positions")
     if window >= most_length:
         window = 0                                          # (every key is inside)
     nbytes = _scratch_bytes(tables.shape[0], heads, kv_heads, head_dim, k_scale is not None, min(int(most_new), rows), most_length, window)

@@ -139,3 +139,21 @@ def test_scratch_is_bounded():
             # (the prompt form splits only what does not fill one wave)
             assert need(batch, heads, kv_heads, dim, 1, most_new, reach, 0) <= (256 + 20) << 20, (batch, heads, kv_heads, most_new, reach)
     assert need(1, 32, 8, 128, 1, 1, 131072, 0) > 0 and need(16, 32, 8, 128, 1, 100, 131072, 0) > 0
+
+
+def test_sizes_that_no_call_takes_are_refused_by_name():
+    """... and not by whatever they break on the way to the kernels."""
+    from energonai_b200.paged import _cache
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    pools = lambda *shape: [torch.zeros(shape, dtype=torch.float16) for _ in range(2)]
+
+    def call(pool=(3, 2, 16, 64), cols=2, batch=1, most_new=1, most_length=None):
+        k, v = pools(*pool)
+        return _cache("it", torch.float16, k, v, torch.empty((batch, cols), dtype=torch.int32), i32(batch + 1), i32(batch), None, None, most_new, most_length, False)
+
+    assert call()[:3] == (2, 64, 32)
+    for bad, words in ((dict(pool=(3, 0, 16, 64)), "pools of pages"), (dict(pool=(0, 2, 16, 64)), "pools of pages"), (dict(pool=(3, 2, 24, 64)), "pools of pages"),
+                       (dict(pool=(3, 2, 16, 80)), "pools of pages"), (dict(cols=1 << 26), "2\\^30"), (dict(batch=1 << 16), "65535"), (dict(most_new=-1), "negative"),
+                       (dict(most_length=-5), "negative"), (dict(cols=0), "one or more rows")):
+        with pytest.raises(RuntimeError, match=words):
+            call(**bad)
