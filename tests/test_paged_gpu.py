@@ -457,6 +457,50 @@ def test_values_that_are_not_finite_reach_no_row_of_a_prompt_in_front_of_them(ne
 
 
 
+@pytest.mark.parametrize("dtype,bits", [(F16, 16), (BF16, 16), (F16, 8), (BF16, 8)])
+@pytest.mark.parametrize("new,past,heads,kv_heads", [([1, 80], [20000, 40], 8, 2), ([1, 3, 70], [9000, 17000, 6000], 4, 4), ([100, 1], [30000, 8400], 2, 1)])
+def test_split_sequences_beside_prompts(new, past, heads, kv_heads, dtype, bits):
+    """Both kernels cut keys over CTAs in one call: their partial rows share the call's scratch."""
+    from energonai_b200 import _lib
+    from energonai_b200.paged import paged_attention
+    c = Case(new, past, heads, kv_heads, 64, 64, dtype, bits, seed=17)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    kw = dict(k_scale=scales[0], v_scale=scales[1])
+    assert _lib.lib().eb_paged_attention_scratch_bytes(len(new), heads, kv_heads, 64, int(bits == 8), most_new, tables.shape[1] * 64, 0) > 0
+    want, tol = c.attention(prompt=64 * kv_heads // heads)
+    graph = torch.cuda.CUDAGraph()
+    close(paged_attention(q, *pools, tables, starts, lengths, most_new, **kw), want, tol)
+    with torch.cuda.graph(graph):
+        out = paged_attention(q, *pools, tables, starts, lengths, most_new, **kw)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(paged_attention(q, *pools, tables, starts, lengths, most_new, **kw))
+        graph.replay()
+    torch.cuda.synchronize()
+    close(out, want, tol)
+    assert all(torch.equal(x, out) for g in got for x in g)
+
+
+def test_partial_rows_of_wide_tables():
+    """Tables that address so much more than the sequences hold that the partial rows reach their bound: a CTA takes more keys then."""
+    from energonai_b200 import _lib
+    from energonai_b200.paged import paged_attention
+    past = [30 + 7 * b for b in range(60)] + [9000, 20000, 8193, 5]
+    c = Case([1] * 62 + [20, 3], past, 8, 2, 64, 16, BF16, 8, seed=23)
+    (q, _, _), pools, scales, (tables, starts, lengths, most_new) = c.device()
+    need = lambda cols: _lib.lib().eb_paged_attention_scratch_bytes(64, 8, 2, 64, 1, most_new, cols * 16, 0)
+    want, tol = c.attention(prompt=16)
+    for cols in (tables.shape[1], 1 << 16, 1 << 20):                         # (6 MB of them, and what 256 MB hold)
+        wide = torch.full((64, cols), -1, dtype=torch.int32, device="cuda")
+        wide[:, :tables.shape[1]] = tables
+        assert 0 < need(cols) <= 276 << 20
+        close(paged_attention(q, *pools, wide, starts, lengths, most_new, k_scale=scales[0], v_scale=scales[1]), want, tol, f"{cols} columns")
+
+
+
 def test_replay_with_other_lengths():
     """A captured step (append, attention) is replayed as sequences grow, from page to page; two captured steps share nothing."""
     from energonai_b200.paged import page_pools, paged_append, paged_attention
