@@ -169,12 +169,23 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
   // A weight of 0 does not hide a value that is not finite: later tokens of the call, or keys that a window has left behind, may hold such for rows that do
   // not see them.  Where a tile hides keys from some of the CTA's rows (three tiles at either end at most), such values leave it, and are added at
-  // the end to the rows that see them.  (2 % of long prompts, 5 % of e4m3 ones of three to seven tiles.)
+  // the end to the rows that see them.  (2 % of 16-bit prompts, 5 % of e4m3 ones of
+  // three to seven tiles.)
   auto hides = [&](int j) { return j >= (int)bad[1] || j * kKeys <= (int)bad[3]; };
   auto bad_of = [&](int j) { return 4 + 4 * (j >= (int)bad[1] ? j - (int)bad[1] : 4 + j - (int)bad[2]); };
   auto is_bad = [&](int j, int row) {
     atomicOr(const_cast<uint32_t *>(bad) + bad_of(j) + (row >> 5), 1u << (row & 31));
     bad[0] = 1;
+  };
+  // (by a warp, of a tile of values; two may find and write the same)
+  constexpr int kChunks = kKeys * kSub * 8;
+  auto take_out = [&](uint4 *tile, int j) {
+#pragma unroll 1
+    for (int e = lane; e < kChunks; e += 32)
+      if (any_not_finite<M>(tile[e])) {
+        tile[e] = finite_only<M>(tile[e]);
+        is_bad(j, (e >> 3) % kKeys);
+      }
   };
   if (threadIdx.x < 36) {
     const int first_pos = r.past + q0 / p.group, last_pos = r.past + (min(q0 + kCtaRows, all) - 1) / p.group;
@@ -291,7 +302,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int i = j - jmin, ks = i % kKStages, vs = i % kVStages;
       if (!all_wait(k_full + 8 * ks, (i / kKStages) & 1, 3)) return false;
       if (lane == 0) bar_arrive(k_empty + 8 * ks);
-      if (!all_wait(v_ready + 8 * vs, (i / kVStages) & 1, 10)) return false;
+      if (!all_wait((EIGHT ? v_full : v_ready) + 8 * vs, (i / kVStages) & 1, 10)) return false;
       if (lane == 0) bar_arrive(v_empty + 8 * vs);
       return true;
     };
@@ -315,7 +326,15 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       ok = ok && all_wait(q_full, 0, 2) && issue_scores(first) && (first + 1 == end || issue_scores(first + 1));
       for (int n = first; n < end && ok; ++n) {
         const int at = n - first, buf = at & 1, j = n >> 1, i = j - jmin, vs = i % kVStages;
-        ok = all_wait(p_full + 8 * (2 * t + buf), (at >> 1) & 1, 5) && all_wait(v_ready + 8 * vs, (i / kVStages) & 1, 10);
+        if (EIGHT && ((n & 1) == 0 || n == first)) {
+          if (!(ok = all_wait(v_full + 8 * vs, (i / kVStages) & 1, 10))) break;
+          if (__any_sync(0xffffffffu, bad[0]) && hides(j)) {
+            take_out(reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes), j);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+          }
+        }
+        ok = all_wait(p_full + 8 * (2 * t + buf), (at >> 1) & 1, 5) && (EIGHT || all_wait(v_ready + 8 * vs, (i / kVStages) & 1, 10));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -331,41 +350,32 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       }
     }
     for (int j = max((end + 1) / 2, jmin); j < nmax && ok; ++j) ok = pass(j);
-  } else if (warp == kLookWarp) {
-    // ---------------- a look at the values of a tile, on their way to the products ----------------
+  } else if (!EIGHT && warp == kLookWarp) {
+    // ---------------- a look at the 16-bit values of a tile, on their way to the products ----------------
     // (By a warp of its own: the issuing warps, at the same work, took 194 us for the prompts that take 184 so.)
     bool ok = true;
     for (int j = jmin; j < nmax && ok; ++j) {
       const int i = j - jmin, vs = i % kVStages;
       if (!(ok = all_wait(v_full + 8 * vs, (i / kVStages) & 1, 12))) break;
-      const bool edge = !EIGHT && (j * kKeys < lo || (j + 1) * kKeys > hi);
-      if (__any_sync(0xffffffffu, EIGHT ? bad[0] && hides(j) : edge || hides(j))) {
+      const bool edge = j * kKeys < lo || (j + 1) * kKeys > hi;
+      if (edge || hides(j)) {
         uint4 *tile = reinterpret_cast<uint4 *>(v_ptr + vs * kKBytes);
-        constexpr int kChunks = kKeys * kSub * 8, kBatch = 8;
-        bool found = EIGHT;                                // (the converting warps have looked)
-        if constexpr (!EIGHT) {
-          if (edge)                                        // value rows that no row sees may hold anything
-            for (int e = lane; e < kChunks; e += 32) {
-              const int key = j * kKeys + (e >> 3) % kKeys;
-              if (key < lo || key >= hi) tile[e] = make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll 1
-          for (int e = lane; e < kChunks; e += 32 * kBatch) {
-            uint4 x[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) x[u] = tile[e + u * 32];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) found |= any_not_finite<M>(x[u]);
+        constexpr int kBatch = 8;
+        if (edge)                                          // value rows that no row sees may hold anything
+          for (int e = lane; e < kChunks; e += 32) {
+            const int key = j * kKeys + (e >> 3) % kKeys;
+            if (key < lo || key >= hi) tile[e] = make_uint4(0, 0, 0, 0);
           }
-        }
-        if (__any_sync(0xffffffffu, found)) {
+        bool found = false;
 #pragma unroll 1
-          for (int e = lane; e < kChunks; e += 32)
-            if (any_not_finite<M>(tile[e])) {
-              tile[e] = finite_only<M>(tile[e]);
-              is_bad(j, (e >> 3) % kKeys);
-            }
+        for (int e = lane; e < kChunks; e += 32 * kBatch) {
+          uint4 x[kBatch];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) x[u] = tile[e + u * 32];
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) found |= any_not_finite<M>(x[u]);
         }
+        if (__any_sync(0xffffffffu, found)) take_out(tile, j);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
@@ -575,7 +585,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       if (walked && bad[0]) {
         const int page_mask = (1 << p.batch.page_shift) - 1;
 #pragma unroll 1
-        for (int j = jmin; j < nmax; ++j) {
+        for (int j = first_half / 2; j < (end_half + 1) / 2; ++j) {
           if (!hides(j)) continue;
 #pragma unroll 1
           for (int key = max(j * kKeys, vis_begin); key < min((j + 1) * kKeys, vis_end); ++key) {
@@ -686,7 +696,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           bool found = false;
 #pragma unroll
           for (int e = 0; e < kLoads; ++e) found |= any_not_finite<uint8_t>(vbuf[e]);
-          if (found) bad[0] = 1;                           // (the looking warp's cue)
+          if (found) bad[0] = 1;                           // (the issuing warps' cue)
         }
         store(v_ptr + vs * kKBytes, vbuf);
         if (lane == 0) bar_arrive(v_full + 8 * vs);
