@@ -1,6 +1,7 @@
 // Attention of few new tokens per sequence over a paged cache (generation steps, draft tokens): one pass over the keys and
-// values, 16-bit or e4m3 codes with a scale for each page and head.  Bound by memory: a cached byte is read
-// once per key / value head and serves all query heads that share it.
+// values, 16-bit or e4m3 codes with a scale for each page and head.  Bound by memory: a cached byte is asked for
+// once per key / value head and tile of 8 or 16 query rows (token, head of the group); up to one tile that is once for all heads that share it, 17 to 24
+// rows are three tiles, of which the second-level cache serves two.
 //
 // Both products are mma.sync tiles with the cached rows on the long side: S^T = K Q^T (16 keys x 8 query rows) and
 // O^T += V^T P^T (16 dimensions x 8 query rows), so that 8 query rows (token, head of the group) fill a tile.  A warp takes
@@ -8,7 +9,7 @@
 // barrier between warps, 16 warps per multiprocessor).  The contraction of S runs over dimensions in any order and that of O
 // over keys in any order, so each lane reads 16 bytes where they lie, as the fragments of the products need them, and the queries
 // are laid out to match; the chunks are swizzled so that these reads meet in no bank.  P^T comes from S^T by an 8 x 8
-// transpose within the warp.  Tried and slower, for 64 sequences of 2048 to 4095 keys in e4m3, 8 heads of 128 (76 us): keys and values straight to
+// transpose within the warp.  Tried and slower, for 64 sequences of 2048 to 4095 keys in e4m3, 8 heads of 128 (76 us then, 81 now): keys and values straight to
 // registers, one tile ahead (88 us); bulk copies into unswizzled rings, twice as deep with 12 warps (93 us).
 //
 // e4m3 codes become fp16 (exact), whatever the model's type: queries of bf16 models go to fp16 with a power of two per
@@ -18,7 +19,7 @@
 // The reference m of a row is raised only when a score exceeds it by 2^8 (one vote per tile instead of a reduction); fp16
 // weights are 2^6 times as large, up to 2^14, which leaves fewer of them below fp16's normal range.
 // Weights of bf16 caches are split into two bf16 pieces, which costs tensor time that is there and keeps
-// the result within its own rounding; fp16 weights are rounded once.
+// the result within its own rounding; fp16 weights (of fp16 caches and of codes) are rounded once, 2^-11.
 //
 // Keys are split over CTAs by a fixed number of keys per CTA (short sequences then take fewer CTAs), the warps of a
 // CTA take every fourth tile; partial rows are merged in order, across CTAs by a second launch.

@@ -19,13 +19,16 @@
 // differ in magnitude.  Both are one fused multiply-add per score, as without scales.
 //
 // bf16 weights over 16-bit pages are rounded once (2^-8 of a weight, which averages out over keys): in two pieces, as in the
-// few-token kernel, the second product would take twice as long.
+// few-token kernel, the second product would take twice as long.  fp16 weights (of fp16 models and of codes) are rounded once, 2^-11.
+//
+// Values that are not finite are taken out of tiles that hide keys from some rows: 16-bit pages by warp 3, which looks at such tiles between the
+// copies and the products, codes by the issuing warps, on the cue of the warps that convert them.
 //
 // Bound by the chain scores -> softmax -> weights of a row tile: 2100 cycles per 64 keys and pair of row tiles, of which the special-function unit
-// is busy 1024 and the tensor core 1280 (1000 to 1500 tokens behind 3700 to 7000 cached ones, e4m3, 32 heads on 8: 277 us, 830 TFLOP/s).
-// Tried and not kept: weights through shared memory, 311 us; weights in columns of their own, scores handed back before the softmax, 289 us; a part of
+// is busy 1024 and the tensor core 1280 (531 to 1024 tokens behind 3700 to 7000 cached ones, e4m3, 32 heads on 8: 280 us, 825 TFLOP/s).
+// Tried and not kept, when that took 277 us: weights through shared memory, 311 us; weights in columns of their own, scores handed back before the softmax, 289 us; a part of
 // the powers of two by multiply-adds (1 to 3 of 8), 290 to 300 us; halves that the mask hides skipped one by one, 296 us; two sets of softmax warps that take halves in turn, 415 us; converting with two warps instead
-// of four, twice as long.  Over 16-bit pages of 64 positions the same takes 330 us: twice the bytes through the second-level cache.
+// of four, twice as long.  Over 16-bit pages of 64 positions the same took 330 us: twice the bytes through the second-level cache.
 // Few rows behind a long past do not fill the machine: the key tiles are then split over CTAs, whose rows are merged by
 // a second launch.
 //
@@ -169,8 +172,7 @@ paged_prompt_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 
   // A weight of 0 does not hide a value that is not finite: later tokens of the call, or keys that a window has left behind, may hold such for rows that do
   // not see them.  Where a tile hides keys from some of the CTA's rows (three tiles at either end at most), such values leave it, and are added at
-  // the end to the rows that see them.  (2 % of 16-bit prompts, 5 % of e4m3 ones of
-  // three to seven tiles.)
+  // the end to the rows that see them.  (2 % of the time of 16-bit prompts, 5 % of that of e4m3 ones of three to seven tiles.)
   auto hides = [&](int j) { return j >= (int)bad[1] || j * kKeys <= (int)bad[3]; };
   auto bad_of = [&](int j) { return 4 + 4 * (j >= (int)bad[1] ? j - (int)bad[1] : 4 + j - (int)bad[2]); };
   auto is_bad = [&](int j, int row) {
