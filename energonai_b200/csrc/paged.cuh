@@ -50,20 +50,25 @@ __device__ __forceinline__ PagedRows paged_rows(const PagedBatch &p, int b) {
   if (r.past < 0 || r.count < 0) r.count = 0;          // (no such sequence)
   return r;
 }
-// Zeros to the rows of `out` (columns `col` to `col + cols`, a multiple of 8) that no sequence serves: those behind the announced ones of
-// sequence b (all of one that is none), in front of the first sequence and behind the last.  By `threads` threads, this one number `thread`.
-template <typename T> __device__ __forceinline__ void paged_clear(const PagedBatch &p, const PagedRows &r, int b, T *out, long long ld, int col, int cols, int thread, int threads) {
-  const bool front = b == 0 && r.row0 > 0, behind = b == p.batch - 1 && r.end < p.rows;
-  if (__builtin_expect(!(front || behind || r.row0 + r.count < r.end), 1)) return;
+// Zeros to rows `from` to `to` of `out` (columns `col` to `col + cols`, a multiple of 8), by `threads` threads, this one number `thread`.
+template <typename T> __device__ __forceinline__ void paged_zeros(T *out, long long ld, int from, int to, int col, int cols, long long thread, long long threads) {
   const int per = cols / 8;
-  auto clear = [&](int from, int to) {
 #pragma unroll 1
-    for (long long i = thread; i < (long long)(to - from) * per; i += threads)
-      *reinterpret_cast<uint4 *>(out + (from + i / per) * ld + col + i % per * 8) = make_uint4(0, 0, 0, 0);
-  };
-  clear(r.row0 + r.count, r.end);
-  if (front) clear(0, min(r.row0, p.rows));
-  if (behind) clear(max(r.end, 0), p.rows);
+  for (long long i = thread; i < (long long)(to - from) * per; i += threads)
+    *reinterpret_cast<uint4 *>(out + (from + i / per) * ld + col + i % per * 8) = make_uint4(0, 0, 0, 0);
+}
+// The rows that no sequence serves: those of a sequence behind its announced ones (all, of one that is none) ...
+template <typename T> __device__ __forceinline__ void paged_clear(const PagedRows &r, T *out, long long ld, int col, int cols, int thread, int threads) {
+  if (__builtin_expect(r.row0 + r.count < r.end, 0)) paged_zeros(out, ld, r.row0 + r.count, r.end, col, cols, thread, threads);
+}
+// ... and those in front of the first sequence and behind the last, by the whole grid (a padded batch may have many).
+template <typename T> __device__ __forceinline__ void paged_clear_ends(const PagedBatch &p, T *out, long long ld, int cols) {
+  const int front = min(max(p.starts[0], 0), p.rows), behind = min(max(p.starts[p.batch], 0), p.rows);
+  if (__builtin_expect(front == 0 && behind == p.rows, 1)) return;
+  const long long cta = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, thread = cta * blockDim.x + threadIdx.x,
+                  threads = (long long)gridDim.x * gridDim.y * gridDim.z * blockDim.x;
+  paged_zeros(out, ld, 0, front, 0, cols, thread, threads);
+  paged_zeros(out, ld, behind, p.rows, 0, cols, thread, threads);
 }
 __device__ __forceinline__ int paged_page(const PagedBatch &p, int b, int at) {   // page of table entry `at`, or -1
   if (at < 0 || at >= p.table_cols) return -1;

@@ -62,8 +62,10 @@ template <typename T, bool EIGHT, int D> __global__ void __launch_bounds__(kAppe
   const int b = blockIdx.z, part = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int page_size = 1 << p.batch.page_shift;
   const PagedRows r = paged_rows(p.batch, b);
-  if (p.batch.clear && p.q_out && blockIdx.x == 0)
-    paged_clear(p.batch, r, b, reinterpret_cast<T *>(p.q_out), p.ldo, 0, p.heads * D, part * kAppendThreads + threadIdx.x, p.parts * kAppendThreads);
+  if (p.batch.clear && p.q_out) {
+    paged_clear_ends(p.batch, reinterpret_cast<T *>(p.q_out), p.ldo, p.heads * D);
+    if (blockIdx.x == 0) paged_clear(r, reinterpret_cast<T *>(p.q_out), p.ldo, 0, p.heads * D, part * kAppendThreads + threadIdx.x, p.parts * kAppendThreads);
+  }
   const int at = (r.past >> p.batch.page_shift) + blockIdx.x, begin = max(at << p.batch.page_shift, r.past), end = min((at + 1) << p.batch.page_shift, r.past + r.count);
   if (begin >= end) return;
   const int n = end - begin, slot0 = begin & (page_size - 1), row0 = r.row0 + begin - r.past;

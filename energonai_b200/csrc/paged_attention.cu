@@ -126,8 +126,10 @@ __global__ void __launch_bounds__(kStepWarps * 32, StepShape<EIGHT, D, NT>::kCta
   const int split = blockIdx.x, hk = blockIdx.y / p.row_tiles, rt = blockIdx.y % p.row_tiles, b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const PagedRows r = paged_rows(p.batch, b);
-  if (p.batch.clear && split == 0 && rt == 0)
-    paged_clear(p.batch, r, b, reinterpret_cast<T *>(p.o), p.ldo, hk * p.group * D, p.group * D, threadIdx.x, kStepWarps * 32);
+  if (p.batch.clear) {
+    paged_clear_ends(p.batch, reinterpret_cast<T *>(p.o), p.ldo, p.kv_heads * p.group * D);
+    if (split == 0 && rt == 0) paged_clear(r, reinterpret_cast<T *>(p.o), p.ldo, hk * p.group * D, p.group * D, threadIdx.x, kStepWarps * 32);
+  }
   if (r.count * p.group > p.few || rt * kRowsT >= r.count * p.group) return;
   const StepTile t = step_tile(p, r, rt, kRowsT);
   const int lo = (t.lo & ~15) + split * p.chunk, hi = split == p.splits - 1 ? t.hi : min(t.hi, lo + p.chunk);
