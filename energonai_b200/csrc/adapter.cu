@@ -60,16 +60,15 @@ template <typename T> __device__ __forceinline__ int lift_of(float m) {
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((127 + e) << 23); }
 __device__ __forceinline__ float largest_of(const float4 &v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
 
-// Rows and adapter of sequence b, which serves `live` of them, the announced ones; b = batch and batch + 1: the rows behind the last
-// sequence and in front of the first, without one.
+// Rows and adapter of sequence b, which serves `live` of them, the announced ones.
 struct AdapterRows {
   int row0, count, live, adapter;
 };
 __device__ __forceinline__ AdapterRows adapter_rows(const AdapterParams &p, int b) {
   AdapterRows r;
-  r.row0 = b > p.batch ? 0 : min(max(p.starts[b], 0), p.rows);
-  r.count = (b == p.batch ? p.rows : min(p.starts[b > p.batch ? 0 : b + 1], p.rows)) - r.row0;
-  r.adapter = b < p.batch ? p.index[b] : -1;
+  r.row0 = min(max(p.starts[b], 0), p.rows);
+  r.count = min(p.starts[b + 1], p.rows) - r.row0;
+  r.adapter = p.index[b];
   if (r.adapter >= p.count) r.adapter = -1;
   r.live = r.adapter < 0 ? 0 : min(r.count, p.most_new);
   return r;
@@ -223,16 +222,33 @@ template <bool ADD> struct BaseRow {
   }
 };
 
+// The rows in front of the first sequence and behind the last, by the whole grid: a padded batch may have many.
+template <typename T, bool ADD> __device__ __forceinline__ void adapter_ends(const AdapterParams &p) {
+  const int front = min(max(p.starts[0], 0), p.rows), behind = min(max(p.starts[p.batch], 0), p.rows);
+  if (__builtin_expect(front == 0 && behind == p.rows, 1)) return;
+  const int per = p.columns / 8;
+  const long long cta = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x, thread = cta * blockDim.x + threadIdx.x,
+                  threads = (long long)gridDim.x * gridDim.y * gridDim.z * blockDim.x;
+#pragma unroll 1
+  for (long long i = thread; i < (long long)(front + p.rows - behind) * per; i += threads) {
+    const long long at = i / per, row = at < front ? at : at - front + behind, col = i % per * 8;
+    BaseRow<ADD> y;
+    y.load(ADD ? p.base + row * p.ldbase + col : nullptr, true);
+    *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(p.delta) + row * p.ldd + col) = y.template alone<T>();
+  }
+}
+
 // delta[row][n] = s sum_r low[row][r] B[n][r] (ADD: + base[row][n]), 16 rows of a sequence, the warps take turns over the columns.  KR: steps
 // of 16 ranks.
 template <typename T, int KR, bool ADD> __global__ void __launch_bounds__(kAdapterWarps * 32) adapter_delta_kernel(const AdapterParams p) {
   griddep_wait();
   griddep_launch();
   const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  adapter_ends<T, ADD>(p);
   const AdapterRows r = adapter_rows(p, b);
   const int begin = blockIdx.y * p.chunk, end = min(p.columns, begin + p.chunk), first = begin + warp * 32, step = kAdapterWarps * 32;
   T *delta = reinterpret_cast<T *>(p.delta);
-  // (the rows behind the last sequence may be more than the grid has tiles for)
+  // (a sequence may bring more rows than the grid has tiles for)
   for (int t0 = blockIdx.x * kRowTile; t0 < r.count; t0 += gridDim.x * kRowTile) {
     const int rows = min(kRowTile, r.count - t0), live = min(rows, r.live - t0), row0 = r.row0 + t0;
     T *out0 = delta + (long long)(row0 + g) * p.ldd + c * 8, *out1 = out0 + 8 * p.ldd;
@@ -335,6 +351,7 @@ template <typename T, int KR, bool ADD> __global__ void __launch_bounds__(kAdapt
   griddep_wait();
   griddep_launch();
   const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  adapter_ends<T, ADD>(p);
   const AdapterRows r = adapter_rows(p, b);
   const int begin = blockIdx.y * p.chunk, end = min(p.columns, begin + p.chunk), steps = (end - begin + kDeltaCols - 1) / kDeltaCols;
   const uint32_t base = smem_u32(delta_smem);
@@ -513,7 +530,7 @@ template <typename T, int KR, bool ADD> int launch_delta(AdapterParams p, const 
   const int parts = (int)(want < turns ? want : turns);
   p.chunk = (turns + parts - 1) / parts * kDeltaCols;
   static_assert(kDeltaCols == kAdapterWarps * 32, "a turn of either form");
-  const dim3 grid(s.tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch + 2), block(kAdapterWarps * 32);
+  const dim3 grid(s.tiles, (p.columns + p.chunk - 1) / p.chunk, p.batch), block(kAdapterWarps * 32);
   if (!s.many) {
     launch_pdl(adapter_delta_kernel<T, KR, ADD>, grid, block, 0, st, p);
     return EB_OK;

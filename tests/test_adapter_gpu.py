@@ -259,3 +259,23 @@ def test_output_rows_of_any_stride(new, dtype):
     want, tol = c.delta()
     y, size = c.x.double() @ c.w.double().T, c.x.double().abs() @ c.w.double().abs().T
     close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 256 / 16 + 2.0 ** -20) * size)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new", [[3, 1], [60, 20]])
+def test_the_shared_projection_of_a_padded_batch(new, dtype):
+    """Many rows in front of the first sequence and behind the last: x W^T + bias there, rounded once."""
+    from energonai_b200.adapter import adapter_delta, adapter_product
+    c = Case([300] + new, 128, 520, 16, 2, dtype, seed=8, pad_rows=700)
+    c.index[:] = 1
+    a, b, scales, index, starts, _ = c.device()
+    some = (a, b, scales, index[1:], starts[1:], max(new))
+    want, tol = c.delta()
+    want[:300], tol[:300] = 0, 0
+    delta = adapter_delta(c.x.cuda(), *some)
+    close(delta, want, tol)
+    assert not delta[:300].any() and not delta[c.starts[-1]:].any()
+    y = c.x.double() @ c.w.double().T + c.bias.double()
+    size = c.x.double().abs() @ c.w.double().abs().T + c.bias.double().abs()
+    got = adapter_product(c.x.cuda(), c.w.cuda(), *some, bias=c.bias.cuda())
+    close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 128 / 16 + 2.0 ** -20) * size)
