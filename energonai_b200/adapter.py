@@ -39,9 +39,12 @@ def _adapters(what, x, a, b, scales, index, starts, most_new, base=None, out=Non
     if index.dtype is not torch.int32 or starts.dtype is not torch.int32 or index.dim() != 1 or starts.shape != (batch + 1,) or batch == 0 or not (
             index.is_contiguous() and starts.is_contiguous()):
         raise RuntimeError(f"{what}: int32 index [batch] and starts [batch + 1] required")
-    rows, columns, most_new = shape[0], to[1], int(most_new) or 1        # (0: zeros are all that is asked for)
+    rows, columns, most_new = shape[0], to[1], int(most_new)
     ldx = _rows(what, x, width, dtype)
     given, out = out, out if out is not None and out.stride(0) % 8 == 0 else x.new_empty((rows, columns))
+    if most_new == 0:                                                    # (no row has an adapter)
+        nothing = x.new_zeros((rows, columns)) if base is None else base().to(dtype)
+        return nothing if given is None else given.copy_(nothing)
     nbytes = _scratch_bytes(rows, width, rank, batch, most_new)
     scratch = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None       # (of this call: captured calls share none)
     of, sequences = (x.data_ptr(), ldx, a.data_ptr()), (index.data_ptr(), starts.data_ptr())

@@ -279,3 +279,18 @@ def test_the_shared_projection_of_a_padded_batch(new, dtype):
     size = c.x.double().abs() @ c.w.double().abs().T + c.bias.double().abs()
     got = adapter_product(c.x.cuda(), c.w.cuda(), *some, bias=c.bias.cuda())
     close(got, y + want, UNIT[dtype] * (y + want).abs() + tol + (2.0 ** -23 * 128 / 16 + 2.0 ** -20) * size)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_nothing_is_announced(dtype):
+    from energonai_b200.adapter import adapter_delta, adapter_product
+    c = Case([5, 2], 128, 264, 16, 2, dtype, seed=3, pad_rows=1)
+    c.index[:] = 1
+    c.most_new = 0
+    assert not adapter_delta(c.x.cuda(), *c.device()).any()
+    y, size = c.x.double() @ c.w.double().T, c.x.double().abs() @ c.w.double().abs().T
+    out = torch.full((c.rows, 264), 3.0, dtype=dtype, device="cuda")
+    for given in (None, out):
+        got = adapter_product(c.x.cuda(), c.w.cuda(), *c.device(), out=given)
+        close(got, y, UNIT[dtype] * y.abs() + (2.0 ** -23 * 128 / 16 + 2.0 ** -20) * size)
+    assert got.data_ptr() == out.data_ptr()
